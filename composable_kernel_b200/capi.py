@@ -17,7 +17,9 @@ LIB_PATH = os.environ.get("CKB200_LIB") or os.path.join(HERE, "lib", "libckb200.
 # ---- enums (include/ckb200.h) -------------------------------------------------------------------
 CKB_OK, CKB_ERR_UNSUPPORTED, CKB_ERR_INVALID, CKB_ERR_CUDA, CKB_ERR_DEVICE, CKB_ERR_WORKSPACE, \
     CKB_ERR_LIMIT = range(7)
-CKB_F16, CKB_I8, CKB_BF16 = 0, 1, 2
+CKB_F16, CKB_I8, CKB_BF16, CKB_F32, CKB_F8_E4M3, CKB_F8_E5M2 = range(6)
+CKB_GROUP_ROWS, CKB_GROUP_K_BLOCKS = 0, 1
+CKB_SCALED_MAX_GROUPS = 1024
 CKB_ROW_MAJOR, CKB_COL_MAJOR = 0, 1
 (CKB_EPI_PASSTHROUGH, CKB_EPI_SCALE, CKB_EPI_RELU, CKB_EPI_FASTGELU, CKB_EPI_ADD,
  CKB_EPI_ADD_RELU_F16, CKB_EPI_BILINEAR, CKB_EPI_ADD_ADD_FASTGELU, CKB_EPI_ADD_RELU_ADD,
@@ -32,6 +34,12 @@ def tile_config(bn: int = 0, cg: int = 0, no_ksplit: int = 0, kbatch: int = 0, b
     """CKB_TILE_CONFIG(bn, cg, no_ksplit) / CKB_TILE_CONFIG_KBATCH(bn, cg, kbatch) / CKB_TILE_CONFIG_BALANCED(bn, cg)
     of include/ckb200.h; 0 = the library's own choice."""
     return bn | (cg << 12) | (no_ksplit << 16) | (balanced << 17) | (kbatch << 20)
+
+
+def scaled_tile(cols: int, cg: int, swap: int = 0, ksplit: int = 0) -> int:
+    """CKB_SCALED_TILE(cols, cg, swap, ksplit) of include/ckb200.h."""
+    return cols | (cg << 12) | (swap << 16) | (ksplit << 20)
+
 
 EPI_NUM_D = {CKB_EPI_ADD: 1, CKB_EPI_ADD_RELU_F16: 1, CKB_EPI_BILINEAR: 1, CKB_EPI_ADD_RELU: 1,
              CKB_EPI_ADD_HARDSWISH: 1, CKB_EPI_ADD_ADD_FASTGELU: 2, CKB_EPI_ADD_RELU_ADD: 2}
@@ -101,6 +109,58 @@ class Conv3dFwdDesc(Structure):
     ]
 
 
+class ScaledGemmDesc(Structure):
+    """struct ckb_scaled_gemm_desc"""
+    _fields_ = [
+        ("a_dtype", c_int32), ("b_dtype", c_int32), ("e_dtype", c_int32),
+        ("a_layout", c_int32), ("b_layout", c_int32),
+        ("scale_block_m", c_int32), ("scale_block_n", c_int32), ("tile_config", c_int32),
+        ("M", c_int64), ("N", c_int64), ("K", c_int64),
+        ("lda", c_int64), ("ldb", c_int64), ("lde", c_int64),
+        ("a_scale_stride_m", c_int64), ("a_scale_stride_k", c_int64),
+        ("b_scale_stride_n", c_int64), ("b_scale_stride_k", c_int64),
+        ("p_a", c_void_p), ("p_b", c_void_p), ("p_a_scale", c_void_p), ("p_b_scale", c_void_p), ("p_e", c_void_p),
+    ]
+
+
+class ScaledGroupedGemmDesc(Structure):
+    """struct ckb_scaled_grouped_gemm_desc"""
+    _fields_ = [("gemm", ScaledGemmDesc), ("group_axis", c_int32), ("group_count", c_int32), ("p_offsets", c_void_p),
+                ("b_group_stride", c_int64), ("b_scale_group_stride", c_int64), ("e_group_stride", c_int64)]
+
+
+class BlockQuantizeDesc(Structure):
+    """struct ckb_block_quantize_desc"""
+    _fields_ = [
+        ("x_dtype", c_int32), ("q_dtype", c_int32), ("block_m", c_int32), ("block_n", c_int32),
+        ("pow2_scale", c_int32), ("pad_", c_int32),
+        ("M", c_int64), ("N", c_int64), ("ldx", c_int64), ("ldq", c_int64),
+        ("scale_stride_m", c_int64), ("scale_stride_n", c_int64),
+        ("p_x", c_void_p), ("p_q", c_void_p), ("p_scale", c_void_p),
+    ]
+
+
+class LayernormFwdDesc(Structure):
+    """struct ckb_layernorm_fwd_desc"""
+    _fields_ = [
+        ("x_dtype", c_int32), ("w_dtype", c_int32), ("q_dtype", c_int32), ("eps", c_float),
+        ("M", c_int64), ("N", c_int64), ("ldx", c_int64), ("ldy", c_int64), ("ldq", c_int64),
+        ("q_scale_stride_m", c_int64), ("q_scale_stride_n", c_int64),
+        ("p_x", c_void_p), ("p_gamma", c_void_p), ("p_beta", c_void_p), ("p_y", c_void_p), ("p_q", c_void_p),
+        ("p_q_scale", c_void_p), ("p_mean", c_void_p), ("p_rstd", c_void_p),
+    ]
+
+
+class LayernormBwdDesc(Structure):
+    """struct ckb_layernorm_bwd_desc"""
+    _fields_ = [
+        ("x_dtype", c_int32), ("w_dtype", c_int32),
+        ("M", c_int64), ("N", c_int64), ("lddy", c_int64), ("ldx", c_int64), ("lddx", c_int64),
+        ("p_dy", c_void_p), ("p_x", c_void_p), ("p_gamma", c_void_p), ("p_mean", c_void_p), ("p_rstd", c_void_p),
+        ("p_dx", c_void_p), ("p_dgamma", c_void_p), ("p_dbeta", c_void_p),
+    ]
+
+
 # name -> (restype, argtypes); every symbol include/ckb200.h declares.
 SYMBOLS = {
     "ckb_abi_version": (c_int, []),
@@ -129,6 +189,18 @@ SYMBOLS = {
     "ckb_conv2d_fwd_run": (c_int, [POINTER(Conv2dFwdDesc), c_void_p, c_int, POINTER(c_float)]),
     "ckb_conv3d_fwd_supported": (c_int, [POINTER(Conv3dFwdDesc)]),
     "ckb_conv3d_fwd_run": (c_int, [POINTER(Conv3dFwdDesc), c_void_p, c_int, POINTER(c_float)]),
+    "ckb_scaled_gemm_supported": (c_int, [POINTER(ScaledGemmDesc)]),
+    "ckb_scaled_gemm_run": (c_int, [POINTER(ScaledGemmDesc), c_void_p, c_int, POINTER(c_float)]),
+    "ckb_scaled_grouped_gemm_supported": (c_int, [POINTER(ScaledGroupedGemmDesc)]),
+    "ckb_scaled_grouped_gemm_run": (c_int, [POINTER(ScaledGroupedGemmDesc), c_void_p, c_int, POINTER(c_float)]),
+    "ckb_block_quantize_supported": (c_int, [POINTER(BlockQuantizeDesc)]),
+    "ckb_block_quantize_run": (c_int, [POINTER(BlockQuantizeDesc), c_void_p, c_int, POINTER(c_float)]),
+    "ckb_layernorm_fwd_supported": (c_int, [POINTER(LayernormFwdDesc)]),
+    "ckb_layernorm_fwd_run": (c_int, [POINTER(LayernormFwdDesc), c_void_p, c_int, POINTER(c_float)]),
+    "ckb_layernorm_bwd_supported": (c_int, [POINTER(LayernormBwdDesc)]),
+    "ckb_layernorm_bwd_workspace_size": (c_int, [POINTER(LayernormBwdDesc), POINTER(c_size_t)]),
+    "ckb_layernorm_bwd_run": (c_int, [POINTER(LayernormBwdDesc), c_void_p, c_size_t, c_void_p, c_int,
+                                      POINTER(c_float)]),
 }
 
 _lib = None

@@ -16,6 +16,7 @@
 #include <vector>
 
 #include "../../include/ckb200.h"
+#include "ckb_host.h"
 #include "ckb_launch.cuh"
 
 namespace {
@@ -640,6 +641,77 @@ LaunchFn find_launch(int mode, int kind, int epi)
 #undef CKB_INST
     return nullptr;
 }
+} // namespace ckb
+
+// ---- what ckb_host.h declares for the other host sides --------------------------------------------
+namespace ckb {
+
+int host_fail(int code, const char* fmt, ...)
+{
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof(buf), fmt, ap);
+    va_end(ap);
+    return fail(code, "%s", buf);
+}
+
+int host_device(HostDevice* out)
+{
+    DeviceInfo* dev = nullptr;
+    const int rc    = current_device(&dev);
+    if(rc)
+        return rc;
+    out->sm_count      = dev->sm_count;
+    out->status        = dev->status;
+    out->wait_limit_ns = wait_limit_ns();
+    return CKB_OK;
+}
+
+int host_check_pointer(const void* p, const char* what)
+{
+    if(!p)
+        return CKB_OK;
+    int dev = 0;
+    CKB_CUDA(cudaGetDevice(&dev));
+    cudaPointerAttributes at;
+    CKB_CUDA(cudaPointerGetAttributes(&at, p));
+    if(at.type == cudaMemoryTypeUnregistered)
+        return fail(CKB_ERR_INVALID, "%s is not a device pointer", what);
+    if(at.type == cudaMemoryTypeDevice && at.device != dev)
+        return fail(CKB_ERR_INVALID, "%s lies on device %d, the current device is %d", what, at.device, dev);
+    return CKB_OK;
+}
+
+int host_encode_8bit(CUtensorMap* tm, const void* ptr, int64_t rows, int64_t inner, int64_t pitch, int box_rows,
+                     int64_t batch, int64_t batch_pitch, const char* what)
+{
+    cuuint64_t dims[3]    = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(batch)};
+    cuuint64_t strides[2] = {static_cast<cuuint64_t>(pitch), static_cast<cuuint64_t>(batch_pitch)};
+    cuuint32_t box[3]     = {static_cast<cuuint32_t>(BK_BYTES), static_cast<cuuint32_t>(box_rows), 1};
+    return encode_tiled(tm, CKB_I8, batch >= 1 ? 3 : 2, ptr, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, what);
+}
+
+void host_add_pdl(cudaLaunchAttribute* attrs, int* n)
+{
+    if(!programmatic_launch_enabled())
+        return;
+    attrs[*n].id                                         = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[*n].val.programmaticStreamSerializationAllowed = 1;
+    ++*n;
+}
+
+void host_note_plan(const char* fmt, ...)
+{
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(t_last_plan, sizeof(t_last_plan), fmt, ap);
+    va_end(ap);
+}
+
+void host_count_launches(uint64_t n) { g_launches.fetch_add(n); }
+
 } // namespace ckb
 
 namespace ckb {

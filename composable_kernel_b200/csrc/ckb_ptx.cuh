@@ -349,6 +349,8 @@ CKB_MMA_SPLIT(mma_f16_ss_split, "tcgen05.mma.cta_group::1.kind::f16")
 CKB_MMA_SPLIT(mma_i8_ss_split, "tcgen05.mma.cta_group::1.kind::i8")
 CKB_MMA_SPLIT(mma_f16_ss_pair_split, "tcgen05.mma.cta_group::2.kind::f16")
 CKB_MMA_SPLIT(mma_i8_ss_pair_split, "tcgen05.mma.cta_group::2.kind::i8")
+CKB_MMA_SPLIT(mma_f8_ss_split, "tcgen05.mma.cta_group::1.kind::f8f6f4")
+CKB_MMA_SPLIT(mma_f8_ss_pair_split, "tcgen05.mma.cta_group::2.kind::f8f6f4")
 #undef CKB_MMA_SPLIT
 // One arrival on the barrier at offset `bar` in EACH CTA of `cta_mask` once the pair's MMAs issued
 // so far are done (only the barrier arrival fans out; no data does).
@@ -403,6 +405,69 @@ __device__ __forceinline__ void tmem_st_wait()
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
+// 8 and 16 columns; the values are read after tmem_ld_wait_regs.
+__device__ __forceinline__ void tmem_ld_32x32b_x8(uint32_t taddr, uint32_t* v)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                 : "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t* v)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+                 "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+                   "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                 : "r"(taddr)
+                 : "memory");
+}
+// Waits for this warp's loads.  The registers pass through the instruction, so that no use of them can be moved
+// above it.
+__device__ __forceinline__ void tmem_ld_wait_regs8(uint32_t* v)
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7])::"memory");
+}
+__device__ __forceinline__ void tmem_ld_wait_regs16(uint32_t* v)
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
+                   "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]),
+                   "+r"(v[15])::"memory");
+}
+
+// Values of a load that an earlier wait covers: no use of them is moved above this point.
+__device__ __forceinline__ void keep_regs16(uint32_t* v)
+{
+    asm volatile("" : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
+                      "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]));
+}
+
+// ---- packed 32-bit arithmetic: two values per instruction -----------------------------------------
+__device__ __forceinline__ uint64_t pack_f32x2(float lo, float hi)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpack_f32x2(uint64_t v, float& lo, float& hi)
+{
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 // ---- descriptors ------------------------------------------------------------------------------
 // Shared-memory matrix descriptor for a K-major operand tile stored as rows of 128 bytes with
 // the 128-byte swizzle (what a TMA box of 128 inner bytes with SWIZZLE_128B produces):
@@ -443,7 +508,8 @@ __device__ __forceinline__ uint64_t make_smem_desc_mn_sw128(uint32_t smem_addr, 
 
 // Instruction descriptor for tcgen05.mma kind::f16 / kind::i8:
 //   bits 4-5 accumulator format (1 = f32, 2 = s32); bits 7-9 A format; bits 10-12 B format
-//   (f16 kind: 0 = f16, 1 = bf16; i8 kind: 0 = u8, 1 = s8); bit 15 / 16 A / B major (0 = K, 1 = MN);
+//   (f16 kind: 0 = f16, 1 = bf16; i8 kind: 0 = u8, 1 = s8; f8f6f4 kind: 0 = e4m3, 1 = e5m2, A and B independently);
+//   bit 15 / 16 A / B major (0 = K, 1 = MN);
 //   bits 17-22 N >> 3; bits 24-28 M >> 4.
 __host__ __device__ constexpr uint32_t make_idesc(uint32_t c_fmt, uint32_t ab_fmt, uint32_t m,
                                                   uint32_t n, uint32_t a_mn_major = 0, uint32_t b_mn_major = 0)

@@ -14,7 +14,8 @@ from dataclasses import dataclass, field
 from typing import List, Optional, Sequence
 
 from . import capi
-from .capi import (CKB_COL_MAJOR, CKB_F16, CKB_I8, CKB_ROW_MAJOR, Conv2dFwdDesc, GemmDesc,
+from .capi import (CKB_BF16, CKB_COL_MAJOR, CKB_F16, CKB_F32, CKB_F8_E4M3, CKB_F8_E5M2,  # noqa: F401
+                   CKB_GROUP_K_BLOCKS, CKB_GROUP_ROWS, CKB_I8, CKB_ROW_MAJOR, Conv2dFwdDesc, GemmDesc,
                    GroupedGemmDesc)
 
 
@@ -443,6 +444,184 @@ class DeviceConvFwd(BaseOperator):
 
     def GetTypeString(self) -> str:
         return "DeviceConvNdFwd_B200_Tcgen05_Im2colTma<128, 256|128|64, 128B>"
+
+
+class DescArgument(BaseArgument):
+    """Argument of the operations below: the C descriptor and what a call needs besides it."""
+
+    def __init__(self, desc):
+        super().__init__()
+        self.desc = desc
+        self.ref = ctypes.byref(desc)
+        self.ms = ctypes.c_float(0.0)
+        self.ms_ref = ctypes.byref(self.ms)
+
+
+class _DescOperator(BaseOperator):
+    """Operations whose argument is one C descriptor: ``ckb_<_name>_supported`` and ``ckb_<_name>_run``."""
+    _name = ""
+
+    def IsSupportedArgument(self, arg: DescArgument) -> bool:
+        return getattr(capi.lib(), f"ckb_{self._name}_supported")(arg.ref) == capi.CKB_OK
+
+    def _launch(self, arg: DescArgument, stream, n_rep: int) -> int:
+        return getattr(capi.lib(), f"ckb_{self._name}_run")(arg.ref, stream, n_rep, arg.ms_ref)
+
+    def _run(self, arg: DescArgument, sc: StreamConfig) -> float:
+        rc = self._launch(arg, sc.stream_id, sc.nrepeat if sc.time_kernel else 0)
+        if rc != capi.CKB_OK:
+            msg = capi.last_error()
+            if rc in (capi.CKB_ERR_UNSUPPORTED, capi.CKB_ERR_INVALID):
+                msg = f"wrong! {type(self).__name__} has invalid setting: {msg}"
+            raise capi.CkbError(rc, msg)
+        return arg.ms.value
+
+
+def _ptr(p):
+    return int(p) if p else None
+
+
+class DeviceGemmABScale(_DescOperator):
+    """E = (A * scale) (B * scale) with 8-bit A and B: a 32-bit scale for every ``scale_block_m`` rows x 128 K values of A
+    and for every 128 K values x ``scale_block_n`` columns of B (1 or 128 each).
+
+    ``a_dtype`` / ``b_dtype``: CKB_F8_E4M3 or CKB_F8_E5M2, ``e_dtype``: CKB_BF16, CKB_F16 or CKB_F32; layouts as for
+    DeviceGemm.  ``AScaleStrides`` = (elements from one block of rows of A to the next, from one K block to the next),
+    ``BScaleStrides`` = (from one block of columns of B to the next, from one K block to the next)."""
+    _name = "scaled_gemm"
+
+    def __init__(self, a_dtype=CKB_F8_E4M3, b_dtype=CKB_F8_E4M3, e_dtype=CKB_BF16, a_layout=CKB_ROW_MAJOR,
+                 b_layout=CKB_COL_MAJOR, scale_block_m=1, scale_block_n=128, tile_config=0):
+        self.a_dtype, self.b_dtype, self.e_dtype = a_dtype, b_dtype, e_dtype
+        self.a_layout, self.b_layout = a_layout, b_layout
+        self.scale_block_m, self.scale_block_n, self.tile_config = scale_block_m, scale_block_n, tile_config
+
+    def _fill(self, d, p_a, p_b, p_a_scale, p_b_scale, p_e, M, N, K, StrideA, StrideB, StrideE, AScaleStrides, BScaleStrides):
+        d.a_dtype, d.b_dtype, d.e_dtype = self.a_dtype, self.b_dtype, self.e_dtype
+        d.a_layout, d.b_layout = self.a_layout, self.b_layout
+        d.scale_block_m, d.scale_block_n, d.tile_config = self.scale_block_m, self.scale_block_n, self.tile_config
+        d.M, d.N, d.K = int(M), int(N), int(K)
+        d.lda, d.ldb, d.lde = int(StrideA), int(StrideB), int(StrideE)
+        d.a_scale_stride_m, d.a_scale_stride_k = (int(v) for v in AScaleStrides)
+        d.b_scale_stride_n, d.b_scale_stride_k = (int(v) for v in BScaleStrides)
+        d.p_a, d.p_b, d.p_a_scale, d.p_b_scale, d.p_e = _ptr(p_a), _ptr(p_b), _ptr(p_a_scale), _ptr(p_b_scale), _ptr(p_e)
+
+    def MakeArgument(self, p_a, p_b, p_a_scale, p_b_scale, p_e, M, N, K, StrideA, StrideB, StrideE, AScaleStrides,
+                     BScaleStrides) -> DescArgument:
+        arg = DescArgument(capi.ScaledGemmDesc())
+        self._fill(arg.desc, p_a, p_b, p_a_scale, p_b_scale, p_e, M, N, K, StrideA, StrideB, StrideE, AScaleStrides,
+                   BScaleStrides)
+        return arg
+
+    MakeArgumentPointer = MakeArgument
+
+    def GetTypeString(self) -> str:
+        return "DeviceGemmABScale_B200_Tcgen05<128, 16..256, 128B>"
+
+
+class DeviceGroupedGemmABScale(DeviceGemmABScale):
+    """DeviceGemmABScale over groups whose extents only the device knows: ``p_offsets`` is a device array of
+    ``group_count`` + 1 non-decreasing int32.
+
+    ``group_axis`` CKB_GROUP_ROWS: group g owns rows offsets[g] .. offsets[g + 1] of A and E and its own B, ``GroupStrideB``
+    elements (scales: ``GroupStrideBScale``) apart; rows outside every group are left alone.  CKB_GROUP_K_BLOCKS: group g owns
+    the K blocks offsets[g] .. offsets[g + 1] of A and B and its own matrix of E, ``GroupStrideE`` elements apart; a group
+    without blocks gets zeros."""
+    _name = "scaled_grouped_gemm"
+
+    def __init__(self, group_axis=CKB_GROUP_ROWS, *args, **kwargs):
+        super().__init__(*args, **kwargs)
+        self.group_axis = group_axis
+
+    def MakeArgument(self, p_a, p_b, p_a_scale, p_b_scale, p_e, p_offsets, group_count, M, N, K, StrideA, StrideB, StrideE,
+                     AScaleStrides, BScaleStrides, GroupStrideB=0, GroupStrideBScale=0, GroupStrideE=0) -> DescArgument:
+        arg = DescArgument(capi.ScaledGroupedGemmDesc())
+        d = arg.desc
+        self._fill(d.gemm, p_a, p_b, p_a_scale, p_b_scale, p_e, M, N, K, StrideA, StrideB, StrideE, AScaleStrides,
+                   BScaleStrides)
+        d.group_axis, d.group_count, d.p_offsets = self.group_axis, int(group_count), _ptr(p_offsets)
+        d.b_group_stride, d.b_scale_group_stride, d.e_group_stride = int(GroupStrideB), int(GroupStrideBScale), int(GroupStrideE)
+        return arg
+
+    MakeArgumentPointer = MakeArgument
+
+    def GetTypeString(self) -> str:
+        return "DeviceGroupedGemmABScale_B200_Tcgen05<128, 16..256, 128B>"
+
+
+class DeviceBlockQuantize(_DescOperator):
+    """X (M x N, row-major) -> 8-bit values and a 32-bit scale per block of ``block_m`` x ``block_n`` (1 x 128, 128 x 1 or
+    128 x 128): scale = largest magnitude / largest 8-bit value (the next power of two with ``pow2_scale``), q = x / scale.
+    ``ScaleStrides`` = (elements from one block of rows to the next, from one block of columns to the next)."""
+    _name = "block_quantize"
+
+    def __init__(self, x_dtype=CKB_BF16, q_dtype=CKB_F8_E4M3, block_m=1, block_n=128, pow2_scale=False):
+        self.x_dtype, self.q_dtype, self.block_m, self.block_n = x_dtype, q_dtype, block_m, block_n
+        self.pow2_scale = pow2_scale
+
+    def MakeArgument(self, p_x, p_q, p_scale, M, N, StrideX, StrideQ, ScaleStrides) -> DescArgument:
+        arg = DescArgument(capi.BlockQuantizeDesc())
+        d = arg.desc
+        d.x_dtype, d.q_dtype, d.block_m, d.block_n = self.x_dtype, self.q_dtype, self.block_m, self.block_n
+        d.pow2_scale = int(self.pow2_scale)
+        d.M, d.N, d.ldx, d.ldq = int(M), int(N), int(StrideX), int(StrideQ)
+        d.scale_stride_m, d.scale_stride_n = (int(v) for v in ScaleStrides)
+        d.p_x, d.p_q, d.p_scale = _ptr(p_x), _ptr(p_q), _ptr(p_scale)
+        return arg
+
+    MakeArgumentPointer = MakeArgument
+
+
+class DeviceLayernormFwd(_DescOperator):
+    """Layer norm over the rows of X: y = (x - mean) * rstd * gamma + beta, to ``x_dtype`` (``p_y``) and (or) to 8-bit blocks of
+    1 x 128 (``p_q``, ``p_q_scale``), the operand of the next DeviceGemmABScale.  ``p_gamma``, ``p_beta`` (``w_dtype``),
+    ``p_mean`` and ``p_rstd`` may be None."""
+    _name = "layernorm_fwd"
+
+    def __init__(self, x_dtype=CKB_BF16, w_dtype=CKB_F32, q_dtype=CKB_F8_E4M3):
+        self.x_dtype, self.w_dtype, self.q_dtype = x_dtype, w_dtype, q_dtype
+
+    def MakeArgument(self, p_x, p_gamma, p_beta, p_y, p_mean, p_rstd, M, N, StrideX, StrideY, eps, p_q=None, p_q_scale=None,
+                     StrideQ=0, QScaleStrides=(0, 0)) -> DescArgument:
+        arg = DescArgument(capi.LayernormFwdDesc())
+        d = arg.desc
+        d.x_dtype, d.w_dtype, d.q_dtype, d.eps = self.x_dtype, self.w_dtype, self.q_dtype, float(eps)
+        d.M, d.N, d.ldx, d.ldy, d.ldq = int(M), int(N), int(StrideX), int(StrideY), int(StrideQ)
+        d.q_scale_stride_m, d.q_scale_stride_n = (int(v) for v in QScaleStrides)
+        d.p_x, d.p_gamma, d.p_beta, d.p_y = _ptr(p_x), _ptr(p_gamma), _ptr(p_beta), _ptr(p_y)
+        d.p_q, d.p_q_scale, d.p_mean, d.p_rstd = _ptr(p_q), _ptr(p_q_scale), _ptr(p_mean), _ptr(p_rstd)
+        return arg
+
+    MakeArgumentPointer = MakeArgument
+
+
+class DeviceLayernormBwd(_DescOperator):
+    """Gradients of layer norm: dx, dgamma, dbeta from dy, x and the forward's mean and rstd (any of the three may be None).
+    The workspace contract is that of DeviceGroupedGemm."""
+    _name = "layernorm_bwd"
+
+    def __init__(self, x_dtype=CKB_BF16, w_dtype=CKB_F32):
+        self.x_dtype, self.w_dtype = x_dtype, w_dtype
+
+    def MakeArgument(self, p_dy, p_x, p_gamma, p_mean, p_rstd, p_dx, p_dgamma, p_dbeta, M, N, StrideDY, StrideX,
+                     StrideDX) -> DescArgument:
+        arg = DescArgument(capi.LayernormBwdDesc())
+        d = arg.desc
+        d.x_dtype, d.w_dtype = self.x_dtype, self.w_dtype
+        d.M, d.N, d.lddy, d.ldx, d.lddx = int(M), int(N), int(StrideDY), int(StrideX), int(StrideDX)
+        d.p_dy, d.p_x, d.p_gamma, d.p_mean, d.p_rstd = _ptr(p_dy), _ptr(p_x), _ptr(p_gamma), _ptr(p_mean), _ptr(p_rstd)
+        d.p_dx, d.p_dgamma, d.p_dbeta = _ptr(p_dx), _ptr(p_dgamma), _ptr(p_dbeta)
+        return arg
+
+    MakeArgumentPointer = MakeArgument
+
+    def GetWorkSpaceSize(self, arg: DescArgument) -> int:
+        n = ctypes.c_size_t(0)
+        capi.check(capi.lib().ckb_layernorm_bwd_workspace_size(arg.ref, ctypes.byref(n)))
+        return int(n.value)
+
+    def _launch(self, arg: DescArgument, stream, n_rep: int) -> int:
+        return capi.lib().ckb_layernorm_bwd_run(arg.ref, arg.p_workspace_, arg.workspace_bytes_ or 0, stream, n_rep, arg.ms_ref)
 
 
 def device_status() -> int:

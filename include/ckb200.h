@@ -43,7 +43,10 @@ enum {
 enum {
     CKB_F16 = 0, /* IEEE binary16  (ck::half_t, utility/data_type.hpp:11)     */
     CKB_I8  = 1, /* int8_t, int32 accumulate                                   */
-    CKB_BF16 = 2 /* bfloat16 (ck::bhalf_t, utility/data_type.hpp:10)           */
+    CKB_BF16 = 2, /* bfloat16 (ck::bhalf_t, utility/data_type.hpp:10)          */
+    CKB_F32 = 3,     /* IEEE binary32: results, scales, layer norm                 */
+    CKB_F8_E4M3 = 4, /* 8-bit float, 4 exponent bits, largest value 448, no infinity   */
+    CKB_F8_E5M2 = 5  /* 8-bit float, 5 exponent bits, largest value 57344              */
 };
 
 /* ---- matrix layouts (tensor_layout::gemm, device/tensor_layout.hpp:13-25).
@@ -301,6 +304,150 @@ typedef struct ckb_conv3d_fwd_desc {
 
 int ckb_conv3d_fwd_supported(const ckb_conv3d_fwd_desc* desc);
 int ckb_conv3d_fwd_run(const ckb_conv3d_fwd_desc* desc, void* stream, int n_rep, float* avg_ms);
+
+/* ---- 8-bit products with block scales ------------------------------------------------------------
+ * E[m,n] = sum over K blocks kb of 128:  SA[m / scale_block_m, kb] * SB[n / scale_block_n, kb] *
+ *                                        sum over k in kb of A[m,k] * B[k,n]
+ * A and B hold 8-bit floats (e4m3 or e5m2, each its own), SA and SB 32-bit scales, E is bf16, f16 or f32.  Products
+ * and sums of a block are 32-bit on the tensor cores; the scaled blocks are added in 32 bits and E is rounded once.
+ * (The pair of scales is multiplied first: scales whose product is subnormal lose bits.)
+ * Layouts as for the plain GEMM, so a layer's three products are all here: forward (A row-major, B column-major, blocks
+ * 1 x 128 and 128 x 128), the input's gradient (B row-major) and the weights' gradient (A column-major, B row-major,
+ * both with a scale per column and 128 tokens).  M, N and K are arbitrary; base and pitch of A and B are multiples of
+ * 16 bytes.  A scale stride may be 0 (one scale for a whole row of blocks or a whole tensor). */
+typedef struct ckb_scaled_gemm_desc {
+    int32_t a_dtype, b_dtype;    /* CKB_F8_E4M3 / CKB_F8_E5M2                            */
+    int32_t e_dtype;             /* CKB_BF16 / CKB_F16 / CKB_F32                          */
+    int32_t a_layout, b_layout;  /* as ckb_gemm_desc; E is row-major                      */
+    int32_t scale_block_m;       /* rows of A per scale: 1 or 128                         */
+    int32_t scale_block_n;       /* columns of B per scale: 1 or 128                      */
+    int32_t tile_config;         /* 0 or CKB_SCALED_TILE(...)                             */
+    int64_t M, N, K;
+    int64_t lda, ldb, lde;       /* leading dimensions in elements                       */
+    int64_t a_scale_stride_m;    /* elements from the scale of one block of rows of A to the next   */
+    int64_t a_scale_stride_k;    /* ... from one K block to the next                                */
+    int64_t b_scale_stride_n;
+    int64_t b_scale_stride_k;
+    const void* p_a;
+    const void* p_b;
+    const float* p_a_scale;
+    const float* p_b_scale;
+    void* p_e;
+} ckb_scaled_gemm_desc;
+
+/* Pins the tile of an 8-bit product: `cols` columns of the narrower tile side and `cg` CTAs per tile.
+ *   cg = 2  a CTA pair on 256 x cols, cols = 64, 96 .. 256; `swap` = 1 puts the columns of B on the 256 side
+ *   cg = 1  128 columns of B x cols rows of A, cols = 16, 32, 64 or 128; ksplit = 2, 4 or 8 cuts K over a cluster
+ *           of as many CTAs (plain products only; slices of two K blocks at least)
+ * 0 leaves the choice to the library; a pin that the problem cannot use is refused. */
+#define CKB_SCALED_TILE(cols, cg, swap, ksplit) ((cols) | ((cg) << 12) | ((swap) << 16) | ((ksplit) << 20))
+
+int ckb_scaled_gemm_supported(const ckb_scaled_gemm_desc* desc);
+/* n_rep / avg_ms as ckb_gemm_run.  Uses no scratch and allocates nothing: it may be captured into a graph (after one
+ * call on the device outside a capture). */
+int ckb_scaled_gemm_run(const ckb_scaled_gemm_desc* desc, void* stream, int n_rep, float* avg_ms);
+
+/* The same over groups (the experts of a layer) whose extents are known on the device only.  `offsets` is a device
+ * array of group_count + 1 non-decreasing int32.
+ *   CKB_GROUP_ROWS      group g multiplies rows offsets[g] .. offsets[g+1] of A (gemm.M rows in all, row-major,
+ *                       scale_block_m = 1) with its own B (b_group_stride elements apart) into the same rows of E.
+ *                       Rows of E outside every group are left as they were.
+ *   CKB_GROUP_K_BLOCKS  group g multiplies the K blocks offsets[g] .. offsets[g+1] of A and B (gemm.K in all) into its
+ *                       own M x N matrix of E (e_group_stride elements apart): the experts' weight gradients.  A group
+ *                       without blocks gets zeros.
+ * Offsets are clipped to the extent they index, so no value of theirs makes a kernel leave the tensors. */
+enum { CKB_GROUP_ROWS = 0, CKB_GROUP_K_BLOCKS = 1 };
+#define CKB_SCALED_MAX_GROUPS 1024
+typedef struct ckb_scaled_grouped_gemm_desc {
+    ckb_scaled_gemm_desc gemm;
+    int32_t group_axis;          /* CKB_GROUP_ROWS / CKB_GROUP_K_BLOCKS                   */
+    int32_t group_count;         /* 1 .. CKB_SCALED_MAX_GROUPS                            */
+    const int32_t* p_offsets;
+    int64_t b_group_stride;      /* CKB_GROUP_ROWS: multiple of 16                        */
+    int64_t b_scale_group_stride;
+    int64_t e_group_stride;      /* CKB_GROUP_K_BLOCKS                                    */
+} ckb_scaled_grouped_gemm_desc;
+
+int ckb_scaled_grouped_gemm_supported(const ckb_scaled_grouped_gemm_desc* desc);
+int ckb_scaled_grouped_gemm_run(const ckb_scaled_grouped_gemm_desc* desc, void* stream, int n_rep, float* avg_ms);
+
+/* ---- block quantizer: the operands of the 8-bit products -------------------------------------------
+ * X (M x N, row-major) is cut into blocks of block_m x block_n (1 x 128, 128 x 1 or 128 x 128; the last ones may be
+ * smaller).  With amax = the largest magnitude of a block and qmax = 448 (e4m3) or 57344 (e5m2):
+ *   scale = amax / qmax rounded to 32 bits, at least 2^-126; 1 for a block of zeros; with pow2_scale the next power of
+ *           two that is not below it
+ *   q     = x / scale rounded to the nearest 8-bit value (ties to even), limited to +-qmax
+ * An infinity makes the scale of its block infinite, a NaN makes it NaN: every value of such a block reads back as NaN.
+ * The input is never altered.  q may start anywhere and have any pitch (16-byte ones are faster). */
+typedef struct ckb_block_quantize_desc {
+    int32_t x_dtype;             /* CKB_BF16 / CKB_F16 / CKB_F32                          */
+    int32_t q_dtype;             /* CKB_F8_E4M3 / CKB_F8_E5M2                             */
+    int32_t block_m, block_n;
+    int32_t pow2_scale;          /* 0 or 1                                                */
+    int32_t pad_;                /* 0                                                     */
+    int64_t M, N;
+    int64_t ldx, ldq;            /* row pitches in elements                               */
+    int64_t scale_stride_m, scale_stride_n; /* elements from one block of rows / columns to the next */
+    const void* p_x;
+    void* p_q;
+    float* p_scale;
+} ckb_block_quantize_desc;
+
+int ckb_block_quantize_supported(const ckb_block_quantize_desc* desc);
+int ckb_block_quantize_run(const ckb_block_quantize_desc* desc, void* stream, int n_rep, float* avg_ms);
+
+/* ---- layer norm -----------------------------------------------------------------------------------
+ * Over the N values of each of M rows, statistics in 32 bits:
+ *   mean = sum x / N,  rstd = 1 / sqrt(sum (x - mean)^2 / N + eps),  y = (x - mean) * rstd * gamma + beta
+ * Y is written as x_dtype (p_y) and (or) as 8-bit blocks of 1 x 128 of the unrounded y (p_q, p_q_scale, as the block
+ * quantizer makes them); at least one of the two.  gamma and beta (w_dtype: x_dtype or CKB_F32) may be null (1 and 0),
+ * p_mean and p_rstd (M 32-bit values each) may be null. */
+typedef struct ckb_layernorm_fwd_desc {
+    int32_t x_dtype;             /* CKB_BF16 / CKB_F16 / CKB_F32                          */
+    int32_t w_dtype;             /* x_dtype or CKB_F32                                    */
+    int32_t q_dtype;             /* CKB_F8_E4M3 / CKB_F8_E5M2 (read when p_q is set)      */
+    float eps;                   /* >= 0                                                  */
+    int64_t M, N;
+    int64_t ldx, ldy, ldq;       /* row pitches in elements                               */
+    int64_t q_scale_stride_m, q_scale_stride_n;
+    const void* p_x;
+    const void* p_gamma;
+    const void* p_beta;
+    void* p_y;
+    void* p_q;
+    float* p_q_scale;
+    float* p_mean;
+    float* p_rstd;
+} ckb_layernorm_fwd_desc;
+
+int ckb_layernorm_fwd_supported(const ckb_layernorm_fwd_desc* desc);
+int ckb_layernorm_fwd_run(const ckb_layernorm_fwd_desc* desc, void* stream, int n_rep, float* avg_ms);
+
+/* Backward pass, from the forward's x, mean and rstd.  With xhat = (x - mean) * rstd and w = dy * gamma:
+ *   dx = rstd * (w - mean of w over the row - xhat * mean of w * xhat over the row)
+ *   dgamma = sum of dy * xhat over the rows,  dbeta = sum of dy over the rows
+ * dx has x_dtype, dgamma and dbeta w_dtype.  p_gamma may be null (1); p_dx may be null (only the weights' gradients),
+ * p_dgamma and p_dbeta too (at least one of the three is set).  The sums over rows are formed in a fixed order through a
+ * device workspace of the caller (ckb_layernorm_bwd_workspace_size bytes, 16-byte aligned, nothing kept in it between
+ * calls; calls that may overlap need one each): the same inputs give the same bits. */
+typedef struct ckb_layernorm_bwd_desc {
+    int32_t x_dtype, w_dtype;
+    int64_t M, N;
+    int64_t lddy, ldx, lddx;
+    const void* p_dy;
+    const void* p_x;
+    const void* p_gamma;
+    const float* p_mean;
+    const float* p_rstd;
+    void* p_dx;
+    void* p_dgamma;
+    void* p_dbeta;
+} ckb_layernorm_bwd_desc;
+
+int ckb_layernorm_bwd_supported(const ckb_layernorm_bwd_desc* desc);
+int ckb_layernorm_bwd_workspace_size(const ckb_layernorm_bwd_desc* desc, size_t* bytes);
+int ckb_layernorm_bwd_run(const ckb_layernorm_bwd_desc* desc, void* workspace, size_t workspace_bytes, void* stream,
+                          int n_rep, float* avg_ms);
 
 /* ---- device memory helpers (DeviceMem, library/src/host_tensor/device_memory.cpp:7-28) */
 int ckb_malloc(void** dev_ptr, size_t bytes);
