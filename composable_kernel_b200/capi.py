@@ -36,9 +36,9 @@ def tile_config(bn: int = 0, cg: int = 0, no_ksplit: int = 0, kbatch: int = 0, b
     return bn | (cg << 12) | (no_ksplit << 16) | (balanced << 17) | (kbatch << 20)
 
 
-def scaled_tile(cols: int, cg: int, swap: int = 0, ksplit: int = 0) -> int:
-    """CKB_SCALED_TILE(cols, cg, swap, ksplit) of include/ckb200.h."""
-    return cols | (cg << 12) | (swap << 16) | (ksplit << 20)
+def scaled_tile(cols: int, cg: int, ksplit: int = 0) -> int:
+    """CKB_SCALED_TILE(cols, cg, ksplit) of include/ckb200.h."""
+    return cols | (cg << 12) | (ksplit << 20)
 
 
 EPI_NUM_D = {CKB_EPI_ADD: 1, CKB_EPI_ADD_RELU_F16: 1, CKB_EPI_BILINEAR: 1, CKB_EPI_ADD_RELU: 1,

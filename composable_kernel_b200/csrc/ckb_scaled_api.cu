@@ -60,12 +60,10 @@ int check_scaled(const ScaledProblem& q, bool need_pointers)
         else if(q.e_group < 0 || (q.groups > 1 && q.e_group < (d.M - 1) * d.lde + d.N))
             return host_fail(CKB_ERR_INVALID, "e_group_stride is smaller than a matrix of E");
     }
-    const int cols = d.tile_config & 0xFFF, cg = (d.tile_config >> 12) & 0xF, swap = (d.tile_config >> 16) & 1;
-    const int ks = (d.tile_config >> 20) & 0xF;
-    if(d.tile_config < 0 || (d.tile_config & ~0xF1FFFF) != 0 || cg > 2 || (d.tile_config != 0 && (cols == 0 || cg == 0)) ||
-       !(ks == 0 || ks == 1 || ks == 2 || ks == 4 || ks == 8) || (cg == 1 && swap == 1))
+    const int cols = d.tile_config & 0xFFF, cg = (d.tile_config >> 12) & 0xF, ks = (d.tile_config >> 20) & 0xF;
+    if(d.tile_config < 0 || (d.tile_config & ~0xF0FFFF) != 0 || cg > 2 || (d.tile_config != 0 && (cols == 0 || cg == 0)) ||
+       !(ks == 0 || ks == 1 || ks == 2 || ks == 4 || ks == 8))
         return host_fail(CKB_ERR_INVALID, "tile_config 0x%x is not a CKB_SCALED_TILE value", d.tile_config);
-    (void)cols;
     if(need_pointers)
     {
         if(!d.p_a || !d.p_b || !d.p_a_scale || !d.p_b_scale || !d.p_e || (q.mode != SCALED_PLAIN && !q.offsets))
@@ -96,7 +94,7 @@ int cluster_caps(const HostDevice& dev, int (&cap)[3])
             ScaledParams p;
             memset(&p, 0, sizeof(p));
             int n = 0;
-            if(launch_scaled<0>(128, 1, p, (2 << i) * 64, nullptr, 2 << i, &n) != cudaSuccess)
+            if(launch_scaled<0, 1>(128, p, (2 << i) * 64, nullptr, 2 << i, &n) != cudaSuccess)
             {
                 cudaGetLastError();
                 n = 0;
@@ -131,7 +129,6 @@ bool plan_problem(const ScaledProblem& q, int sm_count, const int (&cap)[3], Sca
     {
         in.cols   = d.tile_config & 0xFFF;
         in.cg     = (d.tile_config >> 12) & 0xF;
-        in.swap   = in.cg == 1 ? 1 : (d.tile_config >> 16) & 1;
         in.ksplit = (d.tile_config >> 20) & 0xF;
         if(in.ksplit == 0)
             in.ksplit = 1;
@@ -224,12 +221,13 @@ int scaled_run(const ScaledProblem& q, void* stream_, int n_rep, float* avg_ms)
     p.offsets       = q.offsets;
     p.wait_limit_ns = dev.wait_limit_ns;
     p.status        = dev.status;
-    const int vmode = scaled_vmode(swapped ? d.scale_block_n : d.scale_block_m, swapped ? d.scale_block_m : d.scale_block_n);
-    auto* fn        = vmode == 0 ? &launch_scaled<0> : vmode == 1 ? &launch_scaled<1> : &launch_scaled<2>;
+    const int vmode = scaled_vmode(swapped ? d.scale_block_m : d.scale_block_n);
+    auto* fn        = plan.cg == 1 ? (vmode == 0 ? &launch_scaled<0, 1> : &launch_scaled<1, 1>)
+                                   : (vmode == 0 ? &launch_scaled<0, 2> : &launch_scaled<1, 2>);
     host_note_plan("scaled%s tile=%dx%d cg=%d swapped=%d grid=%d ksplit=%d vmode=%d", rows ? " rows" : q.mode == SCALED_GROUP_K ? " kblocks" : "",
                    plan.t.u_rows, plan.t.width, plan.cg, plan.t.swapped, plan.grid, plan.t.ksplit, vmode);
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-    return host_run_timed([&]() { return fn(plan.t.width, plan.cg, p, plan.grid, stream, 0, nullptr); }, 1, stream, n_rep, avg_ms);
+    return host_run_timed([&]() { return fn(plan.t.width, p, plan.grid, stream, 0, nullptr); }, 1, stream, n_rep, avg_ms);
 }
 
 ScaledProblem plain_problem(const ckb_scaled_gemm_desc* d)

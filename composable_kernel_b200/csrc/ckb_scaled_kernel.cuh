@@ -6,22 +6,22 @@
 // registers for the whole tile.
 //   warp 0     TMA producer: a ring of stages, each one K block (128 bytes of K) of the U tile (128 rows per CTA) and
 //              the V tile (BN / CG rows per CTA), 128-byte swizzle, K-major or MN-major as the operand lies
-//   warp 1     one thread issues four tcgen05.mma (kind::f8f6f4, 32 bytes of K each) per K block into one of two
-//              tensor-memory accumulators and ONE commit per K block: its barrier tells the producer that the stage is
-//              free and the epilogue warps that the accumulator is complete
-//   warps 4-11 two per lane quarter, each half of the columns: load the accumulator, release it, fused multiply-add
-//              into the sums (two values per instruction).  The scales of the next two K blocks are on their way
-//              while one is added.
-// Per 256 x 256 tile of a CTA pair and K block the tensor pipe needs 512 cycles; an epilogue warp needs four loads of
-// 32 columns and 64 packed multiply-adds, about 350, so the tensor pipe stays the limit while loads come in time
-// (32 KB per CTA and K block = 64 bytes per cycle, just under what L2 delivers to all SMs at once).
+//   warp 1     one thread issues four tcgen05.mma (kind::f8f6f4, 32 bytes of K each) per K block into one of two to four
+//              tensor-memory accumulators, with ONE wait (data there, accumulator free) and ONE commit per K block: the
+//              commit's barrier tells the producer that the stage is free and the epilogue warps that the accumulator is
+//              complete.  A wait costs this thread about 80 cycles even if nothing is waited for
+//   warps 2, 3 bring the scales into a ring in shared memory
+//   warps 4-   two or four per lane quarter, each its part of the columns: load the accumulator, release it, fused multiply-add
+//              into the sums (two values per instruction).  They issue no global loads: a hand-over behind one would
+//              wait for it (the first version, which loaded its scales itself and released the accumulator with a
+//              cluster-scope release, took 2300 cycles per K block).
+// Per 256 x 256 tile of a CTA pair and K block the tensor pipe needs 512 cycles, the copies 32 KB per CTA.
 //
 // Where the scales come from (VMODE).  A scale of the U side is one number per lane or per tile; on the V side:
 //   VMODE 0  one scale per 128 columns: a chunk of 16 columns has one factor per lane, in a register
-//   VMODE 1  one scale per column, U scale uniform over the tile: their products are staged in shared memory
-//   VMODE 2  one scale per column and one per lane: two packed operations per pair of values
+//   VMODE 1  one scale per column: two packed operations per pair of values, the second on the product of the scales
 //
-// CTA pairs (CG = 2, BN = 256): as in ckb_kernel.cuh - the leader issues tcgen05.mma.cta_group::2 for both CTAs, each
+// CTA pairs (CG = 2, BN = 128 .. 256): as in ckb_kernel.cuh - the leader issues tcgen05.mma.cta_group::2 for both CTAs, each
 // CTA loads its own 128 U rows and its own half of the V rows (no load has more than one destination), all bytes are
 // counted on the leader's barrier, the commit fans out to both.
 // Single CTAs (CG = 1, BN = 16 .. 128): U = columns of B, V = rows of A; few rows then cost few columns instead of a
@@ -62,35 +62,74 @@ struct ScaledParams
     uint32_t* status;
 };
 
-// Warps 0-3 (producer, MMA issuer, two that only take part in the barriers) form one warpgroup, the epilogue warps two
-// more, so that registers can be dealt out unevenly: 128 sums per lane (BN = 256) next to a chunk of 32 accumulator
-// columns, addresses and scales do not fit the 168 that twelve warps get at launch.  72 + 216 + 216 = 3 x 168.
+// Warps 0-3 (producer, MMA issuer, two for the scales) form one warpgroup.  Tiles of 128 columns and more have sixteen
+// epilogue warps, a quarter of the columns each: adding 128 x 256 values to the sums keeps the multiply-add pipes of an SM
+// busy for about 330 cycles, but a warp needs 680 from its wait to its last addition, mostly latency, and four warps
+// per scheduler overlap more of it than two.  20 warps get 96 registers each at launch; where 64 sums per lane need more,
+// the first warpgroup gives some of its own away (64 + 4 x 104 = 5 x 96).
 constexpr int SCALED_EPI_WARP0 = 4;
-constexpr int SCALED_THREADS   = 32 * (SCALED_EPI_WARP0 + NUM_EPI_WARPS);
-constexpr int SCALED_REGS_LOW = 72, SCALED_REGS_HIGH = 216;
-static_assert(SCALED_REGS_LOW + 2 * SCALED_REGS_HIGH == 3 * 168, "the shares add up to what the block is launched with");
+constexpr int SCALED_REGS_LOW = 64, SCALED_REGS_HIGH = 104;
 
 template <int BN, int CG>
 struct ScaledSmem
 {
+    static constexpr int EPI_WARPS   = BN >= 128 ? 16 : 8;
+    static constexpr int THREADS     = 32 * (SCALED_EPI_WARP0 + EPI_WARPS);
+    static constexpr bool SPLIT_REGS = BN >= 192;
+    static_assert(!SPLIT_REGS || SCALED_REGS_LOW + 4 * SCALED_REGS_HIGH <= 5 * 96, "shares of what the block is launched with");
     static constexpr int U_BYTES     = 128 * BK_BYTES;
-    static constexpr int V_BYTES     = (BN / CG) * BK_BYTES;
+    // (a pair's CTA always has room for 128 rows: an MN-major box is that wide whatever the tile)
+    static constexpr int V_BYTES     = (CG == 2 ? 128 : BN) * BK_BYTES;
     static constexpr int STAGE_BYTES = U_BYTES + V_BYTES;
-    // CG = 2: 4 KB per epilogue warp through which rows of E leave in whole lines.
+    // CG = 2: 2 KB per epilogue warp through which rows of E leave in whole sectors.
     // CG = 1: the slices of a K split, BN columns x 128 rows of 32 bits.
-    static constexpr int OUT_BYTES = CG == 2 ? NUM_EPI_WARPS * 4096 : BN * 512;
+    static constexpr int OUT_BYTES = CG == 2 ? EPI_WARPS * 2048 : BN * 512;
     static constexpr int STAGES    = CG == 2 ? 5 : BN == 128 ? 4 : BN == 64 ? 6 : 8;
     static constexpr int OUT_OFFSET = STAGES * STAGE_BYTES;
-    static constexpr int HALF       = BN / 2; // columns of an epilogue warp
-    static constexpr int COL_OFFSET = OUT_OFFSET + OUT_BYTES; // column scales: two buffers per epilogue warp
-    static constexpr int GRP_OFFSET = COL_OFFSET + NUM_EPI_WARPS * 2 * (HALF < 32 ? 32 : HALF) * 4;
+    static constexpr int COLS       = BN / (EPI_WARPS / 4); // columns of an epilogue warp
+    // scales: a ring of SLOTS batches of SCALE_BATCH K blocks, 128 of U and up to BN of V for each of them
+    static constexpr int SLOTS        = 2;
+    static constexpr int SCALE_BATCH  = CG == 2 ? 4 : 8; // K blocks whose scales are handed over together
+    static constexpr int V_SCALES     = BN < 32 ? 32 : BN;
+    static constexpr int SCALE_WORDS  = 128 + V_SCALES;
+    static constexpr int SCALE_OFFSET = OUT_OFFSET + OUT_BYTES;
+    static constexpr int GRP_OFFSET   = SCALE_OFFSET + SLOTS * SCALE_BATCH * SCALE_WORDS * 4;
     static constexpr int BAR_OFFSET = GRP_OFFSET + (3 * CKB_SCALED_MAX_GROUPS + 4) * 4;
-    // full[STAGES], done[STAGES], acc_empty[2], drain
-    static constexpr int NUM_BARS    = 2 * STAGES + 3;
+    // accumulators in tensor memory: as many as fit, four at most
+    static constexpr int NUM_ACC     = 4 * BN <= 512 ? 4 : 2;
+    static constexpr int ACC_COLS    = NUM_ACC * BN <= 64 ? 64 : NUM_ACC * BN <= 128 ? 128 : NUM_ACC * BN <= 256 ? 256 : 512;
+    static_assert(STAGES >= NUM_ACC, "see full_bar");
+    // full[STAGES], done[STAGES], scale_full[SLOTS], scale_empty[SLOTS], drain
+    static constexpr int NUM_BARS    = 2 * STAGES + 2 * SLOTS + 1;
     static constexpr int MISC_OFFSET = BAR_OFFSET + NUM_BARS * 8;
     static constexpr int TOTAL       = MISC_OFFSET + 16;
     static constexpr int DYN_BYTES   = TOTAL + 1024; // slack to align the base to 1024 B
 };
+
+// bounded_wait for the hand-overs of every K block: less code in the loops of the roles (their instructions have to
+// stay in the cache together), and the clock, which takes longer to read than most of these waits, only every 1024 polls.
+__device__ __forceinline__ bool block_wait(uint32_t bar, uint32_t parity, const WaitCtx& w, uint32_t code)
+{
+    uint32_t polls = 0;
+    uint64_t t0    = 0;
+    while(!mbar_try_wait(bar, parity))
+    {
+        if((++polls & 1023u) != 0)
+            continue;
+        const uint64_t now = global_timer_ns();
+        if(polls == 1024)
+            t0 = now;
+        if(*w.abort_flag != 0)
+            return false;
+        if(now - t0 > w.limit_ns || polls > (1u << 30))
+        {
+            atomicCAS(w.status, 0u, (code << 24) | (blockIdx.x & 0xFFFFFFu));
+            *w.abort_flag = 1;
+            return false;
+        }
+    }
+    return true;
+}
 
 template <typename T>
 __device__ __forceinline__ T scaled_out(float v);
@@ -110,78 +149,109 @@ __device__ __forceinline__ __nv_bfloat16 scaled_out<__nv_bfloat16>(float v)
     return __float2bfloat16_rn(v);
 }
 
-// Rows of E of one warp (32 rows x ncols columns, one row per lane in `acc`) through the warp's 4 KB of shared memory,
-// so that a store instruction writes four runs of 128 contiguous bytes instead of 32 pieces of 16 a pitch apart.
-template <typename T, int HALF>
-__device__ __forceinline__ void store_rows(const uint64_t (&acc)[HALF / 2], uint8_t* tile, T* e, int64_t lde, int row0,
-                                           int row_end, int col0, int col_end, int ncols, bool vec, int lane)
+// Rows of E leave a warp through its 2 KB of shared memory, 32 rows x 64 bytes at a time, so that a store instruction
+// writes eight runs of 64 contiguous bytes instead of pieces a pitch apart.  The 16-byte pieces of a row are permuted so
+// that neither side has bank conflicts.
+__device__ __forceinline__ uint32_t out_piece(int row, int c) { return row * 64 + ((c ^ ((row >> 1) & 3)) * 16); }
+
+// Writes one pass (columns n0 .. n0 + 64 bytes of the warp's COLS columns) to E.
+template <typename T, int COLS>
+__device__ __forceinline__ void store_pass(const uint8_t* tile, int n0, T* e, int64_t lde, int row0, int row_end, int col0,
+                                           int col_end, bool vec, int lane)
 {
-    constexpr int PER  = 16 / sizeof(T);  // values of a 16-byte piece
-    constexpr int PASS = 8 * PER;         // columns of a pass: 128 bytes
-    static_assert(HALF % PASS == 0, "a pass is 128 bytes wide");
+    constexpr int PER = 16 / sizeof(T); // values of a piece
+    const int c = lane & 3, n = n0 + c * PER;
+    if(n >= COLS)
+        return;
 #pragma unroll
-    for(int p = 0; p < HALF / PASS; ++p)
+    for(int i = 0; i < 4; ++i)
     {
-        if(p * PASS >= ncols)
-            break;
-        __syncwarp();
-#pragma unroll
-        for(int c = 0; c < 8; ++c)
+        const int r = i * 8 + (lane >> 2);
+        if(row0 + r >= row_end)
+            continue;
+        const uint4 v = *reinterpret_cast<const uint4*>(tile + out_piece(r, c));
+        T* dst        = e + static_cast<int64_t>(row0 + r) * lde + col0 + n;
+        if(vec && col0 + n + PER <= col_end)
+            *reinterpret_cast<uint4*>(dst) = v;
+        else
         {
-            alignas(16) T piece[PER];
+            const T* w = reinterpret_cast<const T*>(&v);
 #pragma unroll
-            for(int i = 0; i < PER; i += 2)
-            {
-                float lo, hi;
-                unpack_f32x2(acc[(p * PASS + c * PER + i) / 2], lo, hi);
-                piece[i]     = scaled_out<T>(lo);
-                piece[i + 1] = scaled_out<T>(hi);
-            }
-            *reinterpret_cast<uint4*>(tile + lane * 128 + ((c ^ (lane & 7)) * 16)) = *reinterpret_cast<const uint4*>(piece);
-        }
-        __syncwarp();
-        const int c = lane & 7;
-        const int n = p * PASS + c * PER; // first column of this lane's pieces
-        if(n < ncols)
-        {
-#pragma unroll
-            for(int i = 0; i < 8; ++i)
-            {
-                const int r = i * 4 + (lane >> 3);
-                if(row0 + r >= row_end)
-                    continue;
-                const uint4 v = *reinterpret_cast<const uint4*>(tile + r * 128 + ((c ^ (r & 7)) * 16));
-                T* dst        = e + static_cast<int64_t>(row0 + r) * lde + col0 + n;
-                if(vec && col0 + n + PER <= col_end)
-                    *reinterpret_cast<uint4*>(dst) = v;
-                else
-                {
-                    const T* w = reinterpret_cast<const T*>(&v);
-#pragma unroll
-                    for(int j = 0; j < PER; ++j)
-                        if(col0 + n + j < col_end)
-                            dst[j] = w[j];
-                }
-            }
+            for(int j = 0; j < PER; ++j)
+                if(col0 + n + j < col_end)
+                    dst[j] = w[j];
         }
     }
 }
 
+// FRAG = false: a lane holds its row, columns in order.  FRAG = true: fragments of 8 columns (tmem_ld_16x256b): pair
+// 4 g + 2 h + k of a lane = row 16 h + 8 k + lane / 4, columns 8 g + 2 (lane % 4) and the next one.
+template <typename T, int COLS, bool FRAG>
+__device__ __forceinline__ void store_rows(const uint64_t (&acc)[COLS / 2], uint8_t* tile, T* e, int64_t lde, int row0,
+                                           int row_end, int col0, int col_end, bool vec, int lane)
+{
+    constexpr int PER  = 16 / sizeof(T);
+    constexpr int PASS = 4 * PER; // columns of a pass
+    static_assert(COLS % 8 == 0, "whole pieces and fragments");
+#pragma unroll
+    for(int n0 = 0; n0 < COLS; n0 += PASS)
+    {
+        __syncwarp();
+        if constexpr(!FRAG)
+        {
+#pragma unroll
+            for(int c = 0; c < 4 && n0 + c * PER < COLS; ++c)
+            {
+                alignas(16) T piece[PER];
+#pragma unroll
+                for(int i = 0; i < PER; i += 2)
+                {
+                    float lo, hi;
+                    unpack_f32x2(acc[(n0 + c * PER + i) / 2], lo, hi);
+                    piece[i]     = scaled_out<T>(lo);
+                    piece[i + 1] = scaled_out<T>(hi);
+                }
+                *reinterpret_cast<uint4*>(tile + out_piece(lane, c)) = *reinterpret_cast<const uint4*>(piece);
+            }
+        }
+        else
+        {
+#pragma unroll
+            for(int g = n0 / 8; g < (n0 + PASS) / 8 && g < COLS / 8; ++g)
+#pragma unroll
+                for(int k = 0; k < 4; ++k) // rows 8 k + lane / 4
+                {
+                    float lo, hi;
+                    unpack_f32x2(acc[g * 4 + k], lo, hi);
+                    alignas(8) T pair[2] = {scaled_out<T>(lo), scaled_out<T>(hi)};
+                    const int byte = ((g * 8 - n0) + 2 * (lane & 3)) * static_cast<int>(sizeof(T));
+                    uint8_t* dst   = tile + out_piece(k * 8 + (lane >> 2), byte >> 4) + (byte & 15);
+                    if constexpr(sizeof(T) == 4)
+                        *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(pair);
+                    else
+                        *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(pair);
+                }
+        }
+        __syncwarp();
+        store_pass<T, COLS>(tile, n0, e, lde, row0, row_end, col0, col_end, vec, lane);
+    }
+}
+
 // The sums of a lane are a column of E (U = columns of B): for every row of E the lanes write neighbouring columns.
-template <typename T, int HALF>
-__device__ __forceinline__ void store_cols(const uint64_t (&acc)[HALF / 2], T* e, int64_t lde, int u, int u_end, int v0,
-                                           int v_end, int ncols)
+template <typename T, int COLS>
+__device__ __forceinline__ void store_cols(const uint64_t (&acc)[COLS / 2], T* e, int64_t lde, int u, int u_end, int v0,
+                                           int v_end)
 {
     if(u >= u_end)
         return;
 #pragma unroll
-    for(int c = 0; c < HALF; c += 2)
+    for(int c = 0; c < COLS; c += 2)
     {
         float lo, hi;
         unpack_f32x2(acc[c / 2], lo, hi);
-        if(c < ncols && v0 + c < v_end)
+        if(v0 + c < v_end)
             e[static_cast<int64_t>(v0 + c) * lde + u] = scaled_out<T>(lo);
-        if(c + 1 < ncols && v0 + c + 1 < v_end)
+        if(v0 + c + 1 < v_end)
             e[static_cast<int64_t>(v0 + c + 1) * lde + u] = scaled_out<T>(hi);
     }
 }
@@ -189,11 +259,11 @@ __device__ __forceinline__ void store_cols(const uint64_t (&acc)[HALF / 2], T* e
 // Owner side of a K split: sums column part `rank` over the slices, in slice order, and stores it.
 template <typename T>
 __device__ __forceinline__ void store_slices(const float* part, int pw, int slices, T* e, int64_t lde, int u, int u_end,
-                                             int v0, int v_end, int row, int first)
+                                             int v0, int v_end, int row, int first, int step)
 {
     if(u >= u_end)
         return;
-    for(int c = first; c < pw; c += 2)
+    for(int c = first; c < pw; c += step)
     {
         if(v0 + c >= v_end)
             break;
@@ -205,13 +275,21 @@ __device__ __forceinline__ void store_slices(const float* part, int pw, int slic
 }
 
 template <int BN, int CG, int VMODE>
-__global__ void __launch_bounds__(SCALED_THREADS, 1) scaled_kernel(const __grid_constant__ ScaledParams P)
+__global__ void __launch_bounds__(ScaledSmem<BN, CG>::THREADS, 1) scaled_kernel(const __grid_constant__ ScaledParams P)
 {
     using L                     = ScaledSmem<BN, CG>;
     constexpr int STAGES        = L::STAGES;
-    constexpr int HALF          = L::HALF;
-    constexpr uint32_t ACC_COLS = 2 * BN; // 32 .. 512, a power of two
-    constexpr int CHUNK         = HALF < 32 ? HALF : 32;
+    constexpr int COLS          = L::COLS;
+    constexpr int EPI_WARPS     = L::EPI_WARPS;
+    constexpr uint32_t ACC_COLS = L::ACC_COLS;
+    constexpr int SLOTS         = L::SLOTS;
+    constexpr int SCALE_BATCH   = L::SCALE_BATCH;
+    constexpr int CHUNK         = COLS < 16 ? COLS : 16;
+    constexpr bool STRADDLES    = 128 % COLS != 0; // a warp's columns may touch two blocks of 128
+    // Scales per column: with a row per lane every lane reads every column's scale, 512 bytes per four columns and warp,
+    // and shared memory takes twice as long as the sums (640 cycles for 128 columns, 365 with a scale per row); in
+    // fragments a lane has a quarter of the columns and four rows.
+    constexpr bool FRAG         = CG == 2 && VMODE != 0;
 
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw_addr  = smem_u32(smem_raw);
@@ -221,8 +299,10 @@ __global__ void __launch_bounds__(SCALED_THREADS, 1) scaled_kernel(const __grid_
     const uint32_t bar_base  = base_addr + L::BAR_OFFSET;
     auto full_bar            = [&](int s) { return bar_base + 8u * s; };
     auto done_bar            = [&](int s) { return bar_base + 8u * (STAGES + s); };
-    auto acc_empty_bar       = [&](int a) { return bar_base + 8u * (2 * STAGES + a); };
-    const uint32_t drain_bar = bar_base + 8u * (2 * STAGES + 2);
+    auto scale_full_bar      = [&](int s) { return bar_base + 8u * (2 * STAGES + s); };
+    auto scale_empty_bar     = [&](int s) { return bar_base + 8u * (2 * STAGES + SLOTS + s); };
+    const uint32_t drain_bar = bar_base + 8u * (2 * STAGES + 2 * SLOTS);
+    float* scale_ring        = reinterpret_cast<float*>(smem + L::SCALE_OFFSET);
     volatile uint32_t* misc  = reinterpret_cast<volatile uint32_t*>(smem + L::MISC_OFFSET);
     // misc[0] = TMEM base address, misc[1] = abort flag, misc[2] = constant 0, misc[3] = number of tiles (GROUP_ROWS)
     int32_t* grp_start = reinterpret_cast<int32_t*>(smem + L::GRP_OFFSET);
@@ -240,11 +320,16 @@ __global__ void __launch_bounds__(SCALED_THREADS, 1) scaled_kernel(const __grid_
     {
         for(int s = 0; s < STAGES; ++s)
         {
-            mbar_init(full_bar(s), 1); // the (leader's) producer arrival + all bytes of the stage
+            // the (leader's) producer arrival, all bytes of the stage, and the release of the accumulator that the K block
+            // will use: one arrival per epilogue warp (of both CTAs)
+            mbar_init(full_bar(s), 1 + EPI_WARPS * CG);
             mbar_init(done_bar(s), 1); // one tcgen05.commit arrival
         }
-        for(int a = 0; a < 2; ++a)
-            mbar_init(acc_empty_bar(a), NUM_EPI_WARPS * CG);
+        for(int s = 0; s < SLOTS; ++s)
+        {
+            mbar_init(scale_full_bar(s), 64); // one arrival per lane of the two scale warps
+            mbar_init(scale_empty_bar(s), EPI_WARPS);
+        }
         mbar_init(drain_bar, 1);
         misc[1] = 0;
         misc[2] = 0;
@@ -278,7 +363,7 @@ __global__ void __launch_bounds__(SCALED_THREADS, 1) scaled_kernel(const __grid_
     if(P.tiles.mode == SCALED_GROUP_ROWS)
     {
         // tiles of every group, then their running sum (one warp, 32 groups at a time)
-        for(int g = threadIdx.x; g < P.tiles.groups; g += SCALED_THREADS)
+        for(int g = threadIdx.x; g < P.tiles.groups; g += L::THREADS)
             scaled_group_span(P.offsets, g, P.tiles.swapped ? P.tiles.ext_v : P.tiles.ext_u, &grp_row0[g], &grp_row1[g]);
         __syncthreads();
         if(warp == 0)
@@ -326,11 +411,11 @@ __global__ void __launch_bounds__(SCALED_THREADS, 1) scaled_kernel(const __grid_
     };
 
     WaitCtx wc{&misc[1], P.wait_limit_ns, P.status};
-    const int half_cols = CG == 2 ? P.tiles.width >> 1 : HALF; // columns of an epilogue warp in this launch
+    constexpr int NUM_ACC = L::NUM_ACC;
 
     if(warp < SCALED_EPI_WARP0)
     {
-    if constexpr(BN >= 128)
+    if constexpr(L::SPLIT_REGS)
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(SCALED_REGS_LOW));
     if(warp == 0)
     {
@@ -342,45 +427,45 @@ __global__ void __launch_bounds__(SCALED_THREADS, 1) scaled_kernel(const __grid_
         int loads           = 0;
         bool ok             = true;
         const uint32_t bar0 = (CG == 2) ? mapa_shared(full_bar(0), 0) : full_bar(0);
-        // lane 0 loads the U box, lane 1 the V box
-        const bool is_v      = lane == 1;
-        const bool mn        = is_v ? P.v_mn != 0 : P.u_mn != 0;
-        const bool batched   = is_v ? P.v_batched != 0 : P.u_batched != 0;
-        const CUtensorMap* m = is_v ? &P.tm_v : &P.tm_u;
         // an MN-major V box always spans 128 columns (its smem tile has room for them: BN / CG = 128)
         const uint32_t stage_tx = CG * (L::U_BYTES + (P.v_mn ? 128 : P.v_box_rows) * BK_BYTES);
+        const int pair_rank     = CG == 2 ? static_cast<int>(cta_rank) : 0;
+        auto load_box = [&](const CUtensorMap* m, uint32_t dst, uint32_t bar, int c0, int c1, bool batched, int group) {
+            if(batched)
+            {
+                if constexpr(CG == 2)
+                    tma_load_3d_pair(dst, m, bar, c0, c1, group);
+                else
+                    tma_load_3d(dst, m, bar, c0, c1, group);
+            }
+            else
+            {
+                if constexpr(CG == 2)
+                    tma_load_2d_pair(dst, m, bar, c0, c1);
+                else
+                    tma_load_2d(dst, m, bar, c0, c1);
+            }
+        };
+        // The loops of the two single-thread roles are run by the whole warp, one elected lane issues: the loop state then
+        // lives in uniform registers, which the copy and MMA instructions take their operands from.
         for(int t = unit; ok && t < num_tiles; t += P.num_units)
         {
             const ScaledItem it = item_of(t);
-            const int row       = is_v ? it.v0 + static_cast<int>(CG == 2 ? cta_rank : 0) * half_cols
-                                       : it.u0 + static_cast<int>(CG == 2 ? cta_rank : 0) * 128;
+            const int u = it.u0 + pair_rank * 128, v = it.v0 + pair_rank * (BN / 2);
             for(int kb = it.kb0; kb < it.kb1; ++kb)
             {
-                ok = bounded_wait(done_bar(stage), phase ^ 1u, wc, WAIT_EMPTY);
+                ok = block_wait(done_bar(stage), phase ^ 1u, wc, WAIT_EMPTY);
                 ok = __all_sync(0xffffffffu, ok);
                 if(!ok)
                     break;
-                if(is_leader && lane == 0)
-                    mbar_arrive_expect_tx(full_bar(stage), stage_tx);
-                if(lane < 2)
+                const uint32_t dst = base_addr + stage * L::STAGE_BYTES, bar = bar0 + 8u * stage;
+                const int k = kb * SCALED_BLOCK;
+                if(elect_one_sync())
                 {
-                    const uint32_t dst = base_addr + stage * L::STAGE_BYTES + (is_v ? L::U_BYTES : 0);
-                    const uint32_t bar = bar0 + 8u * stage;
-                    const int c0 = mn ? row : kb * SCALED_BLOCK, c1 = mn ? kb * SCALED_BLOCK : row;
-                    if(batched)
-                    {
-                        if constexpr(CG == 2)
-                            tma_load_3d_pair(dst, m, bar, c0, c1, it.group);
-                        else
-                            tma_load_3d(dst, m, bar, c0, c1, it.group);
-                    }
-                    else
-                    {
-                        if constexpr(CG == 2)
-                            tma_load_2d_pair(dst, m, bar, c0, c1);
-                        else
-                            tma_load_2d(dst, m, bar, c0, c1);
-                    }
+                    if(is_leader)
+                        mbar_arrive_expect_tx(full_bar(stage), stage_tx);
+                    load_box(&P.tm_u, dst, bar, P.u_mn ? u : k, P.u_mn ? k : u, P.u_batched != 0, it.group);
+                    load_box(&P.tm_v, dst + L::U_BYTES, bar, P.v_mn ? v : k, P.v_mn ? k : v, P.v_batched != 0, it.group);
                 }
                 __syncwarp();
                 ++loads;
@@ -404,13 +489,13 @@ __global__ void __launch_bounds__(SCALED_THREADS, 1) scaled_kernel(const __grid_
     else if(warp == 1)
     {
         // ------------------------------------------------------------------ MMA issuer
-        if(lane == 0 && is_leader)
+        if(is_leader)
         {
-            int stage       = 0;
-            uint32_t phase  = 0;
-            uint32_t iter   = 0; // K blocks so far
-            bool ok         = true;
-            bool issued_any = false;
+            int stage          = 0;
+            uint32_t phase     = 0;
+            int acc            = 0;
+            bool ok            = true;
+            bool issued_any    = false;
             const uint64_t u_const = P.u_mn ? make_smem_desc_mn_sw128(0, 128 * BK_BYTES) : make_smem_desc_k_sw128(0);
             const uint64_t v_const = P.v_mn ? make_smem_desc_mn_sw128(0, 128 * BK_BYTES) : make_smem_desc_k_sw128(0);
             const uint32_t u_hi = static_cast<uint32_t>(u_const >> 32), v_hi = static_cast<uint32_t>(v_const >> 32);
@@ -419,33 +504,36 @@ __global__ void __launch_bounds__(SCALED_THREADS, 1) scaled_kernel(const __grid_
             for(int t = unit; ok && t < num_tiles; t += P.num_units)
             {
                 const ScaledItem it = item_of(t);
-                for(int kb = it.kb0; kb < it.kb1; ++kb, ++iter)
+                for(int kb = it.kb0; kb < it.kb1; ++kb)
                 {
-                    const int acc = iter & 1;
-                    ok = bounded_wait(acc_empty_bar(acc), ((iter >> 1) & 1u) ^ 1u, wc, WAIT_TMEM_EMPTY) &&
-                         bounded_wait(full_bar(stage), phase, wc, WAIT_FULL);
+                    ok = block_wait(full_bar(stage), phase, wc, WAIT_FULL);
+                    ok = __all_sync(0xffffffffu, ok);
                     if(!ok)
                         break;
                     tc_fence_after_sync();
                     const uint32_t u_addr = base_addr + stage * L::STAGE_BYTES;
-                    uint32_t u_lo         = static_cast<uint32_t>(u_const) | ((u_addr & 0x3FFFFu) >> 4);
-                    uint32_t v_lo         = static_cast<uint32_t>(v_const) | (((u_addr + L::U_BYTES) & 0x3FFFFu) >> 4);
+                    const uint32_t u_lo   = static_cast<uint32_t>(u_const) | ((u_addr & 0x3FFFFu) >> 4);
+                    const uint32_t v_lo   = static_cast<uint32_t>(v_const) | (((u_addr + L::U_BYTES) & 0x3FFFFu) >> 4);
                     const uint32_t d      = tmem_base + acc * BN;
-#pragma unroll
-                    for(int k = 0; k < 4; ++k)
+                    if(elect_one_sync())
                     {
+#pragma unroll
+                        for(int k = 0; k < 4; ++k)
+                        {
+                            if constexpr(CG == 2)
+                                mma_f8_ss_pair_split(d, u_lo + k * u_step, u_hi, v_lo + k * v_step, v_hi, P.idesc, k != 0);
+                            else
+                                mma_f8_ss_split(d, u_lo + k * u_step, u_hi, v_lo + k * v_step, v_hi, P.idesc, k != 0);
+                        }
                         if constexpr(CG == 2)
-                            mma_f8_ss_pair_split(d, u_lo, u_hi, v_lo, v_hi, P.idesc, k != 0);
+                            mma_commit_pair_mc(done_bar(stage), 3);
                         else
-                            mma_f8_ss_split(d, u_lo, u_hi, v_lo, v_hi, P.idesc, k != 0);
-                        u_lo += u_step;
-                        v_lo += v_step;
+                            mma_commit(done_bar(stage));
                     }
+                    __syncwarp();
                     issued_any = true;
-                    if constexpr(CG == 2)
-                        mma_commit_pair_mc(done_bar(stage), 3);
-                    else
-                        mma_commit(done_bar(stage));
+                    if(++acc == NUM_ACC)
+                        acc = 0;
                     if(++stage == STAGES)
                     {
                         stage = 0;
@@ -456,217 +544,280 @@ __global__ void __launch_bounds__(SCALED_THREADS, 1) scaled_kernel(const __grid_
             // Every MMA issued must be finished before the tensor memory is freed.
             if(issued_any)
             {
-                if constexpr(CG == 2)
-                    mma_commit_pair(drain_bar);
-                else
-                    mma_commit(drain_bar);
+                if(elect_one_sync())
+                {
+                    if constexpr(CG == 2)
+                        mma_commit_pair(drain_bar);
+                    else
+                        mma_commit(drain_bar);
+                }
+                __syncwarp();
                 WaitCtx drain{&misc[2], kDrainLimitNs, P.status};
                 bounded_wait(drain_bar, 0, drain, WAIT_DRAIN);
             }
         }
         __syncwarp();
     }
+    else
+    {
+        // ------------------------------------------------------------------ scales
+        // Warp 2 brings the scales of the U side, warp 3 those of the V side, as asynchronous copies into the ring in
+        // shared memory (no registers, nothing waits for their latency).  A batch of SCALE_BATCH K blocks belongs to one
+        // tile; the last one of a tile may be shorter.
+        const bool is_v    = warp == 3;
+        const int n_per    = is_v ? (VMODE == 0 ? 1 : L::V_SCALES / 32) : 4; // scales of a lane and K block
+        const int64_t kbs  = is_v ? P.sv_kb : P.su_kb;
+        const uint32_t ring = base_addr + L::SCALE_OFFSET + ((is_v ? 128 : 0) + lane) * 4;
+        int slot           = 0;
+        uint32_t phase     = 0;
+        bool ok            = true;
+        for(int t = unit; ok && t < num_tiles; t += P.num_units)
+        {
+            const ScaledItem it = item_of(t);
+            const float* p      = is_v ? P.sv + it.group * P.sv_group : P.su + it.group * P.su_group;
+            int64_t step        = 0; // from one of the lane's scales to the next
+            int have;                // how many of them exist
+            if(is_v && VMODE == 0)
+            {
+                // blocks of 128 columns that the tile touches: three at most
+                const int b = (it.v0 >> 7) + lane;
+                have        = lane < 3 && (static_cast<int64_t>(b) << 7) < it.v_end ? 1 : 0;
+                p += b * P.sv_row;
+            }
+            else
+            {
+                const int x   = (is_v ? it.v0 : it.u0 + static_cast<int>(CG == 2 ? cta_rank : 0) * 128) + lane;
+                const int end = is_v ? (it.v0 + BN < it.v_end ? it.v0 + BN : it.v_end) : it.u_end;
+                have          = x < end ? (end - x + 31) / 32 : 0;
+                const int sh  = is_v ? 0 : P.u_shift;
+                step          = is_v ? 32 * P.sv_row : sh ? 0 : 32 * P.su_row; // (a U tile lies in one block of 128)
+                p += static_cast<int64_t>(x >> sh) * (is_v ? P.sv_row : P.su_row);
+            }
+            if(have <= 0)
+                p = P.su; // (a valid address, never read)
+            p += it.kb0 * (have > 0 ? kbs : 0);
+            for(int kb = it.kb0; kb < it.kb1; kb += SCALE_BATCH)
+            {
+                ok = block_wait(scale_empty_bar(slot), phase ^ 1u, wc, WAIT_EMPTY);
+                ok = __all_sync(0xffffffffu, ok);
+                if(!ok)
+                    break;
+                const int n_kb = it.kb1 - kb < SCALE_BATCH ? it.kb1 - kb : SCALE_BATCH;
+                uint32_t dst   = ring + slot * SCALE_BATCH * L::SCALE_WORDS * 4;
+                for(int j = 0; j < n_kb; ++j)
+                {
+                    const float* q = p;
+                    for(int i = 0; i < n_per; ++i)
+                    {
+                        const bool in = i < have;
+                        copy_async_4(dst + i * 128, in ? q : P.su, in ? 4u : 0u);
+                        q += in ? step : 0;
+                    }
+                    p += have > 0 ? kbs : 0;
+                    dst += L::SCALE_WORDS * 4;
+                }
+                copy_async_arrive(scale_full_bar(slot));
+                if(++slot == SLOTS)
+                {
+                    slot = 0;
+                    phase ^= 1u;
+                }
+            }
+        }
+        copy_async_wait_all(); // nothing may land in shared memory after the exit
+        __syncwarp();
+    }
     }
     else
     {
-        if constexpr(BN >= 128)
+        if constexpr(L::SPLIT_REGS)
             asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SCALED_REGS_HIGH));
         // ------------------------------------------------------------------ epilogue warps
-        const int quarter = warp & 3, half = (warp - SCALED_EPI_WARP0) >> 2;
+        const int quarter = warp & 3, part = (warp - SCALED_EPI_WARP0) >> 2;
         const int row     = quarter * 32 + lane; // lane of the accumulator
-        const int col     = half * half_cols;    // first column of this warp
-        const uint32_t taddr0  = tmem_base + col + (static_cast<uint32_t>(quarter * 32) << 16);
-        const uint32_t empty0  = (CG == 2) ? mapa_shared(acc_empty_bar(0), 0) : acc_empty_bar(0);
-        constexpr int CV       = (HALF + 31) / 32;
-        constexpr int CBUF     = HALF < 32 ? 32 : HALF;
-        float* colbuf          = reinterpret_cast<float*>(smem + L::COL_OFFSET) + (warp - SCALED_EPI_WARP0) * 2 * CBUF;
-        uint8_t* out_tile      = smem + L::OUT_OFFSET + (warp - SCALED_EPI_WARP0) * 4096;
-        uint64_t acc[HALF / 2];
-        float su_r[2], lo_r[2], hi_r[2], cv_r[2][CV];
-        const float *su_p = nullptr, *sv_p = nullptr, *sv_hi_p = nullptr;
-        bool su_on = false;
-        uint32_t cv_on = 0;
-        int hi_from = 0; // VMODE 0: columns (of the warp) from here on belong to the second scale block
-        ScaledItem it{};
-
-        // scales of K block `kb` into slot j (zeros beyond the item or outside the matrix: never used or never stored)
-        auto load_scales = [&](int j, int kb) {
-            const bool in = kb < it.kb1;
-            su_r[j]       = in && su_on ? __ldg(su_p + kb * P.su_kb) : 0.f;
-            if constexpr(VMODE == 0)
+        const int col     = part * COLS;    // first column of this warp
+        const uint32_t taddr0 = tmem_base + col + (static_cast<uint32_t>(quarter * 32) << 16);
+        // The MMA thread waits on one barrier per K block: releasing the accumulator of K block i is an arrival on the
+        // barrier of the stage that K block i + NUM_ACC will fill (its last phase is over: K block i has been multiplied, and
+        // with it every K block up to i + NUM_ACC - STAGES).  The first NUM_ACC find their accumulators free.
+        const uint32_t ready0 = (CG == 2) ? mapa_shared(full_bar(0), 0) : full_bar(0);
+        auto release_for = [&](int s) { // accumulator of the K block that stage s gets next
+            if(lane == 0)
             {
-                lo_r[j] = in && cv_on != 0 ? __ldg(sv_p + kb * P.sv_kb) : 0.f;
-                hi_r[j] = in && cv_on > 1 ? __ldg(sv_hi_p + kb * P.sv_kb) : lo_r[j];
-            }
-            else
-            {
-#pragma unroll
-                for(int q = 0; q < CV; ++q)
-                    cv_r[j][q] = in && (cv_on >> q & 1u) ? __ldg(sv_p + q * 32 * P.sv_row + kb * P.sv_kb) : 0.f;
+                if constexpr(CG == 2)
+                    mbar_arrive_cluster_relaxed(ready0 + 8u * s);
+                else
+                    mbar_arrive(ready0 + 8u * s);
             }
         };
-        auto open_item = [&](int t) {
-            it          = item_of(t);
-            const int u = it.u0 + static_cast<int>(CG == 2 ? cta_rank : 0) * 128 + (VMODE == 1 ? 0 : row);
-            su_on       = u < it.u_end;
-            su_p        = P.su + it.group * P.su_group + static_cast<int64_t>(u >> P.u_shift) * P.su_row;
-            const int v = it.v0 + col;
-            if constexpr(VMODE == 0)
-            {
-                const int b0 = v >> 7;
-                sv_p         = P.sv + it.group * P.sv_group + static_cast<int64_t>(b0) * P.sv_row;
-                sv_hi_p      = sv_p + P.sv_row;
-                hi_from      = ((b0 + 1) << 7) - v;
-                cv_on        = v < it.v_end ? (hi_from < half_cols && v + hi_from < it.v_end ? 2u : 1u) : 0u;
-            }
-            else
-            {
-                sv_p  = P.sv + it.group * P.sv_group + static_cast<int64_t>(v + lane) * P.sv_row;
-                cv_on = 0;
-#pragma unroll
-                for(int q = 0; q < CV; ++q)
-                    if(v + q * 32 + lane < it.v_end && q * 32 + lane < half_cols)
-                        cv_on |= 1u << q;
-            }
-            load_scales(0, it.kb0);
-            load_scales(1, it.kb0 + 1);
-        };
-
-        int stage      = 0;
-        uint32_t phase = 0, iter = 0;
-        bool ok        = true;
-        if(unit < num_tiles)
-            open_item(unit);
-        for(int t = unit; ok && t < num_tiles;)
+        for(int s = 0; s < NUM_ACC; ++s)
+            release_for(s);
+        int next_stage = NUM_ACC % STAGES;
+        uint8_t* out_tile     = smem + L::OUT_OFFSET + (warp - SCALED_EPI_WARP0) * 2048;
+        uint64_t acc[COLS / 2];
+        int stage = 0, slot = 0, buf = 0;
+        uint32_t phase = 0, slot_phase = 0;
+        bool ok = true;
+        for(int t = unit; ok && t < num_tiles; t += P.num_units)
         {
+            const ScaledItem it = item_of(t);
+            // VMODE 0: the warp's columns touch two blocks of 128 at most; from column hi_from on it is the second
+            const int lo_i    = ((it.v0 + col) >> 7) - (it.v0 >> 7);
+            const int hi_from = (((it.v0 + col) >> 7) + 1) * 128 - (it.v0 + col);
 #pragma unroll
-            for(int i = 0; i < HALF / 2; ++i)
+            for(int i = 0; i < COLS / 2; ++i)
                 acc[i] = 0;
-            auto step = [&](int j, int kb) {
-                ok = bounded_wait(done_bar(stage), phase, wc, WAIT_TMEM_FULL);
-                ok = __all_sync(0xffffffffu, ok);
-                if(!ok)
-                    return;
-                tc_fence_after_sync();
-                const float su = su_r[j];
-                float s_lo = 0.f, s_hi = 0.f;
-                float* cb = colbuf + (iter & 1u) * CBUF;
+            const float* su_s = nullptr;
+            int in_batch      = 0;
+            for(int kb = it.kb0; kb < it.kb1; ++kb)
+            {
+                if(in_batch == 0)
+                {
+                    ok   = block_wait(scale_full_bar(slot), slot_phase, wc, WAIT_FULL);
+                    su_s = scale_ring + slot * SCALE_BATCH * L::SCALE_WORDS;
+                }
+                else
+                    su_s += L::SCALE_WORDS;
+                const float* sv_s = su_s + 128 + (VMODE == 0 ? lo_i : col);
+                uint64_t s_lo = 0, s_hi = 0, su2[4] = {};
                 if constexpr(VMODE == 0)
                 {
-                    s_lo = su * lo_r[j];
-                    s_hi = su * hi_r[j];
+                    const float su = su_s[row], lo = su * sv_s[0];
+                    s_lo = pack_f32x2(lo, lo);
+                    if constexpr(STRADDLES)
+                    {
+                        const float hi = su * sv_s[1];
+                        s_hi           = pack_f32x2(hi, hi);
+                    }
                 }
                 else
                 {
-                    // the other buffer was last read two K blocks ago, a __syncwarp in between
 #pragma unroll
-                    for(int q = 0; q < CV; ++q)
-                        cb[q * 32 + lane] = VMODE == 1 ? cv_r[j][q] * su : cv_r[j][q];
-                    __syncwarp();
+                    for(int k = 0; k < (FRAG ? 4 : 1); ++k)
+                    {
+                        const float su = su_s[FRAG ? quarter * 32 + k * 8 + (lane >> 2) : row];
+                        su2[k]         = pack_f32x2(su, su);
+                    }
                 }
-                load_scales(j, kb + 2);
-                const uint32_t taddr = taddr0 + (iter & 1u) * BN;
-#pragma unroll
-                for(int c = 0; c < HALF; c += CHUNK)
-                {
-                    if(CG == 2 && c >= half_cols)
-                        break;
-                    const bool whole = CG == 1 || c + 32 <= half_cols; // else 16 columns of the chunk
-                    uint32_t v[32];
-                    if constexpr(CHUNK == 32)
+                ok = ok && block_wait(done_bar(stage), phase, wc, WAIT_TMEM_FULL);
+                ok = __all_sync(0xffffffffu, ok);
+                if(!ok)
+                    break;
+                tc_fence_after_sync();
+                const uint32_t taddr = taddr0 + buf * BN;
+                // everything is in registers: a later K block may overwrite the accumulator
+                auto release = [&]() {
+                    tc_fence_before_sync();
+                    __syncwarp();
+                    release_for(next_stage);
+                };
+                // N columns from column c on, from tensor memory into v, and from v into the sums
+                auto load = [&](auto width, int c, uint32_t* v) {
+                    constexpr int N = decltype(width)::value;
+                    if constexpr(FRAG && N == 16)
                     {
-                        tmem_ld_32x32b_x16(taddr + c, v);
-                        if(whole)
-                            tmem_ld_32x32b_x16(taddr + c + 16, v + 16);
-                        tmem_ld_wait_regs16(v);
-                        if(whole)
-                            keep_regs16(v + 16);
+                        tmem_ld_16x256b_x2(taddr + c, v);
+                        tmem_ld_16x256b_x2(taddr + c + (16u << 16), v + 8);
                     }
-                    else if constexpr(CHUNK == 16)
+                    else if constexpr(FRAG)
                     {
-                        tmem_ld_32x32b_x16(taddr + c, v);
-                        tmem_ld_wait_regs16(v);
+                        tmem_ld_16x256b_x1(taddr + c, v);
+                        tmem_ld_16x256b_x1(taddr + c + (16u << 16), v + 4);
                     }
+                    else if constexpr(N == 16)
+                        tmem_ld_32x32b_x16(taddr + c, v);
                     else
-                    {
                         tmem_ld_32x32b_x8(taddr + c, v);
-                        tmem_ld_wait_regs8(v);
-                    }
-                    if(c + CHUNK >= half_cols)
+                };
+                auto pair_of = [](const uint32_t* v) { return pack_f32x2(__uint_as_float(v[0]), __uint_as_float(v[1])); };
+                auto add     = [&](auto width, int c, const uint32_t* v) {
+                    constexpr int N = decltype(width)::value;
+                    if constexpr(VMODE == 0)
                     {
-                        // everything is in registers: the next but one K block may overwrite the accumulator
-                        tc_fence_before_sync();
-                        __syncwarp();
-                        if(lane == 0)
+#pragma unroll
+                        for(int i = 0; i < N; i += 2)
                         {
-                            if constexpr(CG == 2)
-                                mbar_arrive_cluster(empty0 + 8u * (iter & 1u));
-                            else
-                                mbar_arrive(empty0 + 8u * (iter & 1u));
+                            const uint64_t s2 = STRADDLES && c + (i & ~7) >= hi_from ? s_hi : s_lo;
+                            acc[(c + i) / 2]  = fma_f32x2(pair_of(v + i), s2, acc[(c + i) / 2]);
                         }
                     }
-#pragma unroll
-                    for(int h = 0; h < CHUNK; h += 16)
+                    else if constexpr(FRAG)
                     {
-                        if(h == 16 && !whole)
-                            break;
-                        constexpr int N = CHUNK < 16 ? CHUNK : 16;
-                        if constexpr(VMODE == 0)
-                        {
-                            const float s     = c + h >= hi_from ? s_hi : s_lo;
-                            const uint64_t s2 = pack_f32x2(s, s);
 #pragma unroll
-                            for(int i = 0; i < N; i += 2)
-                                acc[(c + h + i) / 2] = fma_f32x2(
-                                    pack_f32x2(__uint_as_float(v[h + i]), __uint_as_float(v[h + i + 1])), s2, acc[(c + h + i) / 2]);
-                        }
-                        else
+                        for(int g = 0; g < N / 8; ++g)
                         {
-                            const uint64_t su2 = pack_f32x2(su, su);
+                            const uint64_t s2 = *reinterpret_cast<const uint64_t*>(sv_s + c + g * 8 + 2 * (lane & 3));
 #pragma unroll
-                            for(int i = 0; i < N; i += 4)
+                            for(int k = 0; k < 4; ++k) // rows 8 k + lane / 4
                             {
-                                const float4 s4 = *reinterpret_cast<const float4*>(cb + c + h + i);
-                                uint64_t p0 = pack_f32x2(__uint_as_float(v[h + i]), __uint_as_float(v[h + i + 1]));
-                                uint64_t p1 = pack_f32x2(__uint_as_float(v[h + i + 2]), __uint_as_float(v[h + i + 3]));
-                                if constexpr(VMODE == 2)
-                                {
-                                    p0 = mul_f32x2(p0, su2);
-                                    p1 = mul_f32x2(p1, su2);
-                                }
-                                acc[(c + h + i) / 2]     = fma_f32x2(p0, pack_f32x2(s4.x, s4.y), acc[(c + h + i) / 2]);
-                                acc[(c + h + i) / 2 + 1] = fma_f32x2(p1, pack_f32x2(s4.z, s4.w), acc[(c + h + i) / 2 + 1]);
+                                const uint64_t p = pair_of(v + (k >> 1) * (N / 2) + g * 4 + (k & 1) * 2);
+                                uint64_t& a      = acc[(c / 8 + g) * 4 + k];
+                                a                = fma_f32x2(p, mul_f32x2(s2, su2[k]), a);
                             }
                         }
                     }
+                    else
+                    {
+#pragma unroll
+                        for(int i = 0; i < N; i += 4)
+                        {
+                            const ulonglong2 s4 = *reinterpret_cast<const ulonglong2*>(sv_s + c + i);
+                            acc[(c + i) / 2]     = fma_f32x2(pair_of(v + i), mul_f32x2(s4.x, su2[0]), acc[(c + i) / 2]);
+                            acc[(c + i) / 2 + 1] = fma_f32x2(pair_of(v + i + 2), mul_f32x2(s4.y, su2[0]), acc[(c + i) / 2 + 1]);
+                        }
+                    }
+                };
+                // (a chunk in flight while another is added was slower: the warps of a scheduler hide each other's loads)
+                constexpr int LAST = COLS % CHUNK == 0 ? CHUNK : COLS % CHUNK; // BN = 224: 8
+#pragma unroll
+                for(int c = 0; c + CHUNK <= COLS; c += CHUNK)
+                {
+                    uint32_t v[CHUNK];
+                    load(std::integral_constant<int, CHUNK>{}, c, v);
+                    tmem_ld_wait_regs<CHUNK>(v);
+                    if(c + CHUNK == COLS)
+                        release();
+                    add(std::integral_constant<int, CHUNK>{}, c, v);
                 }
-                ++iter;
+                if constexpr(LAST != CHUNK)
+                {
+                    uint32_t v[LAST];
+                    load(std::integral_constant<int, LAST>{}, COLS - LAST, v);
+                    tmem_ld_wait_regs<LAST>(v);
+                    release();
+                    add(std::integral_constant<int, LAST>{}, COLS - LAST, v);
+                }
+                if(++in_batch == SCALE_BATCH || kb + 1 == it.kb1)
+                {
+                    in_batch = 0;
+                    __syncwarp();
+                    if(lane == 0)
+                        mbar_arrive(scale_empty_bar(slot));
+                    if(++slot == SLOTS)
+                    {
+                        slot = 0;
+                        slot_phase ^= 1u;
+                    }
+                }
+                if(++buf == NUM_ACC)
+                    buf = 0;
+                if(++next_stage == STAGES)
+                    next_stage = 0;
                 if(++stage == STAGES)
                 {
                     stage = 0;
                     phase ^= 1u;
                 }
-            };
-            const int kb1 = it.kb1;
-            for(int kb = it.kb0; ok && kb < kb1; kb += 2)
-            {
-                step(0, kb);
-                if(ok && kb + 1 < kb1)
-                    step(1, kb + 1);
             }
             if(!ok)
                 break;
-            const ScaledItem cur = it;
-            t += P.num_units;
-            if(t < num_tiles)
-                open_item(t); // the next tile's first scales arrive while this one is stored
             if(CG == 1 && ksplit > 1)
             {
                 // hand the sums to the CTAs that own the columns: [slice][column of the part][row]
                 const int pw        = BN / ksplit;
                 const uint32_t part = base_addr + L::OUT_OFFSET + static_cast<uint32_t>(cta_rank) * pw * 512u + row * 4u;
 #pragma unroll
-                for(int c = 0; c < HALF; ++c)
+                for(int c = 0; c < COLS; ++c)
                 {
                     float lo, hi;
                     unpack_f32x2(acc[c / 2], lo, hi);
@@ -679,15 +830,14 @@ __global__ void __launch_bounds__(SCALED_THREADS, 1) scaled_kernel(const __grid_
                 }
                 continue; // one tile per cluster: summed below, behind the cluster barrier
             }
-            const int64_t e_off = cur.group * P.e_group;
-            const int u_row     = cur.u0 + static_cast<int>(CG == 2 ? cta_rank : 0) * 128 + quarter * 32;
+            const int64_t e_off = it.group * P.e_group;
+            const int u_row     = it.u0 + static_cast<int>(CG == 2 ? cta_rank : 0) * 128 + quarter * 32;
             auto store = [&](auto* e) {
                 using T = typename std::remove_pointer<decltype(e)>::type;
-                if(CG == 1 || P.tiles.swapped)
-                    store_cols<T, HALF>(acc, e + e_off, P.lde, u_row + lane, cur.u_end, cur.v0 + col, cur.v_end, half_cols);
-                else if constexpr(CG == 2)
-                    store_rows<T, HALF>(acc, out_tile, e + e_off, P.lde, u_row, cur.u_end, cur.v0 + col, cur.v_end, half_cols,
-                                        P.e_vec != 0, lane);
+                if constexpr(CG == 1)
+                    store_cols<T, COLS>(acc, e + e_off, P.lde, u_row + lane, it.u_end, it.v0 + col, it.v_end);
+                else
+                    store_rows<T, COLS, FRAG>(acc, out_tile, e + e_off, P.lde, u_row, it.u_end, it.v0 + col, it.v_end, P.e_vec != 0, lane);
             };
             if(P.e_dtype == CKB_BF16)
                 store(static_cast<__nv_bfloat16*>(P.e));
@@ -708,7 +858,7 @@ __global__ void __launch_bounds__(SCALED_THREADS, 1) scaled_kernel(const __grid_
             const int pw      = BN / ksplit;
             const float* part = reinterpret_cast<const float*>(smem + L::OUT_OFFSET);
             const int v0      = it.v0 + static_cast<int>(cta_rank) * pw;
-            auto sum = [&](auto* e) { store_slices(part, pw, ksplit, e, P.lde, it.u0 + row, it.u_end, v0, it.v_end, row, t >> 7); };
+            auto sum = [&](auto* e) { store_slices(part, pw, ksplit, e, P.lde, it.u0 + row, it.u_end, v0, it.v_end, row, t >> 7, EPI_WARPS / 4); };
             if(P.e_dtype == CKB_BF16)
                 sum(static_cast<__nv_bfloat16*>(P.e));
             else if(P.e_dtype == CKB_F16)

@@ -1,4 +1,4 @@
-// Launch of scaled_kernel instances; instantiated in ckb_scaled_inst_*.cu, one file per VMODE.
+// Launch of scaled_kernel instances; instantiated in ckb_scaled_inst_*.cu, one file per VMODE and CG.
 #pragma once
 #include "ckb_host.h"
 #include "ckb_scaled_kernel.cuh"
@@ -21,14 +21,14 @@ cudaError_t launch_scaled_one(const ScaledParams& p, int grid, cudaStream_t stre
         err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
         if(err != cudaSuccess)
             return err;
-        if constexpr(BN >= 128)
+        if constexpr(ScaledSmem<BN, CG>::SPLIT_REGS)
         {
             // the register shares of the warpgroups are drawn from what the block is launched with
             cudaFuncAttributes fa;
             err = cudaFuncGetAttributes(&fa, kern);
             if(err != cudaSuccess)
                 return err;
-            if(fa.numRegs * 3 < SCALED_REGS_LOW + 2 * SCALED_REGS_HIGH)
+            if(fa.numRegs * 5 < SCALED_REGS_LOW + 4 * SCALED_REGS_HIGH)
                 return cudaErrorInvalidConfiguration;
         }
         if(dev >= 0 && dev < 64)
@@ -36,7 +36,7 @@ cudaError_t launch_scaled_one(const ScaledParams& p, int grid, cudaStream_t stre
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim            = dim3(grid, 1, 1);
-    cfg.blockDim           = dim3(SCALED_THREADS, 1, 1);
+    cfg.blockDim           = dim3(ScaledSmem<BN, CG>::THREADS, 1, 1);
     cfg.dynamicSmemBytes   = SMEM;
     cfg.stream             = stream;
     cudaLaunchAttribute attr[2];
@@ -62,23 +62,34 @@ cudaError_t launch_scaled_one(const ScaledParams& p, int grid, cudaStream_t stre
 }
 
 // query_cluster = 0: launches.  Otherwise only asks how many clusters of that many CTAs the device holds at once.
-template <int VMODE>
-cudaError_t launch_scaled(int bn, int cg, const ScaledParams& p, int grid, cudaStream_t stream, int query_cluster, int* clusters)
+template <int VMODE, int CG>
+cudaError_t launch_scaled(int bn, const ScaledParams& p, int grid, cudaStream_t stream, int query_cluster, int* clusters)
 {
-    if(cg == 2)
-        return launch_scaled_one<256, 2, VMODE>(p, grid, stream, query_cluster, clusters);
-    switch(bn)
-    {
-    case 16: return launch_scaled_one<16, 1, VMODE>(p, grid, stream, query_cluster, clusters);
-    case 32: return launch_scaled_one<32, 1, VMODE>(p, grid, stream, query_cluster, clusters);
-    case 64: return launch_scaled_one<64, 1, VMODE>(p, grid, stream, query_cluster, clusters);
-    case 128: return launch_scaled_one<128, 1, VMODE>(p, grid, stream, query_cluster, clusters);
-    default: return cudaErrorInvalidValue;
-    }
+    if constexpr(CG == 2)
+        switch(bn)
+        {
+        case 128: return launch_scaled_one<128, 2, VMODE>(p, grid, stream, query_cluster, clusters);
+        case 192: return launch_scaled_one<192, 2, VMODE>(p, grid, stream, query_cluster, clusters);
+        case 224: return launch_scaled_one<224, 2, VMODE>(p, grid, stream, query_cluster, clusters);
+        case 256: return launch_scaled_one<256, 2, VMODE>(p, grid, stream, query_cluster, clusters);
+        default: return cudaErrorInvalidValue;
+        }
+    else
+        switch(bn)
+        {
+        case 16: return launch_scaled_one<16, 1, VMODE>(p, grid, stream, query_cluster, clusters);
+        case 32: return launch_scaled_one<32, 1, VMODE>(p, grid, stream, query_cluster, clusters);
+        case 64: return launch_scaled_one<64, 1, VMODE>(p, grid, stream, query_cluster, clusters);
+        case 128: return launch_scaled_one<128, 1, VMODE>(p, grid, stream, query_cluster, clusters);
+        default: return cudaErrorInvalidValue;
+        }
 }
 
-extern template cudaError_t launch_scaled<0>(int, int, const ScaledParams&, int, cudaStream_t, int, int*);
-extern template cudaError_t launch_scaled<1>(int, int, const ScaledParams&, int, cudaStream_t, int, int*);
-extern template cudaError_t launch_scaled<2>(int, int, const ScaledParams&, int, cudaStream_t, int, int*);
+#define CKB_SCALED_EXTERN(V, C) extern template cudaError_t launch_scaled<V, C>(int, const ScaledParams&, int, cudaStream_t, int, int*);
+CKB_SCALED_EXTERN(0, 1)
+CKB_SCALED_EXTERN(1, 1)
+CKB_SCALED_EXTERN(0, 2)
+CKB_SCALED_EXTERN(1, 2)
+#undef CKB_SCALED_EXTERN
 
 } // namespace ckb

@@ -3,6 +3,7 @@
 //
 // One operand of the product is the U side (the 128 rows a CTA's tensor core works on), the other the V side (the
 // columns of the accumulator).  `swapped` = 0: U = A (rows of E), V = B (columns of E); `swapped` = 1: U = B, V = A.
+// CTA pairs work unswapped, single CTAs swapped.
 // A tile is u_rows = 128 x CTAs of U by `width` of V.
 #pragma once
 #include <stdint.h>
@@ -132,8 +133,7 @@ struct ScaledPlanInput
     int a_block, b_block;     // rows / columns per scale
     int sm_count;
     int cluster_cap[3];       // clusters of 2 / 4 / 8 CTAs resident at once
-    // pinned by the caller (0 / -1: free)
-    int cols = 0, cg = 0, swap = -1, ksplit = 0;
+    int cols = 0, cg = 0, ksplit = 0; // pinned by the caller (0: free)
 };
 struct ScaledPlan
 {
@@ -151,7 +151,7 @@ inline double scaled_kb_cycles(int cg, int width, int vmode, bool v_mn)
     const double mma   = 2.0 * width;
     const double bytes = 16384.0 + (v_mn ? 16384.0 : width / cg * 128.0);
     const int chunks   = (width / 2 + 31) / 32;
-    const double epi   = (vmode == 0 ? 110.0 : 180.0) + chunks * (vmode == 0 ? 75.0 : vmode == 1 ? 95.0 : 115.0);
+    const double epi   = (vmode == 0 ? 110.0 : 180.0) + chunks * (vmode == 0 ? 75.0 : 115.0);
     double c           = mma;
     if(bytes / 68.0 > c)
         c = bytes / 68.0;
@@ -160,7 +160,9 @@ inline double scaled_kb_cycles(int cg, int width, int vmode, bool v_mn)
     return c > 400.0 ? c : 400.0;
 }
 
-inline int scaled_vmode(int u_block, int v_block) { return v_block == 128 ? 0 : u_block == 128 ? 1 : 2; }
+constexpr int kScaledWidths[2][4] = {{16, 32, 64, 128}, {128, 192, 224, 256}}; // columns of V per tile, by CTAs per tile
+
+inline int scaled_vmode(int v_block) { return v_block == 128 ? 0 : 1; }
 
 // Chooses tile, orientation and K split by estimated cycles; false when nothing fits (too many tiles, or a pinned
 // configuration that the problem cannot use).
@@ -169,12 +171,12 @@ inline bool plan_scaled(const ScaledPlanInput& in, ScaledPlan* out)
     bool found = false;
     const bool rows = in.mode == SCALED_GROUP_ROWS;
     for(int cg = 1; cg <= 2; ++cg)
-        for(int swap = cg == 1 ? 1 : 0; swap <= 1; ++swap)
-            for(int width = cg == 1 ? 16 : 64; width <= (cg == 1 ? 128 : 256); width = cg == 1 ? width * 2 : width + 32)
+    {
+        const int swap = cg == 1 ? 1 : 0;
+            for(const int width : kScaledWidths[cg - 1])
                 for(int ks = 1; ks <= (cg == 1 ? 8 : 1); ks *= 2)
                 {
-                    if((in.cg && in.cg != cg) || (in.swap >= 0 && in.swap != swap) || (in.cols && in.cols != width) ||
-                       (in.ksplit ? in.ksplit != ks : in.cols && ks != 1))
+                    if((in.cg && in.cg != cg) || (in.cols && in.cols != width) || (in.ksplit ? in.ksplit != ks : in.cols && ks != 1))
                         continue;
                     const bool v_mn = swap ? in.a_mn : in.b_mn;
                     if(cg == 1 && v_mn && width != 128) // an MN-major tile is 128 columns wide
@@ -218,7 +220,7 @@ inline bool plan_scaled(const ScaledPlanInput& in, ScaledPlan* out)
                     const int units = cg == 2 ? in.sm_count / 2 : ks == 1 ? in.sm_count : in.cluster_cap[ks == 2 ? 0 : ks == 4 ? 1 : 2];
                     if(units < 1)
                         continue;
-                    const int vmode   = scaled_vmode(swap ? in.b_block : in.a_block, swap ? in.a_block : in.b_block);
+                    const int vmode   = scaled_vmode(swap ? in.a_block : in.b_block);
                     const double per  = scaled_kb_cycles(cg, width, vmode, v_mn);
                     const double waves = static_cast<double>((static_cast<int64_t>(tiles) + units - 1) / units);
                     const int n_kb    = static_cast<int>((kb + ks - 1) / ks);
@@ -231,6 +233,7 @@ inline bool plan_scaled(const ScaledPlanInput& in, ScaledPlan* out)
                         found = true;
                     }
                 }
+    }
     return found;
 }
 

@@ -336,11 +336,11 @@ typedef struct ckb_scaled_gemm_desc {
 } ckb_scaled_gemm_desc;
 
 /* Pins the tile of an 8-bit product: `cols` columns of the narrower tile side and `cg` CTAs per tile.
- *   cg = 2  a CTA pair on 256 x cols, cols = 64, 96 .. 256; `swap` = 1 puts the columns of B on the 256 side
+ *   cg = 2  a CTA pair on 256 rows of A x cols columns of B, cols = 128, 192, 224 or 256
  *   cg = 1  128 columns of B x cols rows of A, cols = 16, 32, 64 or 128; ksplit = 2, 4 or 8 cuts K over a cluster
  *           of as many CTAs (plain products only; slices of two K blocks at least)
  * 0 leaves the choice to the library; a pin that the problem cannot use is refused. */
-#define CKB_SCALED_TILE(cols, cg, swap, ksplit) ((cols) | ((cg) << 12) | ((swap) << 16) | ((ksplit) << 20))
+#define CKB_SCALED_TILE(cols, cg, ksplit) ((cols) | ((cg) << 12) | ((ksplit) << 20))
 
 int ckb_scaled_gemm_supported(const ckb_scaled_gemm_desc* desc);
 /* n_rep / avg_ms as ckb_gemm_run.  Uses no scratch and allocates nothing: it may be captured into a graph (after one

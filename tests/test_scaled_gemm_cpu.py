@@ -45,18 +45,19 @@ def test_scaled_gemm_rules():
 
 
 def test_scaled_gemm_pinned_tiles():
-    for tile in (capi.scaled_tile(16, 1), capi.scaled_tile(128, 1, 0, 1), capi.scaled_tile(64, 2), capi.scaled_tile(224, 2, 1)):
+    for tile in (capi.scaled_tile(16, 1), capi.scaled_tile(128, 1, 1), capi.scaled_tile(128, 2), capi.scaled_tile(224, 2)):
         op, arg = gemm(tile=tile)
         assert op.IsSupportedArgument(arg), capi.last_error()
     refused(*gemm(tile=capi.scaled_tile(48, 1)), "no tile fits")
     refused(*gemm(tile=capi.scaled_tile(240, 2)), "no tile fits")
     refused(*gemm(tile=capi.scaled_tile(16, 1), a_layout=COL, sa=64), "no tile fits")     # an M-contiguous A needs 128 columns
-    refused(*gemm(tile=capi.scaled_tile(16, 1, 0, 2)), "no tile fits")                   # two K blocks per slice at least
-    refused(*gemm(tile=capi.scaled_tile(16, 1, 1)), "CKB_SCALED_TILE")
+    refused(*gemm(tile=capi.scaled_tile(16, 1, 2)), "no tile fits")                   # two K blocks per slice at least
+    refused(*gemm(tile=capi.scaled_tile(256, 2) | 1 << 16), "CKB_SCALED_TILE")
+    refused(*gemm(tile=capi.scaled_tile(256, 2, 2)), "no tile fits")
     refused(*gemm(tile=capi.scaled_tile(16, 3)), "CKB_SCALED_TILE")
     refused(*gemm(tile=16), "CKB_SCALED_TILE")
     refused(*gemm(tile=-1), "CKB_SCALED_TILE")
-    refused(*gemm(tile=capi.scaled_tile(16, 1, 0, 3)), "CKB_SCALED_TILE")
+    refused(*gemm(tile=capi.scaled_tile(16, 1, 3)), "CKB_SCALED_TILE")
 
 
 def test_scaled_gemm_pointers_are_checked_before_a_launch():
