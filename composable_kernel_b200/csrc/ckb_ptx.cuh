@@ -440,7 +440,7 @@ __device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t* v)
                  : "r"(taddr)
                  : "memory");
 }
-// 16 lanes x 8, 16 or 32 columns as fragments: of every 8 columns, thread t receives row t / 4, columns 2 (t % 4) and the next
+// 16 lanes x 16 or 32 columns as fragments: of every 8 columns, thread t receives row t / 4, columns 2 (t % 4) and the next
 // one in v[4 q], v[4 q + 1], and the same columns of row t / 4 + 8 in v[4 q + 2], v[4 q + 3] (q: which 8 columns).
 __device__ __forceinline__ void tmem_ld_16x256b_x4(uint32_t taddr, uint32_t* v)
 {
@@ -448,13 +448,6 @@ __device__ __forceinline__ void tmem_ld_16x256b_x4(uint32_t taddr, uint32_t* v)
                  "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
                  : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
                    "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-                 : "r"(taddr)
-                 : "memory");
-}
-__device__ __forceinline__ void tmem_ld_16x256b_x1(uint32_t taddr, uint32_t* v)
-{
-    asm volatile("tcgen05.ld.sync.aligned.16x256b.x1.b32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
                  : "r"(taddr)
                  : "memory");
 }

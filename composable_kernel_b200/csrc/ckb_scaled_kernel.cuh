@@ -11,7 +11,7 @@
 //              commit's barrier tells the producer that the stage is free and the epilogue warps that the accumulator is
 //              complete.  A wait costs this thread about 80 cycles even if nothing is waited for
 //   warps 2, 3 bring the scales into a ring in shared memory
-//   warps 4-   two or four per lane quarter, each its part of the columns: load the accumulator, release it, fused multiply-add
+//   warps 4-11 two per lane quarter, each half of the columns: load the accumulator, release it, fused multiply-add
 //              into the sums (two values per instruction).  They issue no global loads: a hand-over behind one would
 //              wait for it (the first version, which loaded its scales itself and released the accumulator with a
 //              cluster-scope release, took 2300 cycles per K block).
@@ -62,21 +62,23 @@ struct ScaledParams
     uint32_t* status;
 };
 
-// Warps 0-3 (producer, MMA issuer, two for the scales) form one warpgroup.  Tiles of 128 columns and more have sixteen
-// epilogue warps, a quarter of the columns each: adding 128 x 256 values to the sums keeps the multiply-add pipes of an SM
-// busy for about 330 cycles, but a warp needs 680 from its wait to its last addition, mostly latency, and four warps
-// per scheduler overlap more of it than two.  20 warps get 96 registers each at launch; where 64 sums per lane need more,
-// the first warpgroup gives some of its own away (64 + 4 x 104 = 5 x 96).
+// Warps 0-3 (producer, MMA issuer, two for the scales) form one warpgroup, the epilogue warps two more, so that registers
+// can be dealt out unevenly: 128 sums per lane (BN = 256) next to a chunk of 32 accumulator columns, addresses and scales
+// do not fit the 168 that twelve warps get at launch, and spills in the first warpgroup cost as much as in the others.
+// What the K loop of an epilogue warp costs is instructions, not arithmetic: about 190 per K block for 64 packed
+// multiply-adds, 5 cycles each.  Sixteen warps with a quarter of the columns each repeat the hand-overs of eight (511
+// against 436 ns per K block of a 256 x 256 tile), and groups of four K blocks unrolled with fixed stages save
+// instructions but not time (424; the loops no longer fit the instruction caches: 365 against 282 at BN = 16).
 constexpr int SCALED_EPI_WARP0 = 4;
-constexpr int SCALED_REGS_LOW = 64, SCALED_REGS_HIGH = 104;
 
 template <int BN, int CG>
 struct ScaledSmem
 {
-    static constexpr int EPI_WARPS   = BN >= 128 ? 16 : 8;
+    static constexpr int EPI_WARPS   = 8;
     static constexpr int THREADS     = 32 * (SCALED_EPI_WARP0 + EPI_WARPS);
-    static constexpr bool SPLIT_REGS = BN >= 192;
-    static_assert(!SPLIT_REGS || SCALED_REGS_LOW + 4 * SCALED_REGS_HIGH <= 5 * 96, "shares of what the block is launched with");
+    static constexpr bool SPLIT_REGS = BN >= 128;
+    static constexpr int REGS_LOW = BN == 128 ? 72 : 56, REGS_HIGH = BN == 128 ? 216 : 224;
+    static_assert(REGS_LOW + 2 * REGS_HIGH == 3 * 168, "the shares add up to what the block is launched with");
     static constexpr int U_BYTES     = 128 * BK_BYTES;
     // (a pair's CTA always has room for 128 rows: an MN-major box is that wide whatever the tile)
     static constexpr int V_BYTES     = (CG == 2 ? 128 : BN) * BK_BYTES;
@@ -284,7 +286,7 @@ __global__ void __launch_bounds__(ScaledSmem<BN, CG>::THREADS, 1) scaled_kernel(
     constexpr uint32_t ACC_COLS = L::ACC_COLS;
     constexpr int SLOTS         = L::SLOTS;
     constexpr int SCALE_BATCH   = L::SCALE_BATCH;
-    constexpr int CHUNK         = COLS < 16 ? COLS : 16;
+    constexpr int CHUNK         = COLS < 32 ? COLS : 32;
     constexpr bool STRADDLES    = 128 % COLS != 0; // a warp's columns may touch two blocks of 128
     // Scales per column: with a row per lane every lane reads every column's scale, 512 bytes per four columns and warp,
     // and shared memory takes twice as long as the sums (640 cycles for 128 columns, 365 with a scale per row); in
@@ -416,7 +418,7 @@ __global__ void __launch_bounds__(ScaledSmem<BN, CG>::THREADS, 1) scaled_kernel(
     if(warp < SCALED_EPI_WARP0)
     {
     if constexpr(L::SPLIT_REGS)
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(SCALED_REGS_LOW));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::REGS_LOW));
     if(warp == 0)
     {
         // ------------------------------------------------------------------ TMA producer
@@ -631,7 +633,7 @@ __global__ void __launch_bounds__(ScaledSmem<BN, CG>::THREADS, 1) scaled_kernel(
     else
     {
         if constexpr(L::SPLIT_REGS)
-            asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SCALED_REGS_HIGH));
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L::REGS_HIGH));
         // ------------------------------------------------------------------ epilogue warps
         const int quarter = warp & 3, part = (warp - SCALED_EPI_WARP0) >> 2;
         const int row     = quarter * 32 + lane; // lane of the accumulator
@@ -714,15 +716,20 @@ __global__ void __launch_bounds__(ScaledSmem<BN, CG>::THREADS, 1) scaled_kernel(
                 // N columns from column c on, from tensor memory into v, and from v into the sums
                 auto load = [&](auto width, int c, uint32_t* v) {
                     constexpr int N = decltype(width)::value;
-                    if constexpr(FRAG && N == 16)
+                    if constexpr(FRAG && N == 32)
+                    {
+                        tmem_ld_16x256b_x4(taddr + c, v);
+                        tmem_ld_16x256b_x4(taddr + c + (16u << 16), v + 16);
+                    }
+                    else if constexpr(N == 32)
+                    {
+                        tmem_ld_32x32b_x16(taddr + c, v);
+                        tmem_ld_32x32b_x16(taddr + c + 16, v + 16);
+                    }
+                    else if constexpr(FRAG && N == 16)
                     {
                         tmem_ld_16x256b_x2(taddr + c, v);
                         tmem_ld_16x256b_x2(taddr + c + (16u << 16), v + 8);
-                    }
-                    else if constexpr(FRAG)
-                    {
-                        tmem_ld_16x256b_x1(taddr + c, v);
-                        tmem_ld_16x256b_x1(taddr + c + (16u << 16), v + 4);
                     }
                     else if constexpr(N == 16)
                         tmem_ld_32x32b_x16(taddr + c, v);
@@ -768,7 +775,7 @@ __global__ void __launch_bounds__(ScaledSmem<BN, CG>::THREADS, 1) scaled_kernel(
                     }
                 };
                 // (a chunk in flight while another is added was slower: the warps of a scheduler hide each other's loads)
-                constexpr int LAST = COLS % CHUNK == 0 ? CHUNK : COLS % CHUNK; // BN = 224: 8
+                constexpr int LAST = COLS % CHUNK == 0 ? CHUNK : COLS % CHUNK; // BN = 224: 16
 #pragma unroll
                 for(int c = 0; c + CHUNK <= COLS; c += CHUNK)
                 {

@@ -28,7 +28,7 @@ cudaError_t launch_scaled_one(const ScaledParams& p, int grid, cudaStream_t stre
             err = cudaFuncGetAttributes(&fa, kern);
             if(err != cudaSuccess)
                 return err;
-            if(fa.numRegs * 5 < SCALED_REGS_LOW + 4 * SCALED_REGS_HIGH)
+            if(fa.numRegs * 3 < ScaledSmem<BN, CG>::REGS_LOW + 2 * ScaledSmem<BN, CG>::REGS_HIGH)
                 return cudaErrorInvalidConfiguration;
         }
         if(dev >= 0 && dev < 64)
