@@ -75,6 +75,18 @@ __device__ __forceinline__ void copy_async_4(uint32_t dst, const void* src, uint
 {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
+// 16 bytes of which the first `bytes` are read and the others zero.
+__device__ __forceinline__ void copy_async_16(uint32_t dst, const void* src, uint32_t bytes)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Waits until at most N of this thread's groups are incomplete.
+template <int N>
+__device__ __forceinline__ void copy_async_wait()
+{
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
 // One arrival of this thread on `bar` (counted at its initialisation) once its copies so far have landed.
 __device__ __forceinline__ void copy_async_arrive(uint32_t bar)
 {

@@ -75,16 +75,38 @@ __device__ __forceinline__ void store8(const float (&f)[8], T* p, int n, bool ve
 }
 
 // ---- 8-bit blocks ------------------------------------------------------------------------------
-// Magnitudes are compared as bit patterns: NaN > infinity > numbers, so neither is lost in the maximum.
-__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-
-__device__ __forceinline__ float block_scale(uint32_t amax_bits, float qmax, bool pow2)
+// Largest magnitude so far; a NaN stays (an infinity is larger than any number anyway), so that neither is lost.
+__device__ __forceinline__ float max_abs(float m, float v)
 {
-    if(amax_bits == 0)
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(v)));
+    return r;
+}
+__device__ __forceinline__ float max16(float v) // over 16 neighbouring lanes
+{
+#pragma unroll
+    for(int d = 8; d >= 1; d >>= 1)
+        v = max_abs(v, __shfl_xor_sync(0xffffffffu, v, d));
+    return v;
+}
+
+// amax / qmax, correctly rounded (see below), at least the smallest normal number (its reciprocal still exists).
+__device__ __forceinline__ float block_scale(float amax, float qmax, float qmax_recip, bool pow2)
+{
+    if(amax == 0.f)
         return 1.f;
-    float s = __fdiv_rn(__uint_as_float(amax_bits), qmax);
-    if(s < 1.17549435e-38f) // the smallest normal number: its reciprocal still exists (NaN passes)
-        s = 1.17549435e-38f;
+    float s;
+    if(amax >= 1e-28f && amax <= 3.402823466e+38f)
+    {
+        const float q0 = amax * qmax_recip;
+        s              = __fmaf_rn(__fmaf_rn(-q0, qmax, amax), qmax_recip, q0);
+    }
+    else // tiny, infinite or NaN
+    {
+        s = __fdiv_rn(amax, qmax);
+        if(s < 1.17549435e-38f)
+            s = 1.17549435e-38f;
+    }
     if(pow2)
     {
         const uint32_t b = __float_as_uint(s);
@@ -121,9 +143,9 @@ __device__ __forceinline__ uint32_t to_f8x2(float lo, float hi)
     return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, E5M2 ? __NV_E5M2 : __NV_E4M3);
 }
 
-// Eight values over one scale -> eight bytes.
+// Eight values (four pairs) over one scale -> eight bytes.
 template <bool E5M2>
-__device__ __forceinline__ uint2 quantize8(const float (&f)[8], const BlockDivisor& d)
+__device__ __forceinline__ uint2 quantize8(const uint64_t (&f)[4], const BlockDivisor& d)
 {
     uint32_t w[4];
     if(d.fast)
@@ -133,7 +155,7 @@ __device__ __forceinline__ uint2 quantize8(const float (&f)[8], const BlockDivis
         for(int i = 0; i < 4; ++i)
         {
             float lo, hi;
-            unpack_f32x2(div_pair(pack_f32x2(f[2 * i], f[2 * i + 1]), ns, r), lo, hi);
+            unpack_f32x2(div_pair(f[i], ns, r), lo, hi);
             w[i] = to_f8x2<E5M2>(lo, hi);
         }
     }
@@ -141,9 +163,42 @@ __device__ __forceinline__ uint2 quantize8(const float (&f)[8], const BlockDivis
     {
 #pragma unroll
         for(int i = 0; i < 4; ++i)
-            w[i] = to_f8x2<E5M2>(__fdiv_rn(f[2 * i], d.scale), __fdiv_rn(f[2 * i + 1], d.scale));
+        {
+            float lo, hi;
+            unpack_f32x2(f[i], lo, hi);
+            w[i] = to_f8x2<E5M2>(__fdiv_rn(lo, d.scale), __fdiv_rn(hi, d.scale));
+        }
     }
     return make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+}
+
+// The eight values of a vector as pairs, and their largest magnitude.
+template <typename T>
+__device__ __forceinline__ void to_pairs(const Vec8<T>& r, uint64_t (&f)[4])
+{
+#pragma unroll
+    for(int i = 0; i < 4; ++i)
+        f[i] = pack_f32x2(to_f32(r.v[2 * i]), to_f32(r.v[2 * i + 1]));
+}
+__device__ __forceinline__ float max_abs8(const Vec8<float>& r)
+{
+    float m = 0.f;
+#pragma unroll
+    for(int i = 0; i < 8; ++i)
+        m = max_abs(m, r.v[i]);
+    return m;
+}
+__device__ __forceinline__ float max_abs8(const Vec8<__half>& r)
+{
+    const __half2* h = reinterpret_cast<const __half2*>(&r);
+    const __half2 m  = __hmax2_nan(__hmax2_nan(__habs2(h[0]), __habs2(h[1])), __hmax2_nan(__habs2(h[2]), __habs2(h[3])));
+    return max_abs(__low2float(m), __high2float(m));
+}
+__device__ __forceinline__ float max_abs8(const Vec8<__nv_bfloat16>& r)
+{
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&r);
+    const __nv_bfloat162 m  = __hmax2_nan(__hmax2_nan(__habs2(h[0]), __habs2(h[1])), __hmax2_nan(__habs2(h[2]), __habs2(h[3])));
+    return max_abs(__low2float(m), __high2float(m));
 }
 
 __device__ __forceinline__ void store_q8(uint2 w, uint8_t* p, int n, bool vec)
@@ -159,14 +214,6 @@ __device__ __forceinline__ void store_q8(uint2 w, uint8_t* p, int n, bool vec)
     }
 }
 
-__device__ __forceinline__ uint32_t max16(uint32_t v) // over 16 neighbouring lanes
-{
-#pragma unroll
-    for(int d = 8; d >= 1; d >>= 1)
-        v = max(v, __shfl_xor_sync(0xffffffffu, v, d));
-    return v;
-}
-
 struct QuantizeParams
 {
     const void* x;
@@ -179,7 +226,7 @@ struct QuantizeParams
     int32_t total;    // blocks (1 x 128), or tiles of 128 x 128
     int32_t pow2;
     int32_t x_vec, q_vec;
-    float qmax;
+    float qmax, qmax_recip;
 };
 __device__ __forceinline__ int32_t block_row(const QuantizeParams& p, int32_t b)
 {
@@ -213,17 +260,11 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const __grid_constan
 #pragma unroll
         for(int j = 0; j < QB; ++j)
         {
-            float f[8];
-            uint32_t m = 0;
-#pragma unroll
-            for(int i = 0; i < 8; ++i)
-            {
-                f[i] = to_f32(raw[j].v[i]);
-                m    = max(m, magnitude(f[i]));
-            }
-            const float s = block_scale(max16(m), P.qmax, P.pow2 != 0);
+            const float s = block_scale(max16(max_abs8(raw[j])), P.qmax, P.qmax_recip, P.pow2 != 0);
             if(n[j] <= -1000)
                 continue; // (all 16 lanes of the block)
+            uint64_t f[4];
+            to_pairs(raw[j], f);
             const uint2 w = quantize8<E5M2>(f, BlockDivisor(s));
             store_q8(w, P.q + row[j] * P.ldq + c0[j], n[j], P.q_vec != 0);
             if(sub == 0)
@@ -239,7 +280,7 @@ __global__ void __launch_bounds__(256) quantize_tile_kernel(const __grid_constan
 {
     grid_dependency_wait();
     grid_launch_dependents();
-    __shared__ uint32_t s_max[SQUARE ? 16 : 16 * 128];
+    __shared__ float s_max[SQUARE ? 16 : 16 * 128];
     const T* x     = static_cast<const T*>(P.x);
     const int sub  = threadIdx.x & 15;
     const int unit = threadIdx.x >> 4;
@@ -255,21 +296,21 @@ __global__ void __launch_bounds__(256) quantize_tile_kernel(const __grid_constan
             const int r = br * 128 + i * 16 + unit;
             load8(raw[i], x + r * P.ldx + c0, r < P.M ? n : 0, P.x_vec != 0);
         }
+        uint64_t nscale[4], recip[4]; // of this thread's columns (SQUARE: all the same)
+        bool fast = true;
         float scale[8];
         if constexpr(SQUARE)
         {
-            uint32_t m = 0;
+            float m = 0.f;
 #pragma unroll
             for(int i = 0; i < 8; ++i)
-#pragma unroll
-                for(int k = 0; k < 8; ++k)
-                    m = max(m, magnitude(to_f32(raw[i].v[k])));
+                m = max_abs(m, max_abs8(raw[i]));
             m = max16(m);
             if(sub == 0)
                 s_max[unit] = m;
             __syncthreads();
             m        = max16(s_max[sub]);
-            scale[0] = block_scale(m, P.qmax, P.pow2 != 0);
+            scale[0] = block_scale(m, P.qmax, P.qmax_recip, P.pow2 != 0);
             if(threadIdx.x == 0)
                 P.scale[br * P.ss_m + bc * P.ss_n] = scale[0];
         }
@@ -278,24 +319,36 @@ __global__ void __launch_bounds__(256) quantize_tile_kernel(const __grid_constan
 #pragma unroll
             for(int k = 0; k < 8; ++k)
             {
-                uint32_t m = 0;
+                float m = 0.f;
 #pragma unroll
                 for(int i = 0; i < 8; ++i)
-                    m = max(m, magnitude(to_f32(raw[i].v[k])));
+                    m = max_abs(m, to_f32(raw[i].v[k]));
                 s_max[unit * 128 + k * 16 + sub] = m; // [unit][k][sub]: lanes write neighbouring words
+            }
+            __syncthreads();
+            if(threadIdx.x < 128)
+            {
+                float m = 0.f;
+#pragma unroll
+                for(int u = 0; u < 16; ++u)
+                    m = max_abs(m, s_max[u * 128 + threadIdx.x]);
+                const float sc = block_scale(m, P.qmax, P.qmax_recip, P.pow2 != 0);
+                s_max[threadIdx.x] = sc; // (only this thread reads or writes the column's words now)
+                const int k = threadIdx.x >> 4, c = bc * 128 + (threadIdx.x & 15) * 8 + k;
+                if(c < P.N)
+                    P.scale[br * P.ss_m + c * P.ss_n] = sc;
             }
             __syncthreads();
 #pragma unroll
             for(int k = 0; k < 8; ++k)
-            {
-                // every thread needs the scales of its own eight columns
-                uint32_t m = 0;
+                scale[k] = s_max[k * 16 + sub];
 #pragma unroll
-                for(int u = 0; u < 16; ++u)
-                    m = max(m, s_max[u * 128 + k * 16 + sub]);
-                scale[k] = block_scale(m, P.qmax, P.pow2 != 0);
-                if(unit == 0 && k < n)
-                    P.scale[br * P.ss_m + (c0 + k) * P.ss_n] = scale[k];
+            for(int k = 0; k < 4; ++k)
+            {
+                const BlockDivisor lo(scale[2 * k]), hi(scale[2 * k + 1]);
+                nscale[k] = pack_f32x2(-lo.scale, -hi.scale);
+                recip[k]  = pack_f32x2(lo.recip, hi.recip);
+                fast      = fast && lo.fast && hi.fast;
             }
         }
 #pragma unroll
@@ -304,10 +357,8 @@ __global__ void __launch_bounds__(256) quantize_tile_kernel(const __grid_constan
             const int r = br * 128 + i * 16 + unit;
             if(r >= P.M)
                 break;
-            float f[8];
-#pragma unroll
-            for(int k = 0; k < 8; ++k)
-                f[k] = to_f32(raw[i].v[k]);
+            uint64_t f[4];
+            to_pairs(raw[i], f);
             uint2 w;
             if constexpr(SQUARE)
                 w = quantize8<E5M2>(f, BlockDivisor(scale[0]));
@@ -315,8 +366,19 @@ __global__ void __launch_bounds__(256) quantize_tile_kernel(const __grid_constan
             {
                 uint32_t h[4];
 #pragma unroll
-                for(int k = 0; k < 8; k += 2)
-                    h[k / 2] = to_f8x2<E5M2>(__fdiv_rn(f[k], scale[k]), __fdiv_rn(f[k + 1], scale[k + 1]));
+                for(int k = 0; k < 4; ++k)
+                {
+                    float lo, hi;
+                    if(fast)
+                        unpack_f32x2(div_pair(f[k], nscale[k], recip[k]), lo, hi);
+                    else
+                    {
+                        unpack_f32x2(f[k], lo, hi);
+                        lo = __fdiv_rn(lo, scale[2 * k]);
+                        hi = __fdiv_rn(hi, scale[2 * k + 1]);
+                    }
+                    h[k] = to_f8x2<E5M2>(lo, hi);
+                }
                 w = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
             }
             store_q8(w, P.q + r * P.ldq + c0, n, P.q_vec != 0);
@@ -362,6 +424,40 @@ __device__ __forceinline__ float rstd_of(float square, float shift, float eps)
     return __frsqrt_rn((var < 0.f ? 0.f : var) + eps); // (a NaN stays one)
 }
 
+// Rows on their way: asynchronous copies into shared memory, DEPTH rows ahead.  Every thread copies the vectors it works
+// on itself and reads nobody else's, so only its own copies have to be waited for.  Vector v of thread t lies in pieces of
+// 16 bytes, [row of the ring][vector][piece][thread].
+constexpr int STAGE_DEPTH = 3;
+template <typename T, int V>
+struct RowRing
+{
+    static constexpr int PIECES = sizeof(T) / 2; // 16-byte pieces of a vector
+    uint32_t base;                               // this thread's first piece
+    int threads;
+    static __host__ __device__ int bytes(int threads) { return STAGE_DEPTH * V * PIECES * threads * 16; }
+    // `n` = values of the row from the vector's first one on
+    __device__ __forceinline__ void copy(int slot, int v, const T* p, int n) const
+    {
+#pragma unroll
+        for(int i = 0; i < PIECES; ++i)
+        {
+            constexpr int PER = 16 / static_cast<int>(sizeof(T));
+            const int have    = n - i * PER < 0 ? 0 : n - i * PER > PER ? PER : n - i * PER;
+            copy_async_16(base + (((slot * V + v) * PIECES + i) * threads) * 16, have > 0 ? p + i * PER : p, have * static_cast<int>(sizeof(T)));
+        }
+    }
+    __device__ __forceinline__ void read(Vec8<T>& r, int slot, int v) const
+    {
+        uint32_t* d = reinterpret_cast<uint32_t*>(&r);
+#pragma unroll
+        for(int i = 0; i < PIECES; ++i)
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(d[4 * i]), "=r"(d[4 * i + 1]), "=r"(d[4 * i + 2]), "=r"(d[4 * i + 3])
+                         : "r"(base + (((slot * V + v) * PIECES + i) * threads) * 16)
+                         : "memory");
+    }
+};
+
 struct LayernormFwdParams
 {
     const void *x, *gamma, *beta;
@@ -372,57 +468,58 @@ struct LayernormFwdParams
     int64_t M;
     int32_t N;
     int32_t w_f32, x_vec, y_vec, q_vec, w_vec;
-    float eps, qmax;
+    float eps, qmax, qmax_recip;
 };
 
-// Weights of columns c .. c + 7 (or every `step`-th from c) in 32 bits.
+// Weights of columns c .. c + 7 in 32 bits.
 template <typename T>
-__device__ __forceinline__ void load_weights8(float (&f)[8], const void* w, bool f32, int c, int N, bool vec, float none)
+__device__ __forceinline__ void load_weights8(uint64_t (&f)[4], const void* w, bool f32, int c, int N, bool vec, float none)
 {
     if(!w)
     {
 #pragma unroll
-        for(int i = 0; i < 8; ++i)
-            f[i] = none;
+        for(int i = 0; i < 4; ++i)
+            f[i] = pack_f32x2(none, none);
     }
     else if(f32)
     {
         Vec8<float> r;
         load8(r, static_cast<const float*>(w) + c, N - c, vec);
-#pragma unroll
-        for(int i = 0; i < 8; ++i)
-            f[i] = r.v[i];
+        to_pairs(r, f);
     }
     else
     {
         Vec8<T> r;
         load8(r, static_cast<const T*>(w) + c, N - c, vec);
-#pragma unroll
-        for(int i = 0; i < 8; ++i)
-            f[i] = to_f32(r.v[i]);
+        to_pairs(r, f);
     }
 }
 
 // y (and q) of 8 columns from their distances to the mean.
 template <typename T, bool E5M2>
-__device__ __forceinline__ void layernorm_out8(const LayernormFwdParams& P, int64_t row, int c, float (&d)[8], float rstd)
+__device__ __forceinline__ void layernorm_out8(const LayernormFwdParams& P, int64_t row, int c, uint64_t (&d)[4], float rstd)
 {
     const int n = P.N - c;
-    float g[8], b[8];
+    uint64_t g[4], b[4];
     load_weights8<T>(g, P.gamma, P.w_f32 != 0, c, P.N, P.w_vec != 0, 1.f);
     load_weights8<T>(b, P.beta, P.w_f32 != 0, c, P.N, P.w_vec != 0, 0.f);
+    const uint64_t r2 = pack_f32x2(rstd, rstd);
+    float y[8];
 #pragma unroll
-    for(int i = 0; i < 8; ++i)
-        d[i] = __fmaf_rn(d[i] * rstd, g[i], b[i]);
+    for(int i = 0; i < 4; ++i)
+    {
+        d[i] = fma_f32x2(mul_f32x2(d[i], r2), g[i], b[i]);
+        unpack_f32x2(d[i], y[2 * i], y[2 * i + 1]);
+    }
     if(P.y)
-        store8(d, static_cast<T*>(P.y) + row * P.ldy + c, n, P.y_vec != 0);
+        store8(y, static_cast<T*>(P.y) + row * P.ldy + c, n, P.y_vec != 0);
     if(P.q)
     {
-        uint32_t m = 0;
+        float m = 0.f;
 #pragma unroll
         for(int i = 0; i < 8; ++i)
-            m = max(m, i < n ? magnitude(d[i]) : 0u);
-        const float s = block_scale(max16(m), P.qmax, false);
+            m = max_abs(m, n >= 8 || i < n ? y[i] : 0.f);
+        const float s = block_scale(max16(m), P.qmax, P.qmax_recip, false);
         const uint2 w = quantize8<E5M2>(d, BlockDivisor(s));
         store_q8(w, P.q + row * P.ldq + c, n, P.q_vec != 0);
         if((threadIdx.x & 15) == 0 && n > 0)
@@ -430,15 +527,48 @@ __device__ __forceinline__ void layernorm_out8(const LayernormFwdParams& P, int6
     }
 }
 
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float sum_f32x2(uint64_t a)
+{
+    float lo, hi;
+    unpack_f32x2(a, lo, hi);
+    return lo + hi;
+}
+// Subtracts `mean` from the eight values, zero where there is no value (n of them exist).
+__device__ __forceinline__ void distances(uint64_t (&d)[4], float mean, int n)
+{
+    const uint64_t m2 = pack_f32x2(-mean, -mean);
+#pragma unroll
+    for(int i = 0; i < 4; ++i)
+        d[i] = add_f32x2(d[i], m2);
+    if(n < 8)
+    {
+#pragma unroll
+        for(int i = 0; i < 4; ++i)
+        {
+            float lo, hi;
+            unpack_f32x2(d[i], lo, hi);
+            d[i] = pack_f32x2(2 * i < n ? lo : 0.f, 2 * i + 1 < n ? hi : 0.f);
+        }
+    }
+}
+
 // A row per warp (WARP, eight rows a CTA) or per CTA, V vectors of 8 values a thread: vector v of thread t holds columns
-// 8 (v * threads + t) .. + 7.  The next row's values are on their way while this one is worked on.
+// 8 (v * threads + t) .. + 7.  RING: rows come through shared memory, STAGE_DEPTH - 1 rows ahead (with one row ahead in
+// registers three CTAs per SM have 30 KB on their way, half of what the memory needs: 8192 x 5120 took 90 us).
 // Mean and variance in two passes over the registers; the second pass also sums the distances themselves, which takes
 // the rounding of the first mean out of both.
-template <typename T, bool E5M2, int V, bool WARP>
-__global__ void __launch_bounds__(WARP || V == 2 ? 256 : 512) layernorm_fwd_kernel(const __grid_constant__ LayernormFwdParams P)
+template <typename T, bool E5M2, int V, bool WARP, bool RING>
+__global__ void __launch_bounds__(WARP ? 256 : 512, WARP || V == 4 ? 1 : 2) layernorm_fwd_kernel(const __grid_constant__ LayernormFwdParams P)
 {
     grid_dependency_wait();
     grid_launch_dependents();
+    extern __shared__ __align__(16) uint8_t ring_smem[];
     __shared__ float buf[4 * 64];
     const int tpr      = WARP ? 32 : static_cast<int>(blockDim.x);
     const int t        = WARP ? static_cast<int>(threadIdx.x) & 31 : static_cast<int>(threadIdx.x);
@@ -447,48 +577,65 @@ __global__ void __launch_bounds__(WARP || V == 2 ? 256 : 512) layernorm_fwd_kern
     const T* x         = static_cast<const T*>(P.x);
     const float inv_n  = 1.f / static_cast<float>(P.N);
     Vec8<T> raw[V];
-    auto fetch = [&](int64_t r) {
+    RowRing<T, V> ring{smem_u32(ring_smem) + t * 16, tpr};
+    auto fetch = [&](int64_t r, int slot) {
 #pragma unroll
         for(int v = 0; v < V; ++v)
         {
-            const int c = (v * tpr + t) * 8;
-            load8(raw[v], x + r * P.ldx + c, r < P.M ? P.N - c : 0, P.x_vec != 0);
+            const int c = (v * tpr + t) * 8, n = r < P.M ? P.N - c : 0;
+            const T* p  = x + (n > 0 ? r * P.ldx + c : 0);
+            if constexpr(RING)
+                ring.copy(slot, v, p, n);
+            else
+                load8(raw[v], p, n, P.x_vec != 0);
         }
+        if constexpr(RING)
+            copy_async_commit();
     };
-    fetch(row);
+    int slot = 0;
+    fetch(row, 0);
+    if constexpr(RING)
+#pragma unroll
+        for(int i = 1; i < STAGE_DEPTH - 1; ++i)
+            fetch(row + i * step, i);
     int flip = 0;
     for(; row < P.M; row += step)
     {
-        float d[V][8];
+        if constexpr(RING)
+        {
+            fetch(row + (STAGE_DEPTH - 1) * step, slot == 0 ? STAGE_DEPTH - 1 : slot - 1);
+            copy_async_wait<STAGE_DEPTH - 1>();
+#pragma unroll
+            for(int v = 0; v < V; ++v)
+                ring.read(raw[v], slot, v);
+            if(++slot == STAGE_DEPTH)
+                slot = 0;
+        }
+        uint64_t d[V][4];
         float sum = 0.f, none = 0.f;
 #pragma unroll
         for(int v = 0; v < V; ++v)
         {
-            float part = 0.f;
-#pragma unroll
-            for(int i = 0; i < 8; ++i)
-            {
-                d[v][i] = to_f32(raw[v].v[i]);
-                part += d[v][i];
-            }
-            sum += part;
+            to_pairs(raw[v], d[v]);
+            sum += sum_f32x2(add_f32x2(add_f32x2(d[v][0], d[v][1]), add_f32x2(d[v][2], d[v][3])));
         }
-        fetch(row + step);
+        if constexpr(!RING)
+            fetch(row + step, 0);
         row_sum2<WARP>(sum, none, buf + flip);
         float mean = sum * inv_n;
-        float s1 = 0.f, s2 = 0.f;
+        uint64_t s1v = 0, s2v = 0;
 #pragma unroll
         for(int v = 0; v < V; ++v)
         {
-            const int n = P.N - (v * tpr + t) * 8;
+            distances(d[v], mean, P.N - (v * tpr + t) * 8);
 #pragma unroll
-            for(int i = 0; i < 8; ++i)
+            for(int i = 0; i < 4; ++i)
             {
-                d[v][i] = i < n ? d[v][i] - mean : 0.f;
-                s1 += d[v][i];
-                s2 = __fmaf_rn(d[v][i], d[v][i], s2);
+                s1v = add_f32x2(s1v, d[v][i]);
+                s2v = fma_f32x2(d[v][i], d[v][i], s2v);
             }
         }
+        float s1 = sum_f32x2(s1v), s2 = sum_f32x2(s2v);
         row_sum2<WARP>(s1, s2, buf + 64 + flip);
         const float shift = s1 * inv_n;
         const float rstd  = rstd_of(s2 * inv_n, shift, P.eps);
@@ -506,12 +653,14 @@ __global__ void __launch_bounds__(WARP || V == 2 ? 256 : 512) layernorm_fwd_kern
             if(__all_sync(0xffffffffu, P.N - (v * tpr + t) * 8 <= 0))
                 continue;
 #pragma unroll
-            for(int i = 0; i < 8; ++i)
-                d[v][i] -= shift;
+            for(int i = 0; i < 4; ++i)
+                d[v][i] = add_f32x2(d[v][i], pack_f32x2(-shift, -shift));
             layernorm_out8<T, E5M2>(P, row, (v * tpr + t) * 8, d[v], rstd);
         }
         flip ^= 128;
     }
+    if constexpr(RING)
+        copy_async_wait_all();
 }
 
 // Rows that do not fit the registers of a CTA: the row is read three times (the second and third time from L2).
@@ -571,10 +720,10 @@ __global__ void __launch_bounds__(1024) layernorm_fwd_long_kernel(const __grid_c
             // (a lane behind the row's end takes part in the shuffles with zeros)
             const int cc = c < P.N ? static_cast<int>(c) : P.N;
             load8(r, x + row * P.ldx + cc, P.N - cc, P.x_vec != 0);
-            float d[8];
-#pragma unroll
-            for(int i = 0; i < 8; ++i)
-                d[i] = c + i < P.N ? (to_f32(r.v[i]) - mean) - shift : 0.f;
+            uint64_t d[4];
+            to_pairs(r, d);
+            distances(d, mean, P.N - cc);
+            distances(d, shift, P.N - cc);
             layernorm_out8<T, E5M2>(P, row, cc, d, rstd);
         }
         __syncthreads(); // buf is used again
@@ -601,101 +750,154 @@ __device__ __forceinline__ int column_of(int v, int i, int t, int tpr)
 {
     return STRIDED ? (v * 8 + i) * tpr + t : (v * tpr + t) * 8 + i;
 }
-template <typename T, bool STRIDED>
+template <typename T>
 __device__ __forceinline__ void load_columns(Vec8<T>& r, const T* row, int v, int t, int tpr, int N, bool on)
 {
-    if constexpr(STRIDED)
-    {
 #pragma unroll
-        for(int i = 0; i < 8; ++i)
-        {
-            const int c = column_of<true>(v, i, t, tpr);
-            r.v[i]      = on && c < N ? row[c] : from_f32<T>(0.f);
-        }
-    }
-    else
+    for(int i = 0; i < 8; ++i)
     {
-        const int c = column_of<false>(v, 0, t, tpr);
-        load8(r, row + c, on ? N - c : 0, true);
+        const int c = column_of<true>(v, i, t, tpr);
+        r.v[i]      = on && c < N ? row[c] : from_f32<T>(0.f);
     }
 }
 
 // dx and the partial sums of dgamma and dbeta in one pass.  A CTA walks rows blockIdx.x, + gridDim.x, ...; a thread keeps
-// the same V x 8 columns throughout, so the column sums stay in its registers until the CTA writes them once.
+// the same V x 8 columns throughout, so the column sums stay in its registers until the CTA writes them once.  Rows that
+// start on 16-byte boundaries come through shared memory (RowRing) and are read from there a second time for dx, which
+// keeps xhat and w out of the registers while the row's sums are formed; STRIDED rows one ahead in registers.
 template <typename T, int V, bool STRIDED>
-__global__ void __launch_bounds__(V == 1 ? 128 : 512) layernorm_bwd_kernel(const __grid_constant__ LayernormBwdParams P)
+__global__ void __launch_bounds__(V == 1 ? 128 : 512, V == 1 ? 4 : 1) layernorm_bwd_kernel(const __grid_constant__ LayernormBwdParams P)
 {
     grid_dependency_wait();
     grid_launch_dependents();
+    extern __shared__ __align__(16) uint8_t ring_smem[];
     __shared__ float buf[2 * 64];
     const int tpr = blockDim.x, t = threadIdx.x;
     const T* x  = static_cast<const T*>(P.x);
     const T* dy = static_cast<const T*>(P.dy);
     const float inv_n = 1.f / static_cast<float>(P.N);
-    float g[V][8], dg[V][8], db[V][8];
+    uint64_t g[V][4], dg[V][4], db[V][4];
 #pragma unroll
     for(int v = 0; v < V; ++v)
     {
+        float f[8];
 #pragma unroll
         for(int i = 0; i < 8; ++i)
         {
             const int c = column_of<STRIDED>(v, i, t, tpr);
-            g[v][i]     = 0.f;
+            f[i]        = 0.f;
             if(c < P.N)
-                g[v][i] = !P.gamma ? 1.f : P.w_f32 ? static_cast<const float*>(P.gamma)[c] : to_f32(static_cast<const T*>(P.gamma)[c]);
-            dg[v][i] = db[v][i] = 0.f;
+                f[i] = !P.gamma ? 1.f : P.w_f32 ? static_cast<const float*>(P.gamma)[c] : to_f32(static_cast<const T*>(P.gamma)[c]);
+        }
+#pragma unroll
+        for(int i = 0; i < 4; ++i)
+        {
+            g[v][i]  = pack_f32x2(f[2 * i], f[2 * i + 1]);
+            dg[v][i] = db[v][i] = 0;
         }
     }
     Vec8<T> rx[V], ry[V];
+    RowRing<T, 2 * V> ring{smem_u32(ring_smem) + t * 16, tpr}; // vectors of x, then of dy
     float mean = 0.f, rstd = 0.f;
-    auto fetch = [&](int64_t r) {
+    auto fetch = [&](int64_t r, int slot) {
         const bool on = r < P.M;
 #pragma unroll
         for(int v = 0; v < V; ++v)
         {
-            load_columns<T, STRIDED>(rx[v], x + r * P.ldx, v, t, tpr, P.N, on);
-            load_columns<T, STRIDED>(ry[v], dy + r * P.lddy, v, t, tpr, P.N, on);
+            if constexpr(STRIDED)
+            {
+                load_columns<T>(rx[v], x + (on ? r * P.ldx : 0), v, t, tpr, P.N, on);
+                load_columns<T>(ry[v], dy + (on ? r * P.lddy : 0), v, t, tpr, P.N, on);
+            }
+            else
+            {
+                const int c = (v * tpr + t) * 8, n = on ? P.N - c : 0;
+                ring.copy(slot, v, x + (n > 0 ? r * P.ldx + c : 0), n);
+                ring.copy(slot, V + v, dy + (n > 0 ? r * P.lddy + c : 0), n);
+            }
         }
-        mean = on ? __ldg(P.mean + r) : 0.f;
-        rstd = on ? __ldg(P.rstd + r) : 0.f;
+        if constexpr(!STRIDED)
+            copy_async_commit();
+    };
+    auto statistics = [&](int64_t r) {
+        mean = r < P.M ? __ldg(P.mean + r) : 0.f;
+        rstd = r < P.M ? __ldg(P.rstd + r) : 0.f;
     };
     int64_t row = blockIdx.x;
-    fetch(row);
+    int slot    = 0;
+    fetch(row, 0);
+    if constexpr(!STRIDED)
+#pragma unroll
+        for(int i = 1; i < STAGE_DEPTH - 1; ++i)
+            fetch(row + i * static_cast<int64_t>(gridDim.x), i);
+    statistics(row);
     int flip = 0;
     for(; row < P.M; row += gridDim.x)
     {
-        float h[V][8], w[V][8];
-        float s1 = 0.f, s2 = 0.f;
+        if constexpr(!STRIDED)
+        {
+            fetch(row + (STAGE_DEPTH - 1) * static_cast<int64_t>(gridDim.x), slot == 0 ? STAGE_DEPTH - 1 : slot - 1);
+            copy_async_wait<STAGE_DEPTH - 1>();
+        }
+        const uint64_t m2 = pack_f32x2(-mean, -mean), r2 = pack_f32x2(rstd, rstd);
         const float rs = rstd;
+        uint64_t h[V][4], w[V][4];
+        // xhat and w of vector v
+        auto values = [&](int v, uint64_t (&hv)[4], uint64_t (&gy)[4], uint64_t (&wv)[4]) {
+            if constexpr(!STRIDED)
+            {
+                ring.read(rx[v], slot, v);
+                ring.read(ry[v], slot, V + v);
+            }
+            to_pairs(rx[v], hv);
+            to_pairs(ry[v], gy);
+#pragma unroll
+            for(int i = 0; i < 4; ++i)
+            {
+                hv[i] = mul_f32x2(add_f32x2(hv[i], m2), r2);
+                wv[i] = mul_f32x2(gy[i], g[v][i]);
+            }
+        };
+        uint64_t s1v = 0, s2v = 0;
 #pragma unroll
         for(int v = 0; v < V; ++v)
+        {
+            uint64_t gy[4];
+            values(v, h[v], gy, w[v]);
+            // (behind the row's end dy and gamma are zero, and so is all that xhat is multiplied with)
 #pragma unroll
-            for(int i = 0; i < 8; ++i)
+            for(int i = 0; i < 4; ++i)
             {
-                const bool in   = STRIDED ? column_of<true>(v, i, t, tpr) < P.N : true; // (elsewhere dy and gamma are zero)
-                const float gy  = to_f32(ry[v].v[i]);
-                h[v][i]         = in ? (to_f32(rx[v].v[i]) - mean) * rs : 0.f;
-                dg[v][i]        = __fmaf_rn(gy, h[v][i], dg[v][i]);
-                db[v][i] += gy;
-                w[v][i] = gy * g[v][i];
-                s1 += w[v][i];
-                s2 = __fmaf_rn(w[v][i], h[v][i], s2);
+                dg[v][i] = fma_f32x2(gy[i], h[v][i], dg[v][i]);
+                db[v][i] = add_f32x2(db[v][i], gy[i]);
+                s1v      = add_f32x2(s1v, w[v][i]);
+                s2v      = fma_f32x2(w[v][i], h[v][i], s2v);
             }
+        }
+        float s1 = sum_f32x2(s1v), s2 = sum_f32x2(s2v);
         const int64_t next = row + gridDim.x;
-        fetch(next);
+        if constexpr(STRIDED)
+            fetch(next, 0);
+        statistics(next);
         row_sum2<false>(s1, s2, buf + flip);
         flip ^= 64;
         if(P.dx)
         {
             const float c1 = s1 * inv_n, c2 = s2 * inv_n;
+            const uint64_t c1v = pack_f32x2(-c1, -c1), c2v = pack_f32x2(-c2, -c2), rsv = pack_f32x2(rs, rs);
             T* out = static_cast<T*>(P.dx) + row * P.lddx;
 #pragma unroll
             for(int v = 0; v < V; ++v)
             {
+                if constexpr(!STRIDED)
+                {
+                    uint64_t gy[4];
+                    values(v, h[v], gy, w[v]);
+                }
                 float o[8];
 #pragma unroll
-                for(int i = 0; i < 8; ++i)
-                    o[i] = rs * (w[v][i] - c1 - h[v][i] * c2);
+                for(int i = 0; i < 4; ++i)
+                    unpack_f32x2(mul_f32x2(rsv, fma_f32x2(h[v][i], c2v, add_f32x2(w[v][i], c1v))), o[2 * i], o[2 * i + 1]);
                 if constexpr(STRIDED)
                 {
 #pragma unroll
@@ -713,7 +915,11 @@ __global__ void __launch_bounds__(V == 1 ? 128 : 512) layernorm_bwd_kernel(const
                 }
             }
         }
+        if(++slot == STAGE_DEPTH)
+            slot = 0;
     }
+    if constexpr(!STRIDED)
+        copy_async_wait_all();
     if(P.partial)
     {
         float* pg = P.partial + static_cast<int64_t>(blockIdx.x) * P.N;
@@ -724,10 +930,13 @@ __global__ void __launch_bounds__(V == 1 ? 128 : 512) layernorm_bwd_kernel(const
             for(int i = 0; i < 8; ++i)
             {
                 const int c = column_of<STRIDED>(v, i, t, tpr);
+                float a[2], b[2];
+                unpack_f32x2(dg[v][i / 2], a[0], a[1]);
+                unpack_f32x2(db[v][i / 2], b[0], b[1]);
                 if(c < P.N)
                 {
-                    pg[c] = dg[v][i];
-                    pb[c] = db[v][i];
+                    pg[c] = a[i & 1];
+                    pb[c] = b[i & 1];
                 }
             }
     }

@@ -18,11 +18,12 @@ float qmax_of(int dtype) { return dtype == CKB_F8_E5M2 ? 57344.f : 448.f; }
 int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 template <typename P>
-cudaError_t launch(void (*kern)(P), int64_t grid_x, int grid_y, int threads, cudaStream_t stream, const P& p)
+cudaError_t launch(void (*kern)(P), int64_t grid_x, int grid_y, int threads, cudaStream_t stream, const P& p, int smem = 0)
 {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim            = dim3(static_cast<unsigned>(grid_x), grid_y, 1);
     cfg.blockDim           = dim3(threads, 1, 1);
+    cfg.dynamicSmemBytes   = smem;
     cfg.stream             = stream;
     cudaLaunchAttribute attr[1];
     int n = 0;
@@ -30,6 +31,27 @@ cudaError_t launch(void (*kern)(P), int64_t grid_x, int grid_y, int threads, cud
     cfg.attrs    = attr;
     cfg.numAttrs = n;
     return cudaLaunchKernelEx(&cfg, kern, p);
+}
+
+// The same for a kernel that takes more than 48 KB of shared memory at times: allowed once per device.
+constexpr int kMaxSmem = 226 * 1024;
+template <auto KERN, typename P>
+cudaError_t launch_big(int64_t grid_x, int threads, cudaStream_t stream, const P& p, int smem)
+{
+    static bool done[64] = {};
+    int dev         = 0;
+    cudaError_t err = cudaGetDevice(&dev);
+    if(err != cudaSuccess)
+        return err;
+    if(dev < 0 || dev >= 64 || !done[dev])
+    {
+        err = cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+        if(err != cudaSuccess)
+            return err;
+        if(dev >= 0 && dev < 64)
+            done[dev] = true;
+    }
+    return launch(KERN, grid_x, 1, threads, stream, p, smem);
 }
 
 // fn(T{}) with T = the type of a CKB_BF16 / CKB_F16 / CKB_F32 tensor
@@ -192,10 +214,10 @@ cudaError_t launch_bwd(LayernormBwdParams p, cudaStream_t stream)
         if(!sums)
             p.partial = nullptr;
         if(V == 1)
-            e = p.vec ? launch(layernorm_bwd_kernel<T, 1, false>, p.parts, 1, threads, stream, p)
+            e = p.vec ? launch_big<&layernorm_bwd_kernel<T, 1, false>>(p.parts, threads, stream, p, RowRing<T, 2>::bytes(threads))
                       : launch(layernorm_bwd_kernel<T, 1, true>, p.parts, 1, threads, stream, p);
         else
-            e = p.vec ? launch(layernorm_bwd_kernel<T, 2, false>, p.parts, 1, threads, stream, p)
+            e = p.vec ? launch_big<&layernorm_bwd_kernel<T, 2, false>>(p.parts, threads, stream, p, RowRing<T, 4>::bytes(threads))
                       : launch(layernorm_bwd_kernel<T, 2, true>, p.parts, 1, threads, stream, p);
     }
     if(e != cudaSuccess || !sums)
@@ -239,6 +261,7 @@ int ckb_block_quantize_run(const ckb_block_quantize_desc* d, void* stream_, int 
     p.x_vec = starts_on(d->p_x, 16) && d->ldx * xb % 16 == 0;
     p.q_vec = starts_on(d->p_q, 8) && d->ldq % 8 == 0;
     p.qmax  = qmax_of(d->q_dtype);
+    p.qmax_recip = 1.f / p.qmax;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     const bool rows = d->block_m == 1, square = d->block_n == 128;
     const int64_t want = rows ? div_up(p.total, 16 * QB) : p.total;
@@ -287,13 +310,14 @@ int ckb_layernorm_fwd_run(const ckb_layernorm_fwd_desc* d, void* stream_, int n_
     p.w_vec = starts_on(d->p_gamma, 16) && starts_on(d->p_beta, 16);
     p.eps   = d->eps;
     p.qmax  = qmax_of(d->q_dtype);
+    p.qmax_recip = 1.f / p.qmax;
     // A row of up to 1024 values per warp, of up to 16384 per CTA in registers, longer ones read again from L2.
     const int64_t vecs = div_up(d->N, 8);
     const bool warp    = d->N <= 1024, lng = d->N > 16384;
-    const int V        = warp ? (vecs <= 32 ? 1 : vecs <= 64 ? 2 : 4) : d->N <= 4096 ? 2 : 4;
+    const int V        = warp ? (vecs <= 32 ? 1 : vecs <= 64 ? 2 : 4) : d->N <= 8192 ? 2 : 4;
     const int threads  = warp ? 256 : lng ? 1024 : static_cast<int>(div_up(div_up(vecs, V), 32) * 32);
     const int64_t want = warp ? div_up(d->M, 8) : d->M;
-    const int64_t most = static_cast<int64_t>(dev.sm_count) * (lng ? 2 : warp ? 8 : 1536 / threads < 1 ? 1 : 1536 / threads);
+    const int64_t most = static_cast<int64_t>(dev.sm_count) * (lng ? 2 : warp ? 8 : V == 4 ? 1 : 1024 / threads);
     const int64_t grid = want < most ? want : most;
     host_note_plan("layernorm_fwd %s threads=%d vectors=%d grid=%lld vec=%d", warp ? "warp" : lng ? "long" : "cta", threads, V,
                    static_cast<long long>(grid), p.x_vec);
@@ -306,11 +330,14 @@ int ckb_layernorm_fwd_run(const ckb_layernorm_fwd_desc* d, void* stream_, int n_
                 if(lng)
                     return launch(layernorm_fwd_long_kernel<T, E5>, grid, 1, threads, stream, p);
                 if(warp)
-                    return V == 1   ? launch(layernorm_fwd_kernel<T, E5, 1, true>, grid, 1, threads, stream, p)
-                           : V == 2 ? launch(layernorm_fwd_kernel<T, E5, 2, true>, grid, 1, threads, stream, p)
-                                    : launch(layernorm_fwd_kernel<T, E5, 4, true>, grid, 1, threads, stream, p);
-                return V == 2 ? launch(layernorm_fwd_kernel<T, E5, 2, false>, grid, 1, threads, stream, p)
-                              : launch(layernorm_fwd_kernel<T, E5, 4, false>, grid, 1, threads, stream, p);
+                    return V == 1   ? launch(layernorm_fwd_kernel<T, E5, 1, true, false>, grid, 1, threads, stream, p)
+                           : V == 2 ? launch(layernorm_fwd_kernel<T, E5, 2, true, false>, grid, 1, threads, stream, p)
+                                    : launch(layernorm_fwd_kernel<T, E5, 4, true, false>, grid, 1, threads, stream, p);
+                if(!p.x_vec)
+                    return V == 2 ? launch(layernorm_fwd_kernel<T, E5, 2, false, false>, grid, 1, threads, stream, p)
+                                  : launch(layernorm_fwd_kernel<T, E5, 4, false, false>, grid, 1, threads, stream, p);
+                return V == 2 ? launch_big<&layernorm_fwd_kernel<T, E5, 2, false, true>>(grid, threads, stream, p, RowRing<T, 2>::bytes(threads))
+                              : launch_big<&layernorm_fwd_kernel<T, E5, 4, false, true>>(grid, threads, stream, p, RowRing<T, 4>::bytes(threads));
             };
             return d->p_q && d->q_dtype == CKB_F8_E5M2 ? both(Flag<true>{}) : both(Flag<false>{});
         });
