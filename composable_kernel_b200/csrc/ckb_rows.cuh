@@ -51,19 +51,30 @@ __device__ __forceinline__ void load8(Vec8<T>& r, const T* p, int n, bool vec)
             r.v[i] = i < n ? p[i] : from_f32<T>(0.f);
     }
 }
+// Two values, rounded, in one word (f32: as they are).
+__device__ __forceinline__ uint32_t round_pair(const __half*, float lo, float hi)
+{
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t round_pair(const __nv_bfloat16*, float lo, float hi)
+{
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
 template <typename T>
 __device__ __forceinline__ void store8(const float (&f)[8], T* p, int n, bool vec)
 {
     if(vec && n >= 8)
     {
-        Vec8<T> r;
-#pragma unroll
-        for(int i = 0; i < 8; ++i)
-            r.v[i] = from_f32<T>(f[i]);
-        const uint4* s = reinterpret_cast<const uint4*>(&r);
-#pragma unroll
-        for(int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
-            reinterpret_cast<uint4*>(p)[i] = s[i];
+        if constexpr(sizeof(T) == 4)
+        {
+            reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
+            reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+        }
+        else
+            *reinterpret_cast<uint4*>(p) = make_uint4(round_pair(p, f[0], f[1]), round_pair(p, f[2], f[3]), round_pair(p, f[4], f[5]),
+                                                      round_pair(p, f[6], f[7]));
     }
     else
     {
@@ -173,12 +184,28 @@ __device__ __forceinline__ uint2 quantize8(const uint64_t (&f)[4], const BlockDi
 }
 
 // The eight values of a vector as pairs, and their largest magnitude.
-template <typename T>
-__device__ __forceinline__ void to_pairs(const Vec8<T>& r, uint64_t (&f)[4])
+__device__ __forceinline__ void to_pairs(const Vec8<float>& r, uint64_t (&f)[4])
 {
 #pragma unroll
     for(int i = 0; i < 4; ++i)
-        f[i] = pack_f32x2(to_f32(r.v[2 * i]), to_f32(r.v[2 * i + 1]));
+        f[i] = pack_f32x2(r.v[2 * i], r.v[2 * i + 1]);
+}
+__device__ __forceinline__ void to_pairs(const Vec8<__half>& r, uint64_t (&f)[4])
+{
+    const __half2* h = reinterpret_cast<const __half2*>(&r);
+#pragma unroll
+    for(int i = 0; i < 4; ++i)
+    {
+        const float2 v = __half22float2(h[i]);
+        f[i]           = pack_f32x2(v.x, v.y);
+    }
+}
+__device__ __forceinline__ void to_pairs(const Vec8<__nv_bfloat16>& r, uint64_t (&f)[4])
+{
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&r);
+#pragma unroll
+    for(int i = 0; i < 4; ++i) // a bf16 is the upper half of the 32-bit number
+        f[i] = pack_f32x2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
 }
 __device__ __forceinline__ float max_abs8(const Vec8<float>& r)
 {
@@ -396,25 +423,65 @@ __device__ __forceinline__ float warp_sum(float v)
     return v;
 }
 
-// Sums of two values over the threads of a row; `buf` holds 2 x 32 words per use, a __syncthreads lies between two
-// uses of the same words.  WARP: the row belongs to one warp.
-template <bool WARP>
-__device__ __forceinline__ void row_sum2(float& a, float& b, float* buf)
+// Threads that share a row: a warp, a whole CTA or (GROUPS) one of several equal parts of a CTA.
+enum { ROW_WARP, ROW_CTA, ROW_GROUP };
+template <int KIND>
+__device__ __forceinline__ void row_barrier(int group, int threads)
+{
+    if constexpr(KIND == ROW_CTA)
+        __syncthreads();
+    else if constexpr(KIND == ROW_GROUP)
+        asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(threads) : "memory");
+}
+
+// Sum of one value over the threads of a row (up to 16 warps; LONG: up to 32); `buf` holds 32 words per use, a barrier
+// lies between two uses of the same words.
+template <int KIND, bool LONG = false>
+__device__ __forceinline__ float row_sum(float a, float* buf, int group, int threads)
 {
     a = warp_sum(a);
-    b = warp_sum(b);
-    if constexpr(!WARP)
+    if constexpr(KIND != ROW_WARP)
     {
-        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+        const int warp = (threadIdx.x - group * threads) >> 5, lane = threadIdx.x & 31, warps = threads >> 5;
         if(lane == 0)
-        {
-            buf[warp]      = a;
-            buf[32 + warp] = b;
-        }
-        __syncthreads();
-        a = warp_sum(lane < warps ? buf[lane] : 0.f);
-        b = warp_sum(lane < warps ? buf[32 + lane] : 0.f);
+            buf[warp] = a;
+        row_barrier<KIND>(group, threads);
+        constexpr int W = LONG ? 32 : 16;
+        const int i     = lane & (W - 1);
+        a               = i < warps ? buf[i] : 0.f;
+#pragma unroll
+        for(int d = W / 2; d >= 1; d >>= 1)
+            a += __shfl_xor_sync(0xffffffffu, a, d);
     }
+    return a;
+}
+// Of two values at once (64 words): the lower half of a warp sums the first, the upper half the second.
+template <int KIND, bool LONG = false>
+__device__ __forceinline__ void row_sum2(float& a, float& b, float* buf, int group, int threads)
+{
+    const int lane  = threadIdx.x & 31;
+    const bool high = lane >= 16;
+    float v         = (high ? b : a) + __shfl_xor_sync(0xffffffffu, high ? a : b, 16);
+#pragma unroll
+    for(int d = 8; d >= 1; d >>= 1)
+        v += __shfl_xor_sync(0xffffffffu, v, d);
+    if constexpr(KIND != ROW_WARP)
+    {
+        const int warp = (threadIdx.x - group * threads) >> 5, warps = threads >> 5, i = lane & 15;
+        if(i == 0)
+            buf[(high ? 32 : 0) + warp] = v;
+        row_barrier<KIND>(group, threads);
+        const float* mine = buf + (high ? 32 : 0);
+        v                 = i < warps ? mine[i] : 0.f;
+        if constexpr(LONG)
+            v += i + 16 < warps ? mine[i + 16] : 0.f;
+#pragma unroll
+        for(int d = 8; d >= 1; d >>= 1)
+            v += __shfl_xor_sync(0xffffffffu, v, d);
+    }
+    const float other = __shfl_xor_sync(0xffffffffu, v, 16);
+    a                 = high ? other : v;
+    b                 = high ? v : other;
 }
 
 // From the mean square and the mean of the distances to the first mean.
@@ -432,18 +499,19 @@ template <typename T, int V>
 struct RowRing
 {
     static constexpr int PIECES = sizeof(T) / 2; // 16-byte pieces of a vector
+    static constexpr int PER    = 16 / sizeof(T);
     uint32_t base;                               // this thread's first piece
     int threads;
     static __host__ __device__ int bytes(int threads) { return STAGE_DEPTH * V * PIECES * threads * 16; }
-    // `n` = values of the row from the vector's first one on
+    // `n` = values of the row from the vector's first one on (<= 0: none, p is not read)
     __device__ __forceinline__ void copy(int slot, int v, const T* p, int n) const
     {
+        const uint32_t dst = base + (((slot * V + v) * PIECES) * threads) * 16;
 #pragma unroll
         for(int i = 0; i < PIECES; ++i)
         {
-            constexpr int PER = 16 / static_cast<int>(sizeof(T));
-            const int have    = n - i * PER < 0 ? 0 : n - i * PER > PER ? PER : n - i * PER;
-            copy_async_16(base + (((slot * V + v) * PIECES + i) * threads) * 16, have > 0 ? p + i * PER : p, have * static_cast<int>(sizeof(T)));
+            const int have = (n - i * PER) * static_cast<int>(sizeof(T)); // bytes
+            copy_async_16(dst + i * threads * 16, p + i * PER, have < 0 ? 0 : have > 16 ? 16 : have);
         }
     }
     __device__ __forceinline__ void read(Vec8<T>& r, int slot, int v) const
@@ -468,6 +536,8 @@ struct LayernormFwdParams
     int64_t M;
     int32_t N;
     int32_t w_f32, x_vec, y_vec, q_vec, w_vec;
+    int32_t tpr;      // threads of a row (ROW_GROUP, ROW_CTA)
+    int32_t w_offset; // ROW_GROUP: where gamma and beta lie in shared memory
     float eps, qmax, qmax_recip;
 };
 
@@ -492,38 +562,6 @@ __device__ __forceinline__ void load_weights8(uint64_t (&f)[4], const void* w, b
         Vec8<T> r;
         load8(r, static_cast<const T*>(w) + c, N - c, vec);
         to_pairs(r, f);
-    }
-}
-
-// y (and q) of 8 columns from their distances to the mean.
-template <typename T, bool E5M2>
-__device__ __forceinline__ void layernorm_out8(const LayernormFwdParams& P, int64_t row, int c, uint64_t (&d)[4], float rstd)
-{
-    const int n = P.N - c;
-    uint64_t g[4], b[4];
-    load_weights8<T>(g, P.gamma, P.w_f32 != 0, c, P.N, P.w_vec != 0, 1.f);
-    load_weights8<T>(b, P.beta, P.w_f32 != 0, c, P.N, P.w_vec != 0, 0.f);
-    const uint64_t r2 = pack_f32x2(rstd, rstd);
-    float y[8];
-#pragma unroll
-    for(int i = 0; i < 4; ++i)
-    {
-        d[i] = fma_f32x2(mul_f32x2(d[i], r2), g[i], b[i]);
-        unpack_f32x2(d[i], y[2 * i], y[2 * i + 1]);
-    }
-    if(P.y)
-        store8(y, static_cast<T*>(P.y) + row * P.ldy + c, n, P.y_vec != 0);
-    if(P.q)
-    {
-        float m = 0.f;
-#pragma unroll
-        for(int i = 0; i < 8; ++i)
-            m = max_abs(m, n >= 8 || i < n ? y[i] : 0.f);
-        const float s = block_scale(max16(m), P.qmax, P.qmax_recip, false);
-        const uint2 w = quantize8<E5M2>(d, BlockDivisor(s));
-        store_q8(w, P.q + row * P.ldq + c, n, P.q_vec != 0);
-        if((threadIdx.x & 15) == 0 && n > 0)
-            P.q_scale[row * P.ss_m + (c >> 7) * P.ss_n] = s;
     }
 }
 
@@ -558,85 +596,201 @@ __device__ __forceinline__ void distances(uint64_t (&d)[4], float mean, int n)
     }
 }
 
-// A row per warp (WARP, eight rows a CTA) or per CTA, V vectors of 8 values a thread: vector v of thread t holds columns
-// 8 (v * threads + t) .. + 7.  RING: rows come through shared memory, STAGE_DEPTH - 1 rows ahead (with one row ahead in
-// registers three CTAs per SM have 30 KB on their way, half of what the memory needs: 8192 x 5120 took 90 us).
+// y (and q) of the 16 columns from c on: y = (d - shift) * rstd * gamma + beta, d = distances to the first mean.
+// Eight neighbouring lanes hold a block of 128.  weights(u, g, b): gamma and beta of columns c + 8 u .. + 7.
+template <typename T, bool E5M2, typename Weights>
+__device__ __forceinline__ void layernorm_out16(const LayernormFwdParams& P, int64_t row, int c, uint64_t (&d)[2][4], float shift, float rstd,
+                                                Weights weights)
+{
+    const uint64_t r2 = pack_f32x2(rstd, rstd), s2 = pack_f32x2(-shift, -shift);
+    float m = 0.f;
+#pragma unroll
+    for(int u = 0; u < 2; ++u)
+    {
+        const int cu = c + u * 8, n = P.N - cu;
+        uint64_t g[4], b[4];
+        weights(u, g, b);
+        float y[8];
+#pragma unroll
+        for(int i = 0; i < 4; ++i)
+        {
+            d[u][i] = fma_f32x2(mul_f32x2(add_f32x2(d[u][i], s2), r2), g[i], b[i]);
+            unpack_f32x2(d[u][i], y[2 * i], y[2 * i + 1]);
+        }
+        if(P.y)
+            store8(y, static_cast<T*>(P.y) + row * P.ldy + cu, n, P.y_vec != 0);
+        if(P.q)
+        {
+            if(n >= 8)
+            {
+#pragma unroll
+                for(int i = 0; i < 8; ++i)
+                    m = max_abs(m, y[i]);
+            }
+            else
+            {
+#pragma unroll
+                for(int i = 0; i < 8; ++i)
+                    m = max_abs(m, i < n ? y[i] : 0.f);
+            }
+        }
+    }
+    if(P.q)
+    {
+#pragma unroll
+        for(int k = 4; k >= 1; k >>= 1)
+            m = max_abs(m, __shfl_xor_sync(0xffffffffu, m, k));
+        const float s = block_scale(m, P.qmax, P.qmax_recip, false);
+        const BlockDivisor div(s);
+        const uint2 w0 = quantize8<E5M2>(d[0], div), w1 = quantize8<E5M2>(d[1], div);
+        const int n = P.N - c;
+        uint8_t* q  = P.q + row * P.ldq + c;
+        if(P.q_vec && n >= 16)
+            *reinterpret_cast<uint4*>(q) = make_uint4(w0.x, w0.y, w1.x, w1.y);
+        else
+        {
+            store_q8(w0, q, n, false);
+            store_q8(w1, q + 8, n - 8, false);
+        }
+        if((threadIdx.x & 7) == 0 && n > 0)
+            P.q_scale[row * P.ss_m + (c >> 7) * P.ss_n] = s;
+    }
+}
+
+// U units of 16 values a thread: unit u of thread t holds columns 16 (u * threads + t) .. + 15, so a scale block belongs to
+// eight lanes.
+//   ROW_WARP   a row per warp, eight rows a CTA
+//   ROW_GROUP  one CTA per SM works on as many rows side by side as fit; gamma and beta wait in shared memory in 32 bits
+//              (read for every row from L2 they were 2.6 times the bytes of the rows, and their latency most of the time)
+//   ROW_CTA    longer rows: the weights from L2
+// RING: rows come through shared memory, STAGE_DEPTH - 1 rows ahead.  What bounds it is instructions (about 25 per value
+// with 8-bit output): units of 16 values instead of 8 halve those for the scale of a block.
 // Mean and variance in two passes over the registers; the second pass also sums the distances themselves, which takes
 // the rounding of the first mean out of both.
-template <typename T, bool E5M2, int V, bool WARP, bool RING>
-__global__ void __launch_bounds__(WARP ? 256 : 512, WARP || V == 4 ? 1 : 2) layernorm_fwd_kernel(const __grid_constant__ LayernormFwdParams P)
+template <typename T, bool E5M2, int U, int KIND, bool RING>
+__global__ void __launch_bounds__(KIND == ROW_WARP ? 256 : KIND == ROW_GROUP ? 768 : 512, KIND == ROW_WARP ? 2 : 1)
+    layernorm_fwd_kernel(const __grid_constant__ LayernormFwdParams P)
 {
     grid_dependency_wait();
     grid_launch_dependents();
     extern __shared__ __align__(16) uint8_t ring_smem[];
-    __shared__ float buf[4 * 64];
-    const int tpr      = WARP ? 32 : static_cast<int>(blockDim.x);
-    const int t        = WARP ? static_cast<int>(threadIdx.x) & 31 : static_cast<int>(threadIdx.x);
-    const int64_t step = WARP ? static_cast<int64_t>(gridDim.x) * 8 : gridDim.x;
-    int64_t row        = WARP ? static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5) : blockIdx.x;
-    const T* x         = static_cast<const T*>(P.x);
-    const float inv_n  = 1.f / static_cast<float>(P.N);
-    Vec8<T> raw[V];
-    RowRing<T, V> ring{smem_u32(ring_smem) + t * 16, tpr};
-    auto fetch = [&](int64_t r, int slot) {
+    __shared__ float sums[KIND == ROW_WARP ? 1 : KIND == ROW_GROUP ? 8 * 192 : 192];
+    const int tpr       = KIND == ROW_WARP ? 32 : P.tpr;
+    const int groups    = KIND == ROW_WARP ? 8 : static_cast<int>(blockDim.x) / tpr;
+    const int group     = static_cast<int>(threadIdx.x) / tpr;
+    const int t         = static_cast<int>(threadIdx.x) - group * tpr;
+    const int64_t step  = static_cast<int64_t>(gridDim.x) * groups;
+    int64_t row         = static_cast<int64_t>(blockIdx.x) * groups + group;
+    const T* x          = static_cast<const T*>(P.x);
+    const float inv_n   = 1.f / static_cast<float>(P.N);
+    float* buf          = sums + (KIND == ROW_GROUP ? group * 192 : 0); // two rows in turn, 96 words each
+    Vec8<T> raw[U][2];
+    RowRing<T, 2 * U> ring{smem_u32(ring_smem) + group * RowRing<T, 2 * U>::bytes(tpr) + t * 16, tpr};
+    auto column = [&](int u, int h) { return (u * tpr + t) * 16 + h * 8; };
+    int have[U][2]; // values of the row in each vector (and, first of all, where it starts: the row's start if it has none)
+    const T* ahead[U][2]; // of the row that is fetched next
 #pragma unroll
-        for(int v = 0; v < V; ++v)
+    for(int u = 0; u < U; ++u)
+#pragma unroll
+        for(int h = 0; h < 2; ++h)
         {
-            const int c = (v * tpr + t) * 8, n = r < P.M ? P.N - c : 0;
-            const T* p  = x + (n > 0 ? r * P.ldx + c : 0);
-            if constexpr(RING)
-                ring.copy(slot, v, p, n);
-            else
-                load8(raw[v], p, n, P.x_vec != 0);
+            have[u][h]  = P.N - column(u, h);
+            ahead[u][h] = x + row * P.ldx + (have[u][h] > 0 ? column(u, h) : 0);
         }
+    const int64_t row_step = step * P.ldx;
+    int64_t ahead_row      = row;
+    auto fetch = [&](int slot) {
+        const bool on = ahead_row < P.M;
+#pragma unroll
+        for(int u = 0; u < U; ++u)
+#pragma unroll
+            for(int h = 0; h < 2; ++h)
+            {
+                if constexpr(RING)
+                {
+                    if(on)
+                        ring.copy(slot, 2 * u + h, ahead[u][h], have[u][h]);
+                }
+                else
+                    load8(raw[u][h], ahead[u][h], on ? have[u][h] : 0, P.x_vec != 0);
+                ahead[u][h] += row_step;
+            }
         if constexpr(RING)
             copy_async_commit();
+        ahead_row += step;
     };
     int slot = 0;
-    fetch(row, 0);
+    fetch(0);
     if constexpr(RING)
 #pragma unroll
         for(int i = 1; i < STAGE_DEPTH - 1; ++i)
-            fetch(row + i * step, i);
+            fetch(i);
+    // ROW_GROUP: [gamma, beta][unit][four values][thread]
+    float4* w_smem = reinterpret_cast<float4*>(ring_smem + (KIND == ROW_GROUP ? P.w_offset : 0));
+    if constexpr(KIND == ROW_GROUP)
+    {
+        for(int i = threadIdx.x; i < 2 * U * 2 * tpr; i += blockDim.x)
+        {
+            // vector i of 8 weights: [which][unit][half][thread]
+            const int which = i / (U * 2 * tpr), rest = i - which * (U * 2 * tpr), uh = rest / tpr, th = rest - uh * tpr;
+            const int c = ((uh >> 1) * tpr + th) * 16 + (uh & 1) * 8;
+            uint64_t f[4];
+            load_weights8<T>(f, which ? P.beta : P.gamma, P.w_f32 != 0, c < P.N ? c : 0, c < P.N ? P.N : 0, P.w_vec != 0, which ? 0.f : 1.f);
+#pragma unroll
+            for(int k = 0; k < 2; ++k)
+            {
+                float4 v;
+                unpack_f32x2(f[2 * k], v.x, v.y);
+                unpack_f32x2(f[2 * k + 1], v.z, v.w);
+                w_smem[((which * U * 2 + uh) * 2 + k) * tpr + th] = v;
+            }
+        }
+        __syncthreads();
+    }
     int flip = 0;
     for(; row < P.M; row += step)
     {
         if constexpr(RING)
         {
-            fetch(row + (STAGE_DEPTH - 1) * step, slot == 0 ? STAGE_DEPTH - 1 : slot - 1);
+            fetch(slot == 0 ? STAGE_DEPTH - 1 : slot - 1);
             copy_async_wait<STAGE_DEPTH - 1>();
 #pragma unroll
-            for(int v = 0; v < V; ++v)
-                ring.read(raw[v], slot, v);
+            for(int u = 0; u < U; ++u)
+#pragma unroll
+                for(int h = 0; h < 2; ++h)
+                    ring.read(raw[u][h], slot, 2 * u + h);
             if(++slot == STAGE_DEPTH)
                 slot = 0;
         }
-        uint64_t d[V][4];
-        float sum = 0.f, none = 0.f;
+        uint64_t d[U][2][4];
+        uint64_t sv = 0;
 #pragma unroll
-        for(int v = 0; v < V; ++v)
-        {
-            to_pairs(raw[v], d[v]);
-            sum += sum_f32x2(add_f32x2(add_f32x2(d[v][0], d[v][1]), add_f32x2(d[v][2], d[v][3])));
-        }
+        for(int u = 0; u < U; ++u)
+#pragma unroll
+            for(int h = 0; h < 2; ++h)
+            {
+                to_pairs(raw[u][h], d[u][h]);
+                sv = add_f32x2(sv, add_f32x2(add_f32x2(d[u][h][0], d[u][h][1]), add_f32x2(d[u][h][2], d[u][h][3])));
+            }
         if constexpr(!RING)
-            fetch(row + step, 0);
-        row_sum2<WARP>(sum, none, buf + flip);
-        float mean = sum * inv_n;
+            fetch(0);
+        float mean   = row_sum<KIND>(sum_f32x2(sv), buf + flip, group, tpr) * inv_n;
         uint64_t s1v = 0, s2v = 0;
 #pragma unroll
-        for(int v = 0; v < V; ++v)
-        {
-            distances(d[v], mean, P.N - (v * tpr + t) * 8);
+        for(int u = 0; u < U; ++u)
 #pragma unroll
-            for(int i = 0; i < 4; ++i)
+            for(int h = 0; h < 2; ++h)
             {
-                s1v = add_f32x2(s1v, d[v][i]);
-                s2v = fma_f32x2(d[v][i], d[v][i], s2v);
+                distances(d[u][h], mean, have[u][h]);
+#pragma unroll
+                for(int i = 0; i < 4; ++i)
+                {
+                    s1v = add_f32x2(s1v, d[u][h][i]);
+                    s2v = fma_f32x2(d[u][h][i], d[u][h][i], s2v);
+                }
             }
-        }
         float s1 = sum_f32x2(s1v), s2 = sum_f32x2(s2v);
-        row_sum2<WARP>(s1, s2, buf + 64 + flip);
+        row_sum2<KIND>(s1, s2, buf + 32 + flip, group, tpr);
         const float shift = s1 * inv_n;
         const float rstd  = rstd_of(s2 * inv_n, shift, P.eps);
         mean += shift;
@@ -648,16 +802,27 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, WARP || V == 4 ? 1 : 2) laye
                 P.rstd[row] = rstd;
         }
 #pragma unroll
-        for(int v = 0; v < V; ++v)
-        {
-            if(__all_sync(0xffffffffu, P.N - (v * tpr + t) * 8 <= 0))
-                continue;
+        for(int u = 0; u < U; ++u)
+            if(!__all_sync(0xffffffffu, column(u, 0) >= P.N))
+                layernorm_out16<T, E5M2>(P, row, column(u, 0), d[u], shift, rstd, [&](int h, uint64_t (&g)[4], uint64_t (&b)[4]) {
+                    if constexpr(KIND == ROW_GROUP)
+                    {
 #pragma unroll
-            for(int i = 0; i < 4; ++i)
-                d[v][i] = add_f32x2(d[v][i], pack_f32x2(-shift, -shift));
-            layernorm_out8<T, E5M2>(P, row, (v * tpr + t) * 8, d[v], rstd);
-        }
-        flip ^= 128;
+                        for(int k = 0; k < 2; ++k)
+                        {
+                            const ulonglong2 gv = *reinterpret_cast<const ulonglong2*>(w_smem + ((u * 2 + h) * 2 + k) * tpr + t);
+                            const ulonglong2 bv = *reinterpret_cast<const ulonglong2*>(w_smem + ((U * 2 + u * 2 + h) * 2 + k) * tpr + t);
+                            g[2 * k] = gv.x, g[2 * k + 1] = gv.y, b[2 * k] = bv.x, b[2 * k + 1] = bv.y;
+                        }
+                    }
+                    else
+                    {
+                        const int c = column(u, h);
+                        load_weights8<T>(g, P.gamma, P.w_f32 != 0, c, P.N, P.w_vec != 0, 1.f);
+                        load_weights8<T>(b, P.beta, P.w_f32 != 0, c, P.N, P.w_vec != 0, 0.f);
+                    }
+                });
+        flip ^= 96;
     }
     if constexpr(RING)
         copy_async_wait_all();
@@ -675,34 +840,33 @@ __global__ void __launch_bounds__(1024) layernorm_fwd_long_kernel(const __grid_c
     const float n = static_cast<float>(P.N);
     for(int64_t row = blockIdx.x; row < P.M; row += gridDim.x)
     {
-        float sum = 0.f, none = 0.f;
+        float sum = 0.f;
         Vec8<T> r;
+        uint64_t d[2][4];
         for(int64_t c = t * 8; c < P.N; c += 8192)
         {
             load8(r, x + row * P.ldx + c, static_cast<int>(P.N - c), P.x_vec != 0);
-            float part = 0.f;
-#pragma unroll
-            for(int i = 0; i < 8; ++i)
-                part += to_f32(r.v[i]);
-            sum += part;
+            to_pairs(r, d[0]);
+            sum += sum_f32x2(add_f32x2(add_f32x2(d[0][0], d[0][1]), add_f32x2(d[0][2], d[0][3])));
         }
-        row_sum2<false>(sum, none, buf);
-        float mean = sum / n, s1 = 0.f, s2 = 0.f;
+        const float mean = row_sum<ROW_CTA, true>(sum, buf, 0, 1024) / n;
+        float s1 = 0.f, s2 = 0.f;
         for(int64_t c = t * 8; c < P.N; c += 8192)
         {
             load8(r, x + row * P.ldx + c, static_cast<int>(P.N - c), P.x_vec != 0);
-            float p1 = 0.f, p2 = 0.f;
+            to_pairs(r, d[0]);
+            distances(d[0], mean, static_cast<int>(P.N - c));
+            uint64_t p1 = 0, p2 = 0;
 #pragma unroll
-            for(int i = 0; i < 8; ++i)
+            for(int i = 0; i < 4; ++i)
             {
-                const float d = c + i < P.N ? to_f32(r.v[i]) - mean : 0.f;
-                p1 += d;
-                p2 = __fmaf_rn(d, d, p2);
+                p1 = add_f32x2(p1, d[0][i]);
+                p2 = fma_f32x2(d[0][i], d[0][i], p2);
             }
-            s1 += p1;
-            s2 += p2;
+            s1 += sum_f32x2(p1);
+            s2 += sum_f32x2(p2);
         }
-        row_sum2<false>(s1, s2, buf + 64);
+        row_sum2<ROW_CTA, true>(s1, s2, buf + 64, 0, 1024);
         const float shift = s1 / n;
         const float rstd  = rstd_of(s2 / n, shift, P.eps);
         if(t == 0)
@@ -712,19 +876,25 @@ __global__ void __launch_bounds__(1024) layernorm_fwd_long_kernel(const __grid_c
             if(P.rstd)
                 P.rstd[row] = rstd;
         }
-        for(int64_t c0 = 0; c0 < P.N; c0 += 8192)
+        for(int64_t c0 = 0; c0 < P.N; c0 += 16384)
         {
-            const int64_t c = c0 + t * 8;
+            const int64_t c = c0 + t * 16;
             if(__all_sync(0xffffffffu, c >= P.N))
                 continue;
             // (a lane behind the row's end takes part in the shuffles with zeros)
             const int cc = c < P.N ? static_cast<int>(c) : P.N;
-            load8(r, x + row * P.ldx + cc, P.N - cc, P.x_vec != 0);
-            uint64_t d[4];
-            to_pairs(r, d);
-            distances(d, mean, P.N - cc);
-            distances(d, shift, P.N - cc);
-            layernorm_out8<T, E5M2>(P, row, cc, d, rstd);
+#pragma unroll
+            for(int h = 0; h < 2; ++h)
+            {
+                const int m = P.N - cc - h * 8;
+                load8(r, x + row * P.ldx + (m > 0 ? cc + h * 8 : 0), m, P.x_vec != 0);
+                to_pairs(r, d[h]);
+                distances(d[h], mean, m);
+            }
+            layernorm_out16<T, E5M2>(P, row, cc, d, shift, rstd, [&](int h, uint64_t (&g)[4], uint64_t (&b)[4]) {
+                load_weights8<T>(g, P.gamma, P.w_f32 != 0, cc + h * 8, P.N, P.w_vec != 0, 1.f);
+                load_weights8<T>(b, P.beta, P.w_f32 != 0, cc + h * 8, P.N, P.w_vec != 0, 0.f);
+            });
         }
         __syncthreads(); // buf is used again
     }
@@ -763,8 +933,7 @@ __device__ __forceinline__ void load_columns(Vec8<T>& r, const T* row, int v, in
 
 // dx and the partial sums of dgamma and dbeta in one pass.  A CTA walks rows blockIdx.x, + gridDim.x, ...; a thread keeps
 // the same V x 8 columns throughout, so the column sums stay in its registers until the CTA writes them once.  Rows that
-// start on 16-byte boundaries come through shared memory (RowRing) and are read from there a second time for dx, which
-// keeps xhat and w out of the registers while the row's sums are formed; STRIDED rows one ahead in registers.
+// start on 16-byte boundaries come through shared memory (RowRing), STRIDED ones one ahead in registers.
 template <typename T, int V, bool STRIDED>
 __global__ void __launch_bounds__(V == 1 ? 128 : 512, V == 1 ? 4 : 1) layernorm_bwd_kernel(const __grid_constant__ LayernormBwdParams P)
 {
@@ -799,71 +968,98 @@ __global__ void __launch_bounds__(V == 1 ? 128 : 512, V == 1 ? 4 : 1) layernorm_
     Vec8<T> rx[V], ry[V];
     RowRing<T, 2 * V> ring{smem_u32(ring_smem) + t * 16, tpr}; // vectors of x, then of dy
     float mean = 0.f, rstd = 0.f;
-    auto fetch = [&](int64_t r, int slot) {
-        const bool on = r < P.M;
+    // of the row that is fetched next: its start, or the start of each vector of this thread
+    const T *x_ahead[STRIDED ? 1 : V], *dy_ahead[STRIDED ? 1 : V];
+    int have[V]; // values of the row in each vector
+#pragma unroll
+    for(int v = 0; v < V; ++v)
+    {
+        const int c = STRIDED ? 0 : column_of<false>(v, 0, t, tpr);
+        have[v]     = P.N - c;
+        if(!STRIDED || v == 0)
+        {
+            x_ahead[STRIDED ? 0 : v]  = x + blockIdx.x * P.ldx + (have[v] > 0 ? c : 0);
+            dy_ahead[STRIDED ? 0 : v] = dy + blockIdx.x * P.lddy + (have[v] > 0 ? c : 0);
+        }
+    }
+    const int64_t x_step = gridDim.x * P.ldx, dy_step = gridDim.x * P.lddy;
+    int64_t ahead_row = blockIdx.x;
+    auto fetch = [&](int slot) {
+        const bool on = ahead_row < P.M;
 #pragma unroll
         for(int v = 0; v < V; ++v)
         {
             if constexpr(STRIDED)
             {
-                load_columns<T>(rx[v], x + (on ? r * P.ldx : 0), v, t, tpr, P.N, on);
-                load_columns<T>(ry[v], dy + (on ? r * P.lddy : 0), v, t, tpr, P.N, on);
+                load_columns<T>(rx[v], x_ahead[0], v, t, tpr, P.N, on);
+                load_columns<T>(ry[v], dy_ahead[0], v, t, tpr, P.N, on);
             }
             else
             {
-                const int c = (v * tpr + t) * 8, n = on ? P.N - c : 0;
-                ring.copy(slot, v, x + (n > 0 ? r * P.ldx + c : 0), n);
-                ring.copy(slot, V + v, dy + (n > 0 ? r * P.lddy + c : 0), n);
+                if(on)
+                {
+                    ring.copy(slot, v, x_ahead[v], have[v]);
+                    ring.copy(slot, V + v, dy_ahead[v], have[v]);
+                }
+                x_ahead[v] += x_step;
+                dy_ahead[v] += dy_step;
             }
         }
-        if constexpr(!STRIDED)
+        if constexpr(STRIDED)
+        {
+            x_ahead[0] += x_step;
+            dy_ahead[0] += dy_step;
+        }
+        else
             copy_async_commit();
+        ahead_row += gridDim.x;
     };
-    auto statistics = [&](int64_t r) {
-        mean = r < P.M ? __ldg(P.mean + r) : 0.f;
-        rstd = r < P.M ? __ldg(P.rstd + r) : 0.f;
+    const float *mean_at = P.mean + blockIdx.x, *rstd_at = P.rstd + blockIdx.x;
+    T* out               = static_cast<T*>(P.dx) + (P.dx ? blockIdx.x * P.lddx : 0);
+    const int64_t dx_step = gridDim.x * P.lddx;
+    auto statistics = [&](bool on) {
+        mean = on ? __ldg(mean_at) : 0.f;
+        rstd = on ? __ldg(rstd_at) : 0.f;
+        mean_at += gridDim.x;
+        rstd_at += gridDim.x;
     };
     int64_t row = blockIdx.x;
     int slot    = 0;
-    fetch(row, 0);
+    fetch(0);
     if constexpr(!STRIDED)
 #pragma unroll
         for(int i = 1; i < STAGE_DEPTH - 1; ++i)
-            fetch(row + i * static_cast<int64_t>(gridDim.x), i);
-    statistics(row);
+            fetch(i);
+    statistics(row < P.M);
     int flip = 0;
     for(; row < P.M; row += gridDim.x)
     {
         if constexpr(!STRIDED)
         {
-            fetch(row + (STAGE_DEPTH - 1) * static_cast<int64_t>(gridDim.x), slot == 0 ? STAGE_DEPTH - 1 : slot - 1);
+            fetch(slot == 0 ? STAGE_DEPTH - 1 : slot - 1);
             copy_async_wait<STAGE_DEPTH - 1>();
         }
         const uint64_t m2 = pack_f32x2(-mean, -mean), r2 = pack_f32x2(rstd, rstd);
         const float rs = rstd;
         uint64_t h[V][4], w[V][4];
-        // xhat and w of vector v
-        auto values = [&](int v, uint64_t (&hv)[4], uint64_t (&gy)[4], uint64_t (&wv)[4]) {
+        uint64_t s1v = 0, s2v = 0;
+#pragma unroll
+        for(int v = 0; v < V; ++v)
+        {
             if constexpr(!STRIDED)
             {
                 ring.read(rx[v], slot, v);
                 ring.read(ry[v], slot, V + v);
             }
-            to_pairs(rx[v], hv);
+            uint64_t gy[4];
+            to_pairs(rx[v], h[v]);
             to_pairs(ry[v], gy);
 #pragma unroll
             for(int i = 0; i < 4; ++i)
             {
-                hv[i] = mul_f32x2(add_f32x2(hv[i], m2), r2);
-                wv[i] = mul_f32x2(gy[i], g[v][i]);
+                h[v][i] = mul_f32x2(add_f32x2(h[v][i], m2), r2);
+                w[v][i] = mul_f32x2(gy[i], g[v][i]);
             }
-        };
-        uint64_t s1v = 0, s2v = 0;
-#pragma unroll
-        for(int v = 0; v < V; ++v)
-        {
-            uint64_t gy[4];
-            values(v, h[v], gy, w[v]);
             // (behind the row's end dy and gamma are zero, and so is all that xhat is multiplied with)
 #pragma unroll
             for(int i = 0; i < 4; ++i)
@@ -875,25 +1071,18 @@ __global__ void __launch_bounds__(V == 1 ? 128 : 512, V == 1 ? 4 : 1) layernorm_
             }
         }
         float s1 = sum_f32x2(s1v), s2 = sum_f32x2(s2v);
-        const int64_t next = row + gridDim.x;
         if constexpr(STRIDED)
-            fetch(next, 0);
-        statistics(next);
-        row_sum2<false>(s1, s2, buf + flip);
+            fetch(0);
+        statistics(row + gridDim.x < P.M);
+        row_sum2<ROW_CTA>(s1, s2, buf + flip, 0, tpr);
         flip ^= 64;
         if(P.dx)
         {
             const float c1 = s1 * inv_n, c2 = s2 * inv_n;
             const uint64_t c1v = pack_f32x2(-c1, -c1), c2v = pack_f32x2(-c2, -c2), rsv = pack_f32x2(rs, rs);
-            T* out = static_cast<T*>(P.dx) + row * P.lddx;
 #pragma unroll
             for(int v = 0; v < V; ++v)
             {
-                if constexpr(!STRIDED)
-                {
-                    uint64_t gy[4];
-                    values(v, h[v], gy, w[v]);
-                }
                 float o[8];
 #pragma unroll
                 for(int i = 0; i < 4; ++i)
@@ -910,11 +1099,11 @@ __global__ void __launch_bounds__(V == 1 ? 128 : 512, V == 1 ? 4 : 1) layernorm_
                 }
                 else
                 {
-                    const int c = column_of<false>(v, 0, t, tpr);
-                    store8(o, out + c, P.N - c, true);
+                    store8(o, out + column_of<false>(v, 0, t, tpr), have[v], true);
                 }
             }
         }
+        out += dx_step;
         if(++slot == STAGE_DEPTH)
             slot = 0;
     }
@@ -965,7 +1154,7 @@ __global__ void __launch_bounds__(1024) layernorm_bwd_long_kernel(const __grid_c
             s1 += w;
             s2 = __fmaf_rn(w, (to_f32(x[c]) - mean) * rstd, s2);
         }
-        row_sum2<false>(s1, s2, buf);
+        row_sum2<ROW_CTA, true>(s1, s2, buf, 0, 1024);
         const float c1 = s1 / n, c2 = s2 / n;
         T* out = static_cast<T*>(P.dx) + row * P.lddx;
         for(int64_t c = threadIdx.x; c < P.N; c += 1024)

@@ -34,7 +34,7 @@ cudaError_t launch(void (*kern)(P), int64_t grid_x, int grid_y, int threads, cud
 }
 
 // The same for a kernel that takes more than 48 KB of shared memory at times: allowed once per device.
-constexpr int kMaxSmem = 226 * 1024;
+constexpr int kMaxSmem = 220 * 1024; // (the kernels have up to 6 KB besides)
 template <auto KERN, typename P>
 cudaError_t launch_big(int64_t grid_x, int threads, cudaStream_t stream, const P& p, int smem)
 {
@@ -306,20 +306,33 @@ int ckb_layernorm_fwd_run(const ckb_layernorm_fwd_desc* d, void* stream_, int n_
     p.w_f32 = d->w_dtype == CKB_F32;
     p.x_vec = starts_on(d->p_x, 16) && d->ldx * xb % 16 == 0;
     p.y_vec = starts_on(d->p_y, 16) && d->ldy * xb % 16 == 0;
-    p.q_vec = starts_on(d->p_q, 8) && d->ldq % 8 == 0;
+    p.q_vec = starts_on(d->p_q, 16) && d->ldq % 16 == 0;
     p.w_vec = starts_on(d->p_gamma, 16) && starts_on(d->p_beta, 16);
     p.eps   = d->eps;
     p.qmax  = qmax_of(d->q_dtype);
     p.qmax_recip = 1.f / p.qmax;
-    // A row of up to 1024 values per warp, of up to 16384 per CTA in registers, longer ones read again from L2.
-    const int64_t vecs = div_up(d->N, 8);
-    const bool warp    = d->N <= 1024, lng = d->N > 16384;
-    const int V        = warp ? (vecs <= 32 ? 1 : vecs <= 64 ? 2 : 4) : d->N <= 8192 ? 2 : 4;
-    const int threads  = warp ? 256 : lng ? 1024 : static_cast<int>(div_up(div_up(vecs, V), 32) * 32);
-    const int64_t want = warp ? div_up(d->M, 8) : d->M;
-    const int64_t most = static_cast<int64_t>(dev.sm_count) * (lng ? 2 : warp ? 8 : V == 4 ? 1 : 1024 / threads);
+    // A row of up to 1024 values per warp, of up to 8192 per part of a CTA, of up to 16384 per CTA in registers, longer
+    // ones read again from L2.
+    const int64_t units = div_up(d->N, 16);
+    const bool warp = d->N <= 1024, lng = d->N > 16384, wide = d->N > 8192;
+    const int U     = warp && units <= 32 ? 1 : 2;
+    p.tpr           = warp ? 32 : lng ? 1024 : static_cast<int>(div_up(div_up(units, U), 32) * 32);
+    // parts of a CTA: 768 threads at most, rows and weights within shared memory, and no more than there are rows for
+    const int ring = p.x_vec ? STAGE_DEPTH * U * 2 * 8 * xb * p.tpr : 0, weights = 2 * U * 16 * 4 * p.tpr;
+    int parts      = warp ? 8 : 1;
+    if(!warp && !wide)
+    {
+        const int64_t rows = div_up(d->M, dev.sm_count);
+        while(parts < 8 && (parts + 1) * p.tpr <= 768 && (parts + 1) * ring + weights <= kMaxSmem && parts < rows)
+            ++parts;
+    }
+    const int threads  = parts * p.tpr;
+    const int smem     = warp || lng ? 0 : parts * ring + (wide ? 0 : weights);
+    p.w_offset         = parts * ring;
+    const int64_t want = div_up(d->M, parts);
+    const int64_t most = static_cast<int64_t>(dev.sm_count) * (lng ? 2 : warp ? 8 : 1);
     const int64_t grid = want < most ? want : most;
-    host_note_plan("layernorm_fwd %s threads=%d vectors=%d grid=%lld vec=%d", warp ? "warp" : lng ? "long" : "cta", threads, V,
+    host_note_plan("layernorm_fwd %s threads=%d vectors=%d grid=%lld vec=%d", warp ? "warp" : lng ? "long" : "cta", threads, 2 * U,
                    static_cast<long long>(grid), p.x_vec);
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     auto once = [&]() {
@@ -330,14 +343,13 @@ int ckb_layernorm_fwd_run(const ckb_layernorm_fwd_desc* d, void* stream_, int n_
                 if(lng)
                     return launch(layernorm_fwd_long_kernel<T, E5>, grid, 1, threads, stream, p);
                 if(warp)
-                    return V == 1   ? launch(layernorm_fwd_kernel<T, E5, 1, true, false>, grid, 1, threads, stream, p)
-                           : V == 2 ? launch(layernorm_fwd_kernel<T, E5, 2, true, false>, grid, 1, threads, stream, p)
-                                    : launch(layernorm_fwd_kernel<T, E5, 4, true, false>, grid, 1, threads, stream, p);
-                if(!p.x_vec)
-                    return V == 2 ? launch(layernorm_fwd_kernel<T, E5, 2, false, false>, grid, 1, threads, stream, p)
-                                  : launch(layernorm_fwd_kernel<T, E5, 4, false, false>, grid, 1, threads, stream, p);
-                return V == 2 ? launch_big<&layernorm_fwd_kernel<T, E5, 2, false, true>>(grid, threads, stream, p, RowRing<T, 2>::bytes(threads))
-                              : launch_big<&layernorm_fwd_kernel<T, E5, 4, false, true>>(grid, threads, stream, p, RowRing<T, 4>::bytes(threads));
+                    return U == 1 ? launch(layernorm_fwd_kernel<T, E5, 1, ROW_WARP, false>, grid, 1, threads, stream, p)
+                                  : launch(layernorm_fwd_kernel<T, E5, 2, ROW_WARP, false>, grid, 1, threads, stream, p);
+                if(wide)
+                    return p.x_vec ? launch_big<&layernorm_fwd_kernel<T, E5, 2, ROW_CTA, true>>(grid, threads, stream, p, smem)
+                                   : launch(layernorm_fwd_kernel<T, E5, 2, ROW_CTA, false>, grid, 1, threads, stream, p);
+                return p.x_vec ? launch_big<&layernorm_fwd_kernel<T, E5, 2, ROW_GROUP, true>>(grid, threads, stream, p, smem)
+                               : launch_big<&layernorm_fwd_kernel<T, E5, 2, ROW_GROUP, false>>(grid, threads, stream, p, smem);
             };
             return d->p_q && d->q_dtype == CKB_F8_E5M2 ? both(Flag<true>{}) : both(Flag<false>{});
         });
