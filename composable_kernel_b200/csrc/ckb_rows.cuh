@@ -25,12 +25,16 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// Eight consecutive values as they lie in memory.
+// Eight consecutive values as they lie in memory, in words.
 template <typename T>
-struct alignas(16) Vec8
+struct Vec8
 {
-    T v[8];
+    static constexpr int WORDS = 2 * sizeof(T);
+    uint32_t w[WORDS];
 };
+__device__ __forceinline__ uint32_t bits_of(float v) { return __float_as_uint(v); }
+__device__ __forceinline__ uint32_t bits_of(__half v) { return __half_as_ushort(v); }
+__device__ __forceinline__ uint32_t bits_of(__nv_bfloat16 v) { return __bfloat16_as_ushort(v); }
 
 // `n` = values that exist (<= 0: none, the vector is zero); `vec`: p is 16-byte aligned.
 template <typename T>
@@ -38,19 +42,26 @@ __device__ __forceinline__ void load8(Vec8<T>& r, const T* p, int n, bool vec)
 {
     if(vec && n >= 8)
     {
-        uint4* d       = reinterpret_cast<uint4*>(&r);
         const uint4* s = reinterpret_cast<const uint4*>(p);
 #pragma unroll
-        for(int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
-            d[i] = __ldg(s + i);
+        for(int i = 0; i < Vec8<T>::WORDS / 4; ++i)
+        {
+            const uint4 q = __ldg(s + i);
+            r.w[4 * i] = q.x, r.w[4 * i + 1] = q.y, r.w[4 * i + 2] = q.z, r.w[4 * i + 3] = q.w;
+        }
     }
     else
     {
+        uint32_t e[8];
 #pragma unroll
         for(int i = 0; i < 8; ++i)
-            r.v[i] = i < n ? p[i] : from_f32<T>(0.f);
+            e[i] = i < n ? bits_of(p[i]) : 0u;
+#pragma unroll
+        for(int i = 0; i < Vec8<T>::WORDS; ++i)
+            r.w[i] = sizeof(T) == 4 ? e[i & 7] : e[(2 * i) & 7] | e[(2 * i + 1) & 7] << 16;
     }
 }
+
 // Two values, rounded, in one word (f32: as they are).
 __device__ __forceinline__ uint32_t round_pair(const __half*, float lo, float hi)
 {
@@ -188,42 +199,49 @@ __device__ __forceinline__ void to_pairs(const Vec8<float>& r, uint64_t (&f)[4])
 {
 #pragma unroll
     for(int i = 0; i < 4; ++i)
-        f[i] = pack_f32x2(r.v[2 * i], r.v[2 * i + 1]);
+        f[i] = pack_f32x2(__uint_as_float(r.w[2 * i]), __uint_as_float(r.w[2 * i + 1]));
 }
 __device__ __forceinline__ void to_pairs(const Vec8<__half>& r, uint64_t (&f)[4])
 {
-    const __half2* h = reinterpret_cast<const __half2*>(&r);
 #pragma unroll
     for(int i = 0; i < 4; ++i)
     {
-        const float2 v = __half22float2(h[i]);
+        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&r.w[i]));
         f[i]           = pack_f32x2(v.x, v.y);
     }
 }
 __device__ __forceinline__ void to_pairs(const Vec8<__nv_bfloat16>& r, uint64_t (&f)[4])
 {
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(&r);
 #pragma unroll
     for(int i = 0; i < 4; ++i) // a bf16 is the upper half of the 32-bit number
-        f[i] = pack_f32x2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+        f[i] = pack_f32x2(__uint_as_float(r.w[i] << 16), __uint_as_float(r.w[i] & 0xffff0000u));
+}
+__device__ __forceinline__ float value_of(const Vec8<float>& r, int k) { return __uint_as_float(r.w[k]); }
+__device__ __forceinline__ float value_of(const Vec8<__half>& r, int k)
+{
+    return __half2float(__ushort_as_half(static_cast<unsigned short>(r.w[k / 2] >> (16 * (k & 1)))));
+}
+__device__ __forceinline__ float value_of(const Vec8<__nv_bfloat16>& r, int k)
+{
+    return __uint_as_float(k & 1 ? r.w[k / 2] & 0xffff0000u : r.w[k / 2] << 16);
 }
 __device__ __forceinline__ float max_abs8(const Vec8<float>& r)
 {
     float m = 0.f;
 #pragma unroll
     for(int i = 0; i < 8; ++i)
-        m = max_abs(m, r.v[i]);
+        m = max_abs(m, __uint_as_float(r.w[i]));
     return m;
 }
 __device__ __forceinline__ float max_abs8(const Vec8<__half>& r)
 {
-    const __half2* h = reinterpret_cast<const __half2*>(&r);
+    const __half2* h = reinterpret_cast<const __half2*>(r.w);
     const __half2 m  = __hmax2_nan(__hmax2_nan(__habs2(h[0]), __habs2(h[1])), __hmax2_nan(__habs2(h[2]), __habs2(h[3])));
     return max_abs(__low2float(m), __high2float(m));
 }
 __device__ __forceinline__ float max_abs8(const Vec8<__nv_bfloat16>& r)
 {
-    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&r);
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(r.w);
     const __nv_bfloat162 m  = __hmax2_nan(__hmax2_nan(__habs2(h[0]), __habs2(h[1])), __hmax2_nan(__habs2(h[2]), __habs2(h[3])));
     return max_abs(__low2float(m), __high2float(m));
 }
@@ -349,7 +367,7 @@ __global__ void __launch_bounds__(256) quantize_tile_kernel(const __grid_constan
                 float m = 0.f;
 #pragma unroll
                 for(int i = 0; i < 8; ++i)
-                    m = max_abs(m, to_f32(raw[i].v[k]));
+                    m = max_abs(m, value_of(raw[i], k));
                 s_max[unit * 128 + k * 16 + sub] = m; // [unit][k][sub]: lanes write neighbouring words
             }
             __syncthreads();
@@ -516,7 +534,7 @@ struct RowRing
     }
     __device__ __forceinline__ void read(Vec8<T>& r, int slot, int v) const
     {
-        uint32_t* d = reinterpret_cast<uint32_t*>(&r);
+        uint32_t(&d)[Vec8<T>::WORDS] = r.w;
 #pragma unroll
         for(int i = 0; i < PIECES; ++i)
             asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
@@ -923,12 +941,16 @@ __device__ __forceinline__ int column_of(int v, int i, int t, int tpr)
 template <typename T>
 __device__ __forceinline__ void load_columns(Vec8<T>& r, const T* row, int v, int t, int tpr, int N, bool on)
 {
+    uint32_t e[8];
 #pragma unroll
     for(int i = 0; i < 8; ++i)
     {
         const int c = column_of<true>(v, i, t, tpr);
-        r.v[i]      = on && c < N ? row[c] : from_f32<T>(0.f);
+        e[i]        = on && c < N ? bits_of(row[c]) : 0u;
     }
+#pragma unroll
+    for(int i = 0; i < Vec8<T>::WORDS; ++i)
+        r.w[i] = sizeof(T) == 4 ? e[i & 7] : e[(2 * i) & 7] | e[(2 * i + 1) & 7] << 16;
 }
 
 // dx and the partial sums of dgamma and dbeta in one pass.  A CTA walks rows blockIdx.x, + gridDim.x, ...; a thread keeps
