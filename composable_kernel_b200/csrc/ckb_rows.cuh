@@ -1204,41 +1204,44 @@ __global__ void __launch_bounds__(1024) layernorm_bwd_long_sums_kernel(const __g
     P.partial[(P.parts + blockIdx.y) * static_cast<int64_t>(P.N) + c] = db;
 }
 
-// Sums the partial column sums in the order of the parts.  32 columns a CTA, eight threads a column.
+// Sums the partial column sums, always in the same order: 32 columns a CTA, 32 threads a column (thread s takes parts
+// s, s + 32, ..., eight loads in flight; with eight threads a column this took longer than a third of a small backward
+// pass, all of it latency).
 template <typename T>
-__global__ void __launch_bounds__(256) layernorm_bwd_finish_kernel(const __grid_constant__ LayernormBwdParams P)
+__global__ void __launch_bounds__(1024) layernorm_bwd_finish_kernel(const __grid_constant__ LayernormBwdParams P)
 {
     grid_dependency_wait();
     grid_launch_dependents();
-    __shared__ float part[8][33];
+    __shared__ float part[32][33];
     const int lane = threadIdx.x & 31, slot = threadIdx.x >> 5;
     const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
     void* out       = blockIdx.y == 0 ? P.dgamma : P.dbeta;
-    const float* in = P.partial + static_cast<int64_t>(blockIdx.y) * P.parts * P.N;
+    if(!out)
+        return;
+    const float* in = P.partial + static_cast<int64_t>(blockIdx.y) * P.parts * P.N + c;
     float sum       = 0.f;
-    if(c < P.N && out)
+    if(c < P.N)
     {
-        int p = slot;
-        for(; p + 24 < P.parts; p += 32) // four loads in flight
+        for(int p = slot; p < P.parts; p += 256)
         {
-            const float a = in[static_cast<int64_t>(p) * P.N + c], b = in[static_cast<int64_t>(p + 8) * P.N + c];
-            const float d = in[static_cast<int64_t>(p + 16) * P.N + c], e = in[static_cast<int64_t>(p + 24) * P.N + c];
-            sum += (a + b) + (d + e);
+            float v[8];
+#pragma unroll
+            for(int i = 0; i < 8; ++i)
+                v[i] = p + i * 32 < P.parts ? in[static_cast<int64_t>(p + i * 32) * P.N] : 0.f;
+            sum += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
         }
-        for(; p < P.parts; p += 8)
-            sum += in[static_cast<int64_t>(p) * P.N + c];
     }
     part[slot][lane] = sum;
     __syncthreads();
-    if(slot == 0 && c < P.N && out)
+    // warp s sums column s: its lanes hold the 32 partial sums
+    const float total  = warp_sum(part[lane][slot]);
+    const int64_t mine = static_cast<int64_t>(blockIdx.x) * 32 + slot;
+    if(lane == 0 && mine < P.N)
     {
-#pragma unroll
-        for(int s = 1; s < 8; ++s)
-            sum += part[s][lane];
         if(P.w_f32)
-            static_cast<float*>(out)[c] = sum;
+            static_cast<float*>(out)[mine] = total;
         else
-            static_cast<T*>(out)[c] = from_f32<T>(sum);
+            static_cast<T*>(out)[mine] = from_f32<T>(total);
     }
 }
 

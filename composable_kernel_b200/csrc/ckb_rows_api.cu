@@ -222,7 +222,7 @@ cudaError_t launch_bwd(LayernormBwdParams p, cudaStream_t stream)
     }
     if(e != cudaSuccess || !sums)
         return e;
-    return launch(layernorm_bwd_finish_kernel<T>, div_up(p.N, 32), 2, 256, stream, p);
+    return launch(layernorm_bwd_finish_kernel<T>, div_up(p.N, 32), 2, 1024, stream, p);
 }
 
 } // namespace
@@ -315,19 +315,22 @@ int ckb_layernorm_fwd_run(const ckb_layernorm_fwd_desc* d, void* stream_, int n_
     // ones read again from L2.
     const int64_t units = div_up(d->N, 16);
     const bool warp = d->N <= 1024, lng = d->N > 16384, wide = d->N > 8192;
-    const int U     = warp && units <= 32 ? 1 : 2;
+    // a CTA that gets one row has nothing to gain from weights in shared memory: twice the threads, everything direct
+    // (7 rows of 4096: 3.4 us, 5.0 the other way)
+    const bool few  = !warp && !wide && d->M <= dev.sm_count;
+    const int U     = few || (warp && units <= 32) ? 1 : 2;
     p.tpr           = warp ? 32 : lng ? 1024 : static_cast<int>(div_up(div_up(units, U), 32) * 32);
     // parts of a CTA: 768 threads at most, rows and weights within shared memory, and no more than there are rows for
     const int ring = p.x_vec ? STAGE_DEPTH * U * 2 * 8 * xb * p.tpr : 0, weights = 2 * U * 16 * 4 * p.tpr;
     int parts      = warp ? 8 : 1;
-    if(!warp && !wide)
+    if(!warp && !wide && !few)
     {
         const int64_t rows = div_up(d->M, dev.sm_count);
         while(parts < 8 && (parts + 1) * p.tpr <= 768 && (parts + 1) * ring + weights <= kMaxSmem && parts < rows)
             ++parts;
     }
     const int threads  = parts * p.tpr;
-    const int smem     = warp || lng ? 0 : parts * ring + (wide ? 0 : weights);
+    const int smem     = warp || lng || few ? 0 : parts * ring + (wide ? 0 : weights);
     p.w_offset         = parts * ring;
     const int64_t want = div_up(d->M, parts);
     const int64_t most = static_cast<int64_t>(dev.sm_count) * (lng ? 2 : warp ? 8 : 1);
@@ -345,6 +348,8 @@ int ckb_layernorm_fwd_run(const ckb_layernorm_fwd_desc* d, void* stream_, int n_
                 if(warp)
                     return U == 1 ? launch(layernorm_fwd_kernel<T, E5, 1, ROW_WARP, false>, grid, 1, threads, stream, p)
                                   : launch(layernorm_fwd_kernel<T, E5, 2, ROW_WARP, false>, grid, 1, threads, stream, p);
+                if(few)
+                    return launch(layernorm_fwd_kernel<T, E5, 1, ROW_CTA, false>, grid, 1, threads, stream, p);
                 if(wide)
                     return p.x_vec ? launch_big<&layernorm_fwd_kernel<T, E5, 2, ROW_CTA, true>>(grid, threads, stream, p, smem)
                                    : launch(layernorm_fwd_kernel<T, E5, 2, ROW_CTA, false>, grid, 1, threads, stream, p);

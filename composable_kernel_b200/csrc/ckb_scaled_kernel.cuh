@@ -156,32 +156,35 @@ __device__ __forceinline__ __nv_bfloat16 scaled_out<__nv_bfloat16>(float v)
 // that neither side has bank conflicts.
 __device__ __forceinline__ uint32_t out_piece(int row, int c) { return row * 64 + ((c ^ ((row >> 1) & 3)) * 16); }
 
-// Writes one pass (columns n0 .. n0 + 64 bytes of the warp's COLS columns) to E.
-template <typename T, int COLS>
-__device__ __forceinline__ void store_pass(const uint8_t* tile, int n0, T* e, int64_t lde, int row0, int row_end, int col0,
-                                           int col_end, bool vec, int lane)
+// Writes one pass (columns n0 .. n0 + 64 bytes of the warp's COLS columns) to E.  `dst` is this lane's first piece: row
+// lane / 4, columns n0 + (lane % 4) * PER; rows: how many of the warp's 32 rows exist, cols: columns from n0 on that do.
+// `whole`: all of them, in 16-byte pieces.
+template <typename T, int LEFT>
+__device__ __forceinline__ void store_pass(const uint8_t* tile, T* dst, int64_t lde8, int rows, int cols, bool vec, bool whole, int lane)
 {
     constexpr int PER = 16 / sizeof(T); // values of a piece
-    const int c = lane & 3, n = n0 + c * PER;
-    if(n >= COLS)
+    const int c = lane & 3, n = c * PER;
+    if(LEFT < 4 * PER && n >= LEFT) // (the tile's columns end inside the pass)
         return;
 #pragma unroll
-    for(int i = 0; i < 4; ++i)
+    for(int i = 0; i < 4; ++i, dst += lde8)
     {
-        const int r = i * 8 + (lane >> 2);
-        if(row0 + r >= row_end)
-            continue;
+        const int r   = i * 8 + (lane >> 2);
         const uint4 v = *reinterpret_cast<const uint4*>(tile + out_piece(r, c));
-        T* dst        = e + static_cast<int64_t>(row0 + r) * lde + col0 + n;
-        if(vec && col0 + n + PER <= col_end)
+        if(whole)
             *reinterpret_cast<uint4*>(dst) = v;
-        else
+        else if(r < rows)
         {
-            const T* w = reinterpret_cast<const T*>(&v);
+            if(vec && n + PER <= cols)
+                *reinterpret_cast<uint4*>(dst) = v;
+            else
+            {
+                const T* w = reinterpret_cast<const T*>(&v);
 #pragma unroll
-            for(int j = 0; j < PER; ++j)
-                if(col0 + n + j < col_end)
-                    dst[j] = w[j];
+                for(int j = 0; j < PER; ++j)
+                    if(n + j < cols)
+                        dst[j] = w[j];
+            }
         }
     }
 }
@@ -195,6 +198,10 @@ __device__ __forceinline__ void store_rows(const uint64_t (&acc)[COLS / 2], uint
     constexpr int PER  = 16 / sizeof(T);
     constexpr int PASS = 4 * PER; // columns of a pass
     static_assert(COLS % 8 == 0, "whole pieces and fragments");
+    const int rows     = row_end - row0, cols = col_end - col0;
+    const bool whole   = vec && rows >= 32 && cols >= COLS;
+    const int64_t lde8 = 8 * lde;
+    T* dst             = e + static_cast<int64_t>(row0 + (lane >> 2)) * lde + col0 + (lane & 3) * PER;
 #pragma unroll
     for(int n0 = 0; n0 < COLS; n0 += PASS)
     {
@@ -235,7 +242,7 @@ __device__ __forceinline__ void store_rows(const uint64_t (&acc)[COLS / 2], uint
                 }
         }
         __syncwarp();
-        store_pass<T, COLS>(tile, n0, e, lde, row0, row_end, col0, col_end, vec, lane);
+        store_pass<T, (COLS - PASS < 0 ? COLS : PASS)>(tile, dst + n0, lde8, rows, cols - n0 < COLS - n0 ? cols - n0 : COLS - n0, vec, whole && n0 + PASS <= COLS, lane);
     }
 }
 
@@ -246,15 +253,17 @@ __device__ __forceinline__ void store_cols(const uint64_t (&acc)[COLS / 2], T* e
 {
     if(u >= u_end)
         return;
+    const int rows = v_end - v0;
+    T* dst         = e + static_cast<int64_t>(v0) * lde + u;
 #pragma unroll
-    for(int c = 0; c < COLS; c += 2)
+    for(int c = 0; c < COLS; c += 2, dst += 2 * lde)
     {
         float lo, hi;
         unpack_f32x2(acc[c / 2], lo, hi);
-        if(v0 + c < v_end)
-            e[static_cast<int64_t>(v0 + c) * lde + u] = scaled_out<T>(lo);
-        if(v0 + c + 1 < v_end)
-            e[static_cast<int64_t>(v0 + c + 1) * lde + u] = scaled_out<T>(hi);
+        if(c < rows)
+            dst[0] = scaled_out<T>(lo);
+        if(c + 1 < rows)
+            dst[lde] = scaled_out<T>(hi);
     }
 }
 
