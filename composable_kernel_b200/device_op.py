@@ -460,16 +460,21 @@ class DescArgument(BaseArgument):
 class _DescOperator(BaseOperator):
     """Operations whose argument is one C descriptor: ``ckb_<_name>_supported`` and ``ckb_<_name>_run``."""
     _name = ""
+    _entry = None  # the run function, looked up at the first call
 
     def IsSupportedArgument(self, arg: DescArgument) -> bool:
         return getattr(capi.lib(), f"ckb_{self._name}_supported")(arg.ref) == capi.CKB_OK
 
+    def _run_entry(self):
+        self._entry = getattr(capi.lib(), f"ckb_{self._name}_run")
+        return self._entry
+
     def _launch(self, arg: DescArgument, stream, n_rep: int) -> int:
-        return getattr(capi.lib(), f"ckb_{self._name}_run")(arg.ref, stream, n_rep, arg.ms_ref)
+        return (self._entry or self._run_entry())(arg.ref, stream, n_rep, arg.ms_ref)
 
     def _run(self, arg: DescArgument, sc: StreamConfig) -> float:
         rc = self._launch(arg, sc.stream_id, sc.nrepeat if sc.time_kernel else 0)
-        if rc != capi.CKB_OK:
+        if rc:
             msg = capi.last_error()
             if rc in (capi.CKB_ERR_UNSUPPORTED, capi.CKB_ERR_INVALID):
                 msg = f"wrong! {type(self).__name__} has invalid setting: {msg}"
@@ -621,7 +626,8 @@ class DeviceLayernormBwd(_DescOperator):
         return int(n.value)
 
     def _launch(self, arg: DescArgument, stream, n_rep: int) -> int:
-        return capi.lib().ckb_layernorm_bwd_run(arg.ref, arg.p_workspace_, arg.workspace_bytes_ or 0, stream, n_rep, arg.ms_ref)
+        return (self._entry or self._run_entry())(arg.ref, arg.p_workspace_, arg.workspace_bytes_ or 0, stream, n_rep,
+                                                  arg.ms_ref)
 
 
 def device_status() -> int:
