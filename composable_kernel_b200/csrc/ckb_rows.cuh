@@ -36,11 +36,26 @@ __device__ __forceinline__ uint32_t bits_of(float v) { return __float_as_uint(v)
 __device__ __forceinline__ uint32_t bits_of(__half v) { return __half_as_ushort(v); }
 __device__ __forceinline__ uint32_t bits_of(__nv_bfloat16 v) { return __bfloat16_as_ushort(v); }
 
-// `n` = values that exist (<= 0: none, the vector is zero); `vec`: p is 16-byte aligned.
+// What a partial or unaligned vector needs is in functions of its own: inlined, the compiler turns it into predicated
+// instructions that every vector issues (a quarter to a half of all instructions of these kernels).
+// `n` = values that exist (<= 0: none, the vector is zero).
+template <typename T>
+__device__ __noinline__ Vec8<T> load8_slow(const T* p, int n)
+{
+    Vec8<T> r;
+    uint32_t e[8];
+#pragma unroll
+    for(int i = 0; i < 8; ++i)
+        e[i] = i < n ? bits_of(p[i]) : 0u;
+#pragma unroll
+    for(int i = 0; i < Vec8<T>::WORDS; ++i)
+        r.w[i] = sizeof(T) == 4 ? e[i & 7] : e[(2 * i) & 7] | e[(2 * i + 1) & 7] << 16;
+    return r;
+}
 template <typename T>
 __device__ __forceinline__ void load8(Vec8<T>& r, const T* p, int n, bool vec)
 {
-    if(vec && n >= 8)
+    if(vec && n >= 8) // p is 16-byte aligned
     {
         const uint4* s = reinterpret_cast<const uint4*>(p);
 #pragma unroll
@@ -51,15 +66,7 @@ __device__ __forceinline__ void load8(Vec8<T>& r, const T* p, int n, bool vec)
         }
     }
     else
-    {
-        uint32_t e[8];
-#pragma unroll
-        for(int i = 0; i < 8; ++i)
-            e[i] = i < n ? bits_of(p[i]) : 0u;
-#pragma unroll
-        for(int i = 0; i < Vec8<T>::WORDS; ++i)
-            r.w[i] = sizeof(T) == 4 ? e[i & 7] : e[(2 * i) & 7] | e[(2 * i + 1) & 7] << 16;
-    }
+        r = load8_slow(p, n);
 }
 
 // Two values, rounded, in one word (f32: as they are).
@@ -72,6 +79,15 @@ __device__ __forceinline__ uint32_t round_pair(const __nv_bfloat16*, float lo, f
 {
     const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <typename T>
+__device__ __noinline__ void store8_slow(float4 lo, float4 hi, T* p, int n)
+{
+    const float f[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+    for(int i = 0; i < 8; ++i)
+        if(i < n)
+            p[i] = from_f32<T>(f[i]);
 }
 template <typename T>
 __device__ __forceinline__ void store8(const float (&f)[8], T* p, int n, bool vec)
@@ -87,13 +103,8 @@ __device__ __forceinline__ void store8(const float (&f)[8], T* p, int n, bool ve
             *reinterpret_cast<uint4*>(p) = make_uint4(round_pair(p, f[0], f[1]), round_pair(p, f[2], f[3]), round_pair(p, f[4], f[5]),
                                                       round_pair(p, f[6], f[7]));
     }
-    else
-    {
-#pragma unroll
-        for(int i = 0; i < 8; ++i)
-            if(i < n)
-                p[i] = from_f32<T>(f[i]);
-    }
+    else if(n > 0)
+        store8_slow(make_float4(f[0], f[1], f[2], f[3]), make_float4(f[4], f[5], f[6], f[7]), p, n);
 }
 
 // ---- 8-bit blocks ------------------------------------------------------------------------------
@@ -112,23 +123,20 @@ __device__ __forceinline__ float max16(float v) // over 16 neighbouring lanes
     return v;
 }
 
+__device__ __noinline__ float block_scale_slow(float amax, float qmax)
+{
+    const float s = __fdiv_rn(amax, qmax);
+    return s < 1.17549435e-38f ? 1.17549435e-38f : s; // (a NaN stays)
+}
 // amax / qmax, correctly rounded (see below), at least the smallest normal number (its reciprocal still exists).
 __device__ __forceinline__ float block_scale(float amax, float qmax, float qmax_recip, bool pow2)
 {
     if(amax == 0.f)
         return 1.f;
-    float s;
-    if(amax >= 1e-28f && amax <= 3.402823466e+38f)
-    {
-        const float q0 = amax * qmax_recip;
-        s              = __fmaf_rn(__fmaf_rn(-q0, qmax, amax), qmax_recip, q0);
-    }
-    else // tiny, infinite or NaN
-    {
-        s = __fdiv_rn(amax, qmax);
-        if(s < 1.17549435e-38f)
-            s = 1.17549435e-38f;
-    }
+    const float q0 = amax * qmax_recip;
+    float s        = __fmaf_rn(__fmaf_rn(-q0, qmax, amax), qmax_recip, q0);
+    if(!(amax >= 1e-28f && amax <= 3.402823466e+38f)) // tiny, infinite or NaN
+        s = block_scale_slow(amax, qmax);
     if(pow2)
     {
         const uint32_t b = __float_as_uint(s);
@@ -167,29 +175,32 @@ __device__ __forceinline__ uint32_t to_f8x2(float lo, float hi)
 
 // Eight values (four pairs) over one scale -> eight bytes.
 template <bool E5M2>
+__device__ __noinline__ uint2 quantize8_slow(ulonglong2 a, ulonglong2 b, float scale)
+{
+    const uint64_t f[4] = {a.x, a.y, b.x, b.y};
+    uint32_t w[4];
+#pragma unroll
+    for(int i = 0; i < 4; ++i)
+    {
+        float lo, hi;
+        unpack_f32x2(f[i], lo, hi);
+        w[i] = to_f8x2<E5M2>(__fdiv_rn(lo, scale), __fdiv_rn(hi, scale));
+    }
+    return make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+}
+template <bool E5M2>
 __device__ __forceinline__ uint2 quantize8(const uint64_t (&f)[4], const BlockDivisor& d)
 {
+    if(!d.fast)
+        return quantize8_slow<E5M2>(make_ulonglong2(f[0], f[1]), make_ulonglong2(f[2], f[3]), d.scale);
     uint32_t w[4];
-    if(d.fast)
-    {
-        const uint64_t ns = pack_f32x2(-d.scale, -d.scale), r = pack_f32x2(d.recip, d.recip);
+    const uint64_t ns = pack_f32x2(-d.scale, -d.scale), r = pack_f32x2(d.recip, d.recip);
 #pragma unroll
-        for(int i = 0; i < 4; ++i)
-        {
-            float lo, hi;
-            unpack_f32x2(div_pair(f[i], ns, r), lo, hi);
-            w[i] = to_f8x2<E5M2>(lo, hi);
-        }
-    }
-    else
+    for(int i = 0; i < 4; ++i)
     {
-#pragma unroll
-        for(int i = 0; i < 4; ++i)
-        {
-            float lo, hi;
-            unpack_f32x2(f[i], lo, hi);
-            w[i] = to_f8x2<E5M2>(__fdiv_rn(lo, d.scale), __fdiv_rn(hi, d.scale));
-        }
+        float lo, hi;
+        unpack_f32x2(div_pair(f[i], ns, r), lo, hi);
+        w[i] = to_f8x2<E5M2>(lo, hi);
     }
     return make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
 }
@@ -246,17 +257,19 @@ __device__ __forceinline__ float max_abs8(const Vec8<__nv_bfloat16>& r)
     return max_abs(__low2float(m), __high2float(m));
 }
 
+__device__ __noinline__ void store_q8_slow(uint2 w, uint8_t* p, int n)
+{
+#pragma unroll
+    for(int i = 0; i < 8; ++i)
+        if(i < n)
+            p[i] = static_cast<uint8_t>((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
+}
 __device__ __forceinline__ void store_q8(uint2 w, uint8_t* p, int n, bool vec)
 {
     if(vec && n >= 8)
         *reinterpret_cast<uint2*>(p) = w;
-    else
-    {
-#pragma unroll
-        for(int i = 0; i < 8; ++i)
-            if(i < n)
-                p[i] = static_cast<uint8_t>((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
-    }
+    else if(n > 0)
+        store_q8_slow(w, p, n);
 }
 
 struct QuantizeParams
@@ -509,37 +522,54 @@ __device__ __forceinline__ float rstd_of(float square, float shift, float eps)
     return __frsqrt_rn((var < 0.f ? 0.f : var) + eps); // (a NaN stays one)
 }
 
-// Rows on their way: asynchronous copies into shared memory, DEPTH rows ahead.  Every thread copies the vectors it works
-// on itself and reads nobody else's, so only its own copies have to be waited for.  Vector v of thread t lies in pieces of
-// 16 bytes, [row of the ring][vector][piece][thread].
+// Rows on their way: asynchronous copies into shared memory, STAGE_DEPTH - 1 rows ahead.  Every thread copies the vectors
+// it works on itself and reads nobody else's, so only its own copies have to be waited for.  A warp's part of the ring is
+// [row][vector][16-byte piece][lane]: with that, and with a warp's columns side by side in the matrix, all addresses of a
+// row are one register plus constants (laid out over the whole CTA the address arithmetic was 200 of 640 instructions per
+// row and thread).
 constexpr int STAGE_DEPTH = 3;
 template <typename T, int V>
 struct RowRing
 {
     static constexpr int PIECES = sizeof(T) / 2; // 16-byte pieces of a vector
     static constexpr int PER    = 16 / sizeof(T);
-    uint32_t base;                               // this thread's first piece
-    int threads;
+    static constexpr int SLOT   = V * PIECES * 512; // bytes of a row and warp
+    uint32_t base;                                  // this lane's first piece
     static __host__ __device__ int bytes(int threads) { return STAGE_DEPTH * V * PIECES * threads * 16; }
+    __device__ __forceinline__ RowRing(const void* smem)
+        : base(smem_u32(smem) + (threadIdx.x >> 5) * (STAGE_DEPTH * SLOT) + (threadIdx.x & 31) * 16)
+    {
+    }
     // `n` = values of the row from the vector's first one on (<= 0: none, p is not read)
     __device__ __forceinline__ void copy(int slot, int v, const T* p, int n) const
     {
-        const uint32_t dst = base + (((slot * V + v) * PIECES) * threads) * 16;
+        const uint32_t dst = base + slot * SLOT + v * (PIECES * 512);
+        if(n >= 8)
+        {
+#pragma unroll
+            for(int i = 0; i < PIECES; ++i)
+                copy_async_16(dst + i * 512, p + i * PER, 16);
+        }
+        else
+            copy_slow(dst, p, n);
+    }
+    static __device__ __noinline__ void copy_slow(uint32_t dst, const T* p, int n)
+    {
 #pragma unroll
         for(int i = 0; i < PIECES; ++i)
         {
             const int have = (n - i * PER) * static_cast<int>(sizeof(T)); // bytes
-            copy_async_16(dst + i * threads * 16, p + i * PER, have < 0 ? 0 : have > 16 ? 16 : have);
+            copy_async_16(dst + i * 512, have > 0 ? p + i * PER : p, have < 0 ? 0 : have > 16 ? 16 : have);
         }
     }
     __device__ __forceinline__ void read(Vec8<T>& r, int slot, int v) const
     {
-        uint32_t(&d)[Vec8<T>::WORDS] = r.w;
+        const uint32_t src = base + slot * SLOT + v * (PIECES * 512);
 #pragma unroll
         for(int i = 0; i < PIECES; ++i)
             asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                         : "=r"(d[4 * i]), "=r"(d[4 * i + 1]), "=r"(d[4 * i + 2]), "=r"(d[4 * i + 3])
-                         : "r"(base + (((slot * V + v) * PIECES + i) * threads) * 16)
+                         : "=r"(r.w[4 * i]), "=r"(r.w[4 * i + 1]), "=r"(r.w[4 * i + 2]), "=r"(r.w[4 * i + 3])
+                         : "r"(src + i * 512)
                          : "memory");
     }
 };
@@ -595,6 +625,29 @@ __device__ __forceinline__ float sum_f32x2(uint64_t a)
     unpack_f32x2(a, lo, hi);
     return lo + hi;
 }
+struct Pairs4
+{
+    uint64_t p[4];
+};
+// The first n values of eight, zero for the others.
+__device__ __noinline__ Pairs4 first_of(Pairs4 d, int n)
+{
+#pragma unroll
+    for(int i = 0; i < 4; ++i)
+    {
+        float lo, hi;
+        unpack_f32x2(d.p[i], lo, hi);
+        d.p[i] = pack_f32x2(2 * i < n ? lo : 0.f, 2 * i + 1 < n ? hi : 0.f);
+    }
+    return d;
+}
+__device__ __forceinline__ void keep_first(uint64_t (&d)[4], int n)
+{
+    const Pairs4 r = first_of(Pairs4{{d[0], d[1], d[2], d[3]}}, n);
+#pragma unroll
+    for(int i = 0; i < 4; ++i)
+        d[i] = r.p[i];
+}
 // Subtracts `mean` from the eight values, zero where there is no value (n of them exist).
 __device__ __forceinline__ void distances(uint64_t (&d)[4], float mean, int n)
 {
@@ -603,57 +656,43 @@ __device__ __forceinline__ void distances(uint64_t (&d)[4], float mean, int n)
     for(int i = 0; i < 4; ++i)
         d[i] = add_f32x2(d[i], m2);
     if(n < 8)
-    {
-#pragma unroll
-        for(int i = 0; i < 4; ++i)
-        {
-            float lo, hi;
-            unpack_f32x2(d[i], lo, hi);
-            d[i] = pack_f32x2(2 * i < n ? lo : 0.f, 2 * i + 1 < n ? hi : 0.f);
-        }
-    }
+        keep_first(d, n);
 }
 
-// y (and q) of the 16 columns from c on: y = (d - shift) * rstd * gamma + beta, d = distances to the first mean.
-// Eight neighbouring lanes hold a block of 128.  weights(u, g, b): gamma and beta of columns c + 8 u .. + 7.
+// y (and q) of 16 columns, `have` of which (at most) exist: y = (d - shift) * rstd * gamma + beta, d = distances to the first
+// mean.  Eight neighbouring lanes hold a block of 128, whose scale goes to `scale`.  weights(h, g, b): gamma and beta of
+// columns 8 h .. + 7.
 template <typename T, bool E5M2, typename Weights>
-__device__ __forceinline__ void layernorm_out16(const LayernormFwdParams& P, int64_t row, int c, uint64_t (&d)[2][4], float shift, float rstd,
-                                                Weights weights)
+__device__ __forceinline__ void layernorm_out16(const LayernormFwdParams& P, T* y_out, uint8_t* q_out, float* scale, int have, uint64_t (&d)[2][4],
+                                                float shift, float rstd, Weights weights)
 {
     const uint64_t r2 = pack_f32x2(rstd, rstd), s2 = pack_f32x2(-shift, -shift);
     float m = 0.f;
 #pragma unroll
     for(int u = 0; u < 2; ++u)
     {
-        const int cu = c + u * 8, n = P.N - cu;
+        const int n = have - u * 8;
         uint64_t g[4], b[4];
         weights(u, g, b);
         float y[8];
 #pragma unroll
         for(int i = 0; i < 4; ++i)
-        {
             d[u][i] = fma_f32x2(mul_f32x2(add_f32x2(d[u][i], s2), r2), g[i], b[i]);
+        if(n < 8)
+            keep_first(d[u], n); // (what does not exist must not count in a block's largest value)
+#pragma unroll
+        for(int i = 0; i < 4; ++i)
             unpack_f32x2(d[u][i], y[2 * i], y[2 * i + 1]);
-        }
-        if(P.y)
-            store8(y, static_cast<T*>(P.y) + row * P.ldy + cu, n, P.y_vec != 0);
-        if(P.q)
+        if(y_out)
+            store8(y, y_out + u * 8, n, P.y_vec != 0);
+        if(q_out)
         {
-            if(n >= 8)
-            {
 #pragma unroll
-                for(int i = 0; i < 8; ++i)
-                    m = max_abs(m, y[i]);
-            }
-            else
-            {
-#pragma unroll
-                for(int i = 0; i < 8; ++i)
-                    m = max_abs(m, i < n ? y[i] : 0.f);
-            }
+            for(int i = 0; i < 8; ++i)
+                m = max_abs(m, y[i]);
         }
     }
-    if(P.q)
+    if(q_out)
     {
 #pragma unroll
         for(int k = 4; k >= 1; k >>= 1)
@@ -661,22 +700,20 @@ __device__ __forceinline__ void layernorm_out16(const LayernormFwdParams& P, int
         const float s = block_scale(m, P.qmax, P.qmax_recip, false);
         const BlockDivisor div(s);
         const uint2 w0 = quantize8<E5M2>(d[0], div), w1 = quantize8<E5M2>(d[1], div);
-        const int n = P.N - c;
-        uint8_t* q  = P.q + row * P.ldq + c;
-        if(P.q_vec && n >= 16)
-            *reinterpret_cast<uint4*>(q) = make_uint4(w0.x, w0.y, w1.x, w1.y);
+        if(P.q_vec && have >= 16)
+            *reinterpret_cast<uint4*>(q_out) = make_uint4(w0.x, w0.y, w1.x, w1.y);
         else
         {
-            store_q8(w0, q, n, false);
-            store_q8(w1, q + 8, n - 8, false);
+            store_q8(w0, q_out, have, false);
+            store_q8(w1, q_out + 8, have - 8, false);
         }
-        if((threadIdx.x & 7) == 0 && n > 0)
-            P.q_scale[row * P.ss_m + (c >> 7) * P.ss_n] = s;
+        if((threadIdx.x & 7) == 0 && have > 0)
+            *scale = s;
     }
 }
 
-// U units of 16 values a thread: unit u of thread t holds columns 16 (u * threads + t) .. + 15, so a scale block belongs to
-// eight lanes.
+// U units of 16 values a thread: unit u of a lane of the row's warp w holds columns 512 (w U + u) + 16 lane .. + 15, so a
+// scale block belongs to eight lanes.
 //   ROW_WARP   a row per warp, eight rows a CTA
 //   ROW_GROUP  one CTA per SM works on as many rows side by side as fit; gamma and beta wait in shared memory in 32 bits
 //              (read for every row from L2 they were 2.6 times the bytes of the rows, and their latency most of the time)
@@ -703,18 +740,11 @@ __global__ void __launch_bounds__(KIND == ROW_WARP ? 256 : KIND == ROW_GROUP ? 7
     const float inv_n   = 1.f / static_cast<float>(P.N);
     float* buf          = sums + (KIND == ROW_GROUP ? group * 192 : 0); // two rows in turn, 96 words each
     Vec8<T> raw[U][2];
-    RowRing<T, 2 * U> ring{smem_u32(ring_smem) + group * RowRing<T, 2 * U>::bytes(tpr) + t * 16, tpr};
-    auto column = [&](int u, int h) { return (u * tpr + t) * 16 + h * 8; };
-    int have[U][2]; // values of the row in each vector (and, first of all, where it starts: the row's start if it has none)
-    const T* ahead[U][2]; // of the row that is fetched next
-#pragma unroll
-    for(int u = 0; u < U; ++u)
-#pragma unroll
-        for(int h = 0; h < 2; ++h)
-        {
-            have[u][h]  = P.N - column(u, h);
-            ahead[u][h] = x + row * P.ldx + (have[u][h] > 0 ? column(u, h) : 0);
-        }
+    const RowRing<T, 2 * U> ring(ring_smem);
+    const int col0 = (t >> 5) * (U * 512) + (t & 31) * 16; // this thread's first column
+    auto offset = [](int u, int h) { return u * 512 + h * 8; };
+    const int have   = P.N - col0; // values of the row from there on
+    const T* ahead   = x + row * P.ldx + (have > 0 ? col0 : 0); // of the row that is fetched next
     const int64_t row_step = step * P.ldx;
     int64_t ahead_row      = row;
     auto fetch = [&](int slot) {
@@ -727,14 +757,14 @@ __global__ void __launch_bounds__(KIND == ROW_WARP ? 256 : KIND == ROW_GROUP ? 7
                 if constexpr(RING)
                 {
                     if(on)
-                        ring.copy(slot, 2 * u + h, ahead[u][h], have[u][h]);
+                        ring.copy(slot, 2 * u + h, ahead + offset(u, h), have - offset(u, h));
                 }
                 else
-                    load8(raw[u][h], ahead[u][h], on ? have[u][h] : 0, P.x_vec != 0);
-                ahead[u][h] += row_step;
+                    load8(raw[u][h], ahead + offset(u, h), on ? have - offset(u, h) : 0, P.x_vec != 0);
             }
         if constexpr(RING)
             copy_async_commit();
+        ahead += row_step;
         ahead_row += step;
     };
     int slot = 0;
@@ -743,15 +773,16 @@ __global__ void __launch_bounds__(KIND == ROW_WARP ? 256 : KIND == ROW_GROUP ? 7
 #pragma unroll
         for(int i = 1; i < STAGE_DEPTH - 1; ++i)
             fetch(i);
-    // ROW_GROUP: [gamma, beta][unit][four values][thread]
-    float4* w_smem = reinterpret_cast<float4*>(ring_smem + (KIND == ROW_GROUP ? P.w_offset : 0));
+    // ROW_GROUP: [warp of the row][gamma, beta][unit][half][four values][lane]
+    constexpr int W_WARP = 2 * U * 2 * 2 * 32; // 16-byte pieces of a warp
+    float4* w_smem       = reinterpret_cast<float4*>(ring_smem + (KIND == ROW_GROUP ? P.w_offset : 0));
     if constexpr(KIND == ROW_GROUP)
     {
         for(int i = threadIdx.x; i < 2 * U * 2 * tpr; i += blockDim.x)
         {
-            // vector i of 8 weights: [which][unit][half][thread]
-            const int which = i / (U * 2 * tpr), rest = i - which * (U * 2 * tpr), uh = rest / tpr, th = rest - uh * tpr;
-            const int c = ((uh >> 1) * tpr + th) * 16 + (uh & 1) * 8;
+            const int ln = i & 31, vec = (i >> 5) % (2 * U * 2), w = (i >> 5) / (2 * U * 2);
+            const int which = vec / (U * 2), uh = vec % (U * 2);
+            const int c     = w * (U * 512) + (uh >> 1) * 512 + ln * 16 + (uh & 1) * 8;
             uint64_t f[4];
             load_weights8<T>(f, which ? P.beta : P.gamma, P.w_f32 != 0, c < P.N ? c : 0, c < P.N ? P.N : 0, P.w_vec != 0, which ? 0.f : 1.f);
 #pragma unroll
@@ -760,11 +791,15 @@ __global__ void __launch_bounds__(KIND == ROW_WARP ? 256 : KIND == ROW_GROUP ? 7
                 float4 v;
                 unpack_f32x2(f[2 * k], v.x, v.y);
                 unpack_f32x2(f[2 * k + 1], v.z, v.w);
-                w_smem[((which * U * 2 + uh) * 2 + k) * tpr + th] = v;
+                w_smem[w * W_WARP + (vec * 2 + k) * 32 + ln] = v;
             }
         }
         __syncthreads();
     }
+    const float4* w_mine = w_smem + (t >> 5) * W_WARP + (t & 31);
+    T* y_row             = P.y ? static_cast<T*>(P.y) + row * P.ldy + col0 : nullptr;
+    uint8_t* q_row       = P.q ? P.q + row * P.ldq + col0 : nullptr;
+    float* s_row         = P.q ? P.q_scale + row * P.ss_m + (col0 >> 7) * P.ss_n : nullptr;
     int flip = 0;
     for(; row < P.M; row += step)
     {
@@ -799,7 +834,7 @@ __global__ void __launch_bounds__(KIND == ROW_WARP ? 256 : KIND == ROW_GROUP ? 7
 #pragma unroll
             for(int h = 0; h < 2; ++h)
             {
-                distances(d[u][h], mean, have[u][h]);
+                distances(d[u][h], mean, have - offset(u, h));
 #pragma unroll
                 for(int i = 0; i < 4; ++i)
                 {
@@ -821,25 +856,31 @@ __global__ void __launch_bounds__(KIND == ROW_WARP ? 256 : KIND == ROW_GROUP ? 7
         }
 #pragma unroll
         for(int u = 0; u < U; ++u)
-            if(!__all_sync(0xffffffffu, column(u, 0) >= P.N))
-                layernorm_out16<T, E5M2>(P, row, column(u, 0), d[u], shift, rstd, [&](int h, uint64_t (&g)[4], uint64_t (&b)[4]) {
+            if(!__all_sync(0xffffffffu, have - offset(u, 0) <= 0))
+                layernorm_out16<T, E5M2>(P, y_row ? y_row + offset(u, 0) : nullptr, q_row ? q_row + offset(u, 0) : nullptr, s_row + u * 4 * P.ss_n,
+                                         have - offset(u, 0), d[u], shift, rstd, [&](int h, uint64_t (&g)[4], uint64_t (&b)[4]) {
                     if constexpr(KIND == ROW_GROUP)
                     {
 #pragma unroll
                         for(int k = 0; k < 2; ++k)
                         {
-                            const ulonglong2 gv = *reinterpret_cast<const ulonglong2*>(w_smem + ((u * 2 + h) * 2 + k) * tpr + t);
-                            const ulonglong2 bv = *reinterpret_cast<const ulonglong2*>(w_smem + ((U * 2 + u * 2 + h) * 2 + k) * tpr + t);
+                            const ulonglong2 gv = *reinterpret_cast<const ulonglong2*>(w_mine + ((u * 2 + h) * 2 + k) * 32);
+                            const ulonglong2 bv = *reinterpret_cast<const ulonglong2*>(w_mine + ((U * 2 + u * 2 + h) * 2 + k) * 32);
                             g[2 * k] = gv.x, g[2 * k + 1] = gv.y, b[2 * k] = bv.x, b[2 * k + 1] = bv.y;
                         }
                     }
                     else
                     {
-                        const int c = column(u, h);
+                        const int c = col0 + offset(u, h);
                         load_weights8<T>(g, P.gamma, P.w_f32 != 0, c, P.N, P.w_vec != 0, 1.f);
                         load_weights8<T>(b, P.beta, P.w_f32 != 0, c, P.N, P.w_vec != 0, 0.f);
                     }
                 });
+        if(y_row)
+            y_row += step * P.ldy;
+        if(q_row)
+            q_row += step * P.ldq;
+        s_row += step * P.ss_m;
         flip ^= 96;
     }
     if constexpr(RING)
@@ -909,7 +950,9 @@ __global__ void __launch_bounds__(1024) layernorm_fwd_long_kernel(const __grid_c
                 to_pairs(r, d[h]);
                 distances(d[h], mean, m);
             }
-            layernorm_out16<T, E5M2>(P, row, cc, d, shift, rstd, [&](int h, uint64_t (&g)[4], uint64_t (&b)[4]) {
+            layernorm_out16<T, E5M2>(P, P.y ? static_cast<T*>(P.y) + row * P.ldy + cc : nullptr, P.q ? P.q + row * P.ldq + cc : nullptr,
+                                     P.q ? P.q_scale + row * P.ss_m + (cc >> 7) * P.ss_n : nullptr, P.N - cc, d, shift, rstd,
+                                     [&](int h, uint64_t (&g)[4], uint64_t (&b)[4]) {
                 load_weights8<T>(g, P.gamma, P.w_f32 != 0, cc + h * 8, P.N, P.w_vec != 0, 1.f);
                 load_weights8<T>(b, P.beta, P.w_f32 != 0, cc + h * 8, P.N, P.w_vec != 0, 0.f);
             });
@@ -933,10 +976,10 @@ struct LayernormBwdParams
 
 // Where element i of vector v of a thread lies.  STRIDED: neighbouring lanes hold neighbouring columns, for rows that
 // do not start on 16-byte boundaries.
-template <bool STRIDED>
+template <int V, bool STRIDED>
 __device__ __forceinline__ int column_of(int v, int i, int t, int tpr)
 {
-    return STRIDED ? (v * 8 + i) * tpr + t : (v * tpr + t) * 8 + i;
+    return STRIDED ? (v * 8 + i) * tpr + t : ((t >> 5) * V + v) * 256 + (t & 31) * 8 + i;
 }
 template <typename T>
 __device__ __forceinline__ void load_columns(Vec8<T>& r, const T* row, int v, int t, int tpr, int N, bool on)
@@ -945,7 +988,7 @@ __device__ __forceinline__ void load_columns(Vec8<T>& r, const T* row, int v, in
 #pragma unroll
     for(int i = 0; i < 8; ++i)
     {
-        const int c = column_of<true>(v, i, t, tpr);
+        const int c = column_of<1, true>(v, i, t, tpr);
         e[i]        = on && c < N ? bits_of(row[c]) : 0u;
     }
 #pragma unroll
@@ -975,7 +1018,7 @@ __global__ void __launch_bounds__(V == 1 ? 128 : 512, V == 1 ? 4 : 1) layernorm_
 #pragma unroll
         for(int i = 0; i < 8; ++i)
         {
-            const int c = column_of<STRIDED>(v, i, t, tpr);
+            const int c = column_of<V, STRIDED>(v, i, t, tpr);
             f[i]        = 0.f;
             if(c < P.N)
                 f[i] = !P.gamma ? 1.f : P.w_f32 ? static_cast<const float*>(P.gamma)[c] : to_f32(static_cast<const T*>(P.gamma)[c]);
@@ -988,22 +1031,12 @@ __global__ void __launch_bounds__(V == 1 ? 128 : 512, V == 1 ? 4 : 1) layernorm_
         }
     }
     Vec8<T> rx[V], ry[V];
-    RowRing<T, 2 * V> ring{smem_u32(ring_smem) + t * 16, tpr}; // vectors of x, then of dy
+    const RowRing<T, 2 * V> ring(ring_smem); // vectors of x, then of dy
     float mean = 0.f, rstd = 0.f;
-    // of the row that is fetched next: its start, or the start of each vector of this thread
-    const T *x_ahead[STRIDED ? 1 : V], *dy_ahead[STRIDED ? 1 : V];
-    int have[V]; // values of the row in each vector
-#pragma unroll
-    for(int v = 0; v < V; ++v)
-    {
-        const int c = STRIDED ? 0 : column_of<false>(v, 0, t, tpr);
-        have[v]     = P.N - c;
-        if(!STRIDED || v == 0)
-        {
-            x_ahead[STRIDED ? 0 : v]  = x + blockIdx.x * P.ldx + (have[v] > 0 ? c : 0);
-            dy_ahead[STRIDED ? 0 : v] = dy + blockIdx.x * P.lddy + (have[v] > 0 ? c : 0);
-        }
-    }
+    const int col0 = STRIDED ? 0 : column_of<V, false>(0, 0, t, tpr);
+    const int have = P.N - col0; // values of the row from this thread's first column on
+    const T* x_ahead  = x + blockIdx.x * P.ldx + (have > 0 ? col0 : 0); // of the row that is fetched next
+    const T* dy_ahead = dy + blockIdx.x * P.lddy + (have > 0 ? col0 : 0);
     const int64_t x_step = gridDim.x * P.ldx, dy_step = gridDim.x * P.lddy;
     int64_t ahead_row = blockIdx.x;
     auto fetch = [&](int slot) {
@@ -1013,31 +1046,23 @@ __global__ void __launch_bounds__(V == 1 ? 128 : 512, V == 1 ? 4 : 1) layernorm_
         {
             if constexpr(STRIDED)
             {
-                load_columns<T>(rx[v], x_ahead[0], v, t, tpr, P.N, on);
-                load_columns<T>(ry[v], dy_ahead[0], v, t, tpr, P.N, on);
+                load_columns<T>(rx[v], x_ahead, v, t, tpr, P.N, on);
+                load_columns<T>(ry[v], dy_ahead, v, t, tpr, P.N, on);
             }
-            else
+            else if(on)
             {
-                if(on)
-                {
-                    ring.copy(slot, v, x_ahead[v], have[v]);
-                    ring.copy(slot, V + v, dy_ahead[v], have[v]);
-                }
-                x_ahead[v] += x_step;
-                dy_ahead[v] += dy_step;
+                ring.copy(slot, v, x_ahead + v * 256, have - v * 256);
+                ring.copy(slot, V + v, dy_ahead + v * 256, have - v * 256);
             }
         }
-        if constexpr(STRIDED)
-        {
-            x_ahead[0] += x_step;
-            dy_ahead[0] += dy_step;
-        }
-        else
+        x_ahead += x_step;
+        dy_ahead += dy_step;
+        if constexpr(!STRIDED)
             copy_async_commit();
         ahead_row += gridDim.x;
     };
     const float *mean_at = P.mean + blockIdx.x, *rstd_at = P.rstd + blockIdx.x;
-    T* out               = static_cast<T*>(P.dx) + (P.dx ? blockIdx.x * P.lddx : 0);
+    T* out               = P.dx ? static_cast<T*>(P.dx) + blockIdx.x * P.lddx + col0 : nullptr;
     const int64_t dx_step = gridDim.x * P.lddx;
     auto statistics = [&](bool on) {
         mean = on ? __ldg(mean_at) : 0.f;
@@ -1114,18 +1139,19 @@ __global__ void __launch_bounds__(V == 1 ? 128 : 512, V == 1 ? 4 : 1) layernorm_
 #pragma unroll
                     for(int i = 0; i < 8; ++i)
                     {
-                        const int c = column_of<true>(v, i, t, tpr);
+                        const int c = column_of<1, true>(v, i, t, tpr);
                         if(c < P.N)
                             out[c] = from_f32<T>(o[i]);
                     }
                 }
                 else
                 {
-                    store8(o, out + column_of<false>(v, 0, t, tpr), have[v], true);
+                    store8(o, out + v * 256, have - v * 256, true);
                 }
             }
         }
-        out += dx_step;
+        if(P.dx)
+            out += dx_step;
         if(++slot == STAGE_DEPTH)
             slot = 0;
     }
@@ -1140,7 +1166,7 @@ __global__ void __launch_bounds__(V == 1 ? 128 : 512, V == 1 ? 4 : 1) layernorm_
 #pragma unroll
             for(int i = 0; i < 8; ++i)
             {
-                const int c = column_of<STRIDED>(v, i, t, tpr);
+                const int c = column_of<V, STRIDED>(v, i, t, tpr);
                 float a[2], b[2];
                 unpack_f32x2(dg[v][i / 2], a[0], a[1]);
                 unpack_f32x2(db[v][i / 2], b[0], b[1]);
