@@ -522,12 +522,175 @@ __device__ __forceinline__ float rstd_of(float square, float shift, float eps)
     return __frsqrt_rn((var < 0.f ? 0.f : var) + eps); // (a NaN stays one)
 }
 
-// Rows on their way: asynchronous copies into shared memory, STAGE_DEPTH - 1 rows ahead.  Every thread copies the vectors
-// it works on itself and reads nobody else's, so only its own copies have to be waited for.  A warp's part of the ring is
+// Words of shared memory from byte `off` (0 .. 15) behind a 16-byte boundary on.
+template <int NW>
+__device__ __forceinline__ void lds_words(uint32_t (&out)[NW], uint32_t addr, int off)
+{
+    uint32_t w[NW + 4];
+    auto load = [&](int i) {
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(w[4 * i]), "=r"(w[4 * i + 1]), "=r"(w[4 * i + 2]), "=r"(w[4 * i + 3])
+                     : "r"(addr + i * 16)
+                     : "memory");
+    };
+#pragma unroll
+    for(int i = 0; i < NW / 4; ++i)
+        load(i);
+    if(off == 0)
+    {
+#pragma unroll
+        for(int i = 0; i < NW; ++i)
+            out[i] = w[i];
+        return;
+    }
+    load(NW / 4);
+    if(off & 8)
+    {
+#pragma unroll
+        for(int i = 0; i < NW + 2; ++i)
+            w[i] = w[i + 2];
+    }
+    if(off & 4)
+    {
+#pragma unroll
+        for(int i = 0; i < NW + 1; ++i)
+            w[i] = w[i + 1];
+    }
+#pragma unroll
+    for(int i = 0; i < NW; ++i)
+        out[i] = __funnelshift_r(w[i], w[i + 1], (off & 3) * 8);
+}
+__device__ __forceinline__ void sts_words(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d)
+{
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+// Rows on their way: asynchronous copies into shared memory, STAGE_DEPTH - 1 rows ahead.  A warp has ELEMS neighbouring
+// values of the row and a ring of its own; only its lanes have to meet.  Rows may start anywhere: the 16-byte pieces that
+// hold them are copied whole and in order (a sector is fetched once, whatever vectors the lanes work on), and a lane
+// shifts its vectors out of them.  (The piece that holds a tensor's first values may begin up to 15 bytes before the
+// tensor, inside the same allocation: those start on 256-byte boundaries.)
+constexpr int STAGE_DEPTH = 3;
+template <typename T, int ELEMS>
+struct WarpRing
+{
+    static constexpr int BYTES = ELEMS * sizeof(T);
+    static constexpr int SLOT  = BYTES + 16;
+    uint32_t base; // of the warp
+    static __host__ __device__ int bytes(int threads) { return STAGE_DEPTH * SLOT * (threads / 32); }
+    __device__ __forceinline__ WarpRing(const void* smem, int which = 0, int of = 1)
+        : base(smem_u32(smem) + ((threadIdx.x >> 5) * of + which) * (STAGE_DEPTH * SLOT))
+    {
+    }
+    // `n` = values of the row from p, the warp's first one, on
+    __device__ __forceinline__ void copy(int slot, const T* p, int n) const
+    {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+        const int off      = static_cast<int>(at & 15);
+        const char* src    = reinterpret_cast<const char*>(at - off) + (threadIdx.x & 31) * 16;
+        const uint32_t dst = base + slot * SLOT + (threadIdx.x & 31) * 16;
+        const int all      = n < ELEMS ? n : ELEMS;                                                              // values
+        const int left     = off + all * static_cast<int>(sizeof(T)) - (static_cast<int>(threadIdx.x) & 31) * 16; // bytes from this lane's piece on
+        if(off == 0 && all == ELEMS)
+        {
+#pragma unroll
+            for(int i = 0; i < BYTES / 512; ++i)
+                copy_async_16(dst + i * 512, src + i * 512, 16);
+        }
+        else if(all > 0)
+        {
+#pragma unroll
+            for(int i = 0; i <= BYTES / 512; ++i)
+            {
+                const int have = left - i * 512;
+                if(i < BYTES / 512 || (threadIdx.x & 31) == 0) // (one piece more than the values fill)
+                    copy_async_16(dst + i * 512, have > 0 ? src + i * 512 : src, have < 0 ? 0 : have > 16 ? 16 : have);
+            }
+        }
+    }
+    // words of the `count` values from value `first` of the span on (first * sizeof(T) a multiple of 16)
+    template <int NW>
+    __device__ __forceinline__ void read(uint32_t (&w)[NW], int slot, int first, int off) const
+    {
+        lds_words(w, base + slot * SLOT + first * static_cast<int>(sizeof(T)), off);
+    }
+};
+
+// A warp's values leave through a piece of its shared memory, 16 bytes per lane and instruction, in order.  `stage` holds
+// BYTES of output from its start on; dst: where its first byte goes (any alignment); n: how many bytes exist.
+template <int BYTES, int ELEM>
+__device__ __forceinline__ void store_span(uint32_t stage, uint8_t* dst, int n)
+{
+    const int lane = threadIdx.x & 31;
+    const int off  = static_cast<int>(reinterpret_cast<uintptr_t>(dst) & 15);
+    __syncwarp();
+    if(off == 0 && n >= BYTES)
+    {
+#pragma unroll
+        for(int i = 0; i < (BYTES + 511) / 512; ++i)
+        {
+            if(BYTES % 512 != 0 && i * 512 + lane * 16 >= BYTES)
+                break;
+            uint32_t w[4];
+            lds_words(w, stage + i * 512 + lane * 16, 0);
+            *reinterpret_cast<uint4*>(dst + i * 512 + lane * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+    else
+    {
+        if(n > BYTES)
+            n = BYTES;
+        for(int j = lane; 16 * j - off < n; j += 32)
+        {
+            const int from = 16 * j - off; // piece j of dst takes bytes from .. from + 15 of the stage
+            if(from >= 0 && from + 16 <= n)
+            {
+                uint32_t w[4];
+                lds_words(w, stage + (from & ~15), from & 15);
+                *reinterpret_cast<uint4*>(dst + from) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            else
+            {
+                for(int b = from < 0 ? 0 : from; b < from + 16 && b < n; b += ELEM)
+                {
+                    uint32_t v;
+                    if constexpr(ELEM == 4)
+                        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(stage + b) : "memory");
+                    else if constexpr(ELEM == 2)
+                        asm volatile("{.reg .b16 t; ld.shared.b16 t, [%1]; cvt.u32.u16 %0, t;}" : "=r"(v) : "r"(stage + b) : "memory");
+                    else
+                        asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(stage + b) : "memory");
+                    if constexpr(ELEM == 4)
+                        *reinterpret_cast<uint32_t*>(dst + b) = v;
+                    else if constexpr(ELEM == 2)
+                        *reinterpret_cast<uint16_t*>(dst + b) = static_cast<uint16_t>(v);
+                    else
+                        dst[b] = static_cast<uint8_t>(v);
+                }
+            }
+        }
+    }
+    __syncwarp();
+}
+// Eight values, rounded to T, into the stage.
+template <typename T>
+__device__ __forceinline__ void stage8(uint32_t addr, const float (&f)[8])
+{
+    const T* t = nullptr;
+    if constexpr(sizeof(T) == 4)
+    {
+        sts_words(addr, __float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+        sts_words(addr + 16, __float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7]));
+    }
+    else
+        sts_words(addr, round_pair(t, f[0], f[1]), round_pair(t, f[2], f[3]), round_pair(t, f[4], f[5]), round_pair(t, f[6], f[7]));
+}
+
+// The same for rows that start on 16-byte boundaries and vectors that lie in order: every thread copies the vectors it
+// works on itself and reads nobody else's, so only its own copies have to be waited for.  A warp's part of the ring is
 // [row][vector][16-byte piece][lane]: with that, and with a warp's columns side by side in the matrix, all addresses of a
 // row are one register plus constants (laid out over the whole CTA the address arithmetic was 200 of 640 instructions per
 // row and thread).
-constexpr int STAGE_DEPTH = 3;
 template <typename T, int V>
 struct RowRing
 {
@@ -659,57 +822,46 @@ __device__ __forceinline__ void distances(uint64_t (&d)[4], float mean, int n)
         keep_first(d, n);
 }
 
-// y (and q) of 16 columns, `have` of which (at most) exist: y = (d - shift) * rstd * gamma + beta, d = distances to the first
-// mean.  Eight neighbouring lanes hold a block of 128, whose scale goes to `scale`.  weights(h, g, b): gamma and beta of
-// columns 8 h .. + 7.
-template <typename T, bool E5M2, typename Weights>
-__device__ __forceinline__ void layernorm_out16(const LayernormFwdParams& P, T* y_out, uint8_t* q_out, float* scale, int have, uint64_t (&d)[2][4],
-                                                float shift, float rstd, Weights weights)
+// y of 16 columns, `have` of which (at most) exist: y = (d - shift) * rstd * gamma + beta, d = distances to the first mean
+// (zero where there is no value).  weights(h, g, b): gamma and beta of columns 8 h .. + 7.
+template <typename Weights>
+__device__ __forceinline__ void layernorm_y16(uint64_t (&d)[2][4], int have, float shift, float rstd, Weights weights)
 {
     const uint64_t r2 = pack_f32x2(rstd, rstd), s2 = pack_f32x2(-shift, -shift);
+#pragma unroll
+    for(int h = 0; h < 2; ++h)
+    {
+        uint64_t g[4], b[4];
+        weights(h, g, b);
+#pragma unroll
+        for(int i = 0; i < 4; ++i)
+            d[h][i] = fma_f32x2(mul_f32x2(add_f32x2(d[h][i], s2), r2), g[i], b[i]);
+        if(have - h * 8 < 8)
+            keep_first(d[h], have - h * 8); // (what does not exist must not count in a block's largest value)
+    }
+}
+// Eight neighbouring lanes hold a block of 128 columns: its scale, and this lane's sixteen values over it.
+template <bool E5M2>
+__device__ __forceinline__ float layernorm_q16(const uint64_t (&d)[2][4], float qmax, float qmax_recip, uint4& q)
+{
     float m = 0.f;
 #pragma unroll
-    for(int u = 0; u < 2; ++u)
-    {
-        const int n = have - u * 8;
-        uint64_t g[4], b[4];
-        weights(u, g, b);
-        float y[8];
+    for(int h = 0; h < 2; ++h)
 #pragma unroll
         for(int i = 0; i < 4; ++i)
-            d[u][i] = fma_f32x2(mul_f32x2(add_f32x2(d[u][i], s2), r2), g[i], b[i]);
-        if(n < 8)
-            keep_first(d[u], n); // (what does not exist must not count in a block's largest value)
-#pragma unroll
-        for(int i = 0; i < 4; ++i)
-            unpack_f32x2(d[u][i], y[2 * i], y[2 * i + 1]);
-        if(y_out)
-            store8(y, y_out + u * 8, n, P.y_vec != 0);
-        if(q_out)
         {
-#pragma unroll
-            for(int i = 0; i < 8; ++i)
-                m = max_abs(m, y[i]);
+            float lo, hi;
+            unpack_f32x2(d[h][i], lo, hi);
+            m = max_abs(max_abs(m, lo), hi);
         }
-    }
-    if(q_out)
-    {
 #pragma unroll
-        for(int k = 4; k >= 1; k >>= 1)
-            m = max_abs(m, __shfl_xor_sync(0xffffffffu, m, k));
-        const float s = block_scale(m, P.qmax, P.qmax_recip, false);
-        const BlockDivisor div(s);
-        const uint2 w0 = quantize8<E5M2>(d[0], div), w1 = quantize8<E5M2>(d[1], div);
-        if(P.q_vec && have >= 16)
-            *reinterpret_cast<uint4*>(q_out) = make_uint4(w0.x, w0.y, w1.x, w1.y);
-        else
-        {
-            store_q8(w0, q_out, have, false);
-            store_q8(w1, q_out + 8, have - 8, false);
-        }
-        if((threadIdx.x & 7) == 0 && have > 0)
-            *scale = s;
-    }
+    for(int k = 4; k >= 1; k >>= 1)
+        m = max_abs(m, __shfl_xor_sync(0xffffffffu, m, k));
+    const float s = block_scale(m, qmax, qmax_recip, false);
+    const BlockDivisor div(s);
+    const uint2 w0 = quantize8<E5M2>(d[0], div), w1 = quantize8<E5M2>(d[1], div);
+    q = make_uint4(w0.x, w0.y, w1.x, w1.y);
+    return s;
 }
 
 // U units of 16 values a thread: unit u of a lane of the row's warp w holds columns 512 (w U + u) + 16 lane .. + 15, so a
@@ -717,12 +869,11 @@ __device__ __forceinline__ void layernorm_out16(const LayernormFwdParams& P, T* 
 //   ROW_WARP   a row per warp, eight rows a CTA
 //   ROW_GROUP  one CTA per SM works on as many rows side by side as fit; gamma and beta wait in shared memory in 32 bits
 //              (read for every row from L2 they were 2.6 times the bytes of the rows, and their latency most of the time)
-//   ROW_CTA    longer rows: the weights from L2
-// RING: rows come through shared memory, STAGE_DEPTH - 1 rows ahead.  What bounds it is instructions (about 25 per value
-// with 8-bit output): units of 16 values instead of 8 halve those for the scale of a block.
+//   ROW_CTA    longer rows, or a row per CTA: the weights from L2
+// Rows come and go through shared memory in 16-byte pieces, in order (WarpRing, store_span).
 // Mean and variance in two passes over the registers; the second pass also sums the distances themselves, which takes
 // the rounding of the first mean out of both.
-template <typename T, bool E5M2, int U, int KIND, bool RING>
+template <typename T, bool E5M2, int U, int KIND>
 __global__ void __launch_bounds__(KIND == ROW_WARP ? 256 : KIND == ROW_GROUP ? 768 : 512, KIND == ROW_WARP ? 2 : 1)
     layernorm_fwd_kernel(const __grid_constant__ LayernormFwdParams P)
 {
@@ -734,45 +885,32 @@ __global__ void __launch_bounds__(KIND == ROW_WARP ? 256 : KIND == ROW_GROUP ? 7
     const int groups    = KIND == ROW_WARP ? 8 : static_cast<int>(blockDim.x) / tpr;
     const int group     = static_cast<int>(threadIdx.x) / tpr;
     const int t         = static_cast<int>(threadIdx.x) - group * tpr;
+    const int lane      = t & 31;
     const int64_t step  = static_cast<int64_t>(gridDim.x) * groups;
     int64_t row         = static_cast<int64_t>(blockIdx.x) * groups + group;
     const T* x          = static_cast<const T*>(P.x);
     const float inv_n   = 1.f / static_cast<float>(P.N);
     float* buf          = sums + (KIND == ROW_GROUP ? group * 192 : 0); // two rows in turn, 96 words each
-    Vec8<T> raw[U][2];
-    const RowRing<T, 2 * U> ring(ring_smem);
-    const int col0 = (t >> 5) * (U * 512) + (t & 31) * 16; // this thread's first column
-    auto offset = [](int u, int h) { return u * 512 + h * 8; };
-    const int have   = P.N - col0; // values of the row from there on
-    const T* ahead   = x + row * P.ldx + (have > 0 ? col0 : 0); // of the row that is fetched next
+    using Ring          = WarpRing<T, U * 512>;
+    const Ring ring(ring_smem);
+    const int warp_col  = (t >> 5) * (U * 512);           // the warp's first column
+    const int warp_have = P.N - warp_col;                 // values of the row from there on
+    const int have      = warp_have - lane * 16;          // and from this lane's first one on
+    const T* ahead      = x + row * P.ldx + (warp_have > 0 ? warp_col : 0); // of the row that is fetched next
+    const T* now        = ahead;
     const int64_t row_step = step * P.ldx;
     int64_t ahead_row      = row;
     auto fetch = [&](int slot) {
-        const bool on = ahead_row < P.M;
-#pragma unroll
-        for(int u = 0; u < U; ++u)
-#pragma unroll
-            for(int h = 0; h < 2; ++h)
-            {
-                if constexpr(RING)
-                {
-                    if(on)
-                        ring.copy(slot, 2 * u + h, ahead + offset(u, h), have - offset(u, h));
-                }
-                else
-                    load8(raw[u][h], ahead + offset(u, h), on ? have - offset(u, h) : 0, P.x_vec != 0);
-            }
-        if constexpr(RING)
-            copy_async_commit();
+        if(ahead_row < P.M)
+            ring.copy(slot, ahead, warp_have);
+        copy_async_commit();
         ahead += row_step;
         ahead_row += step;
     };
     int slot = 0;
-    fetch(0);
-    if constexpr(RING)
 #pragma unroll
-        for(int i = 1; i < STAGE_DEPTH - 1; ++i)
-            fetch(i);
+    for(int i = 0; i < STAGE_DEPTH - 1; ++i)
+        fetch(i);
     // ROW_GROUP: [warp of the row][gamma, beta][unit][half][four values][lane]
     constexpr int W_WARP = 2 * U * 2 * 2 * 32; // 16-byte pieces of a warp
     float4* w_smem       = reinterpret_cast<float4*>(ring_smem + (KIND == ROW_GROUP ? P.w_offset : 0));
@@ -796,37 +934,38 @@ __global__ void __launch_bounds__(KIND == ROW_WARP ? 256 : KIND == ROW_GROUP ? 7
         }
         __syncthreads();
     }
-    const float4* w_mine = w_smem + (t >> 5) * W_WARP + (t & 31);
-    T* y_row             = P.y ? static_cast<T*>(P.y) + row * P.ldy + col0 : nullptr;
-    uint8_t* q_row       = P.q ? P.q + row * P.ldq + col0 : nullptr;
-    float* s_row         = P.q ? P.q_scale + row * P.ss_m + (col0 >> 7) * P.ss_n : nullptr;
-    int flip = 0;
+    const float4* w_mine = w_smem + (t >> 5) * W_WARP + lane;
+    T* y_row             = static_cast<T*>(P.y) + (P.y ? row * P.ldy + warp_col : 0);
+    uint8_t* q_row       = P.q + (P.q ? row * P.ldq + warp_col : 0);
+    float* s_row         = P.q_scale + (P.q ? row * P.ss_m + ((warp_col + lane * 16) >> 7) * P.ss_n : 0);
+    int flip             = 0;
     for(; row < P.M; row += step)
     {
-        if constexpr(RING)
-        {
-            fetch(slot == 0 ? STAGE_DEPTH - 1 : slot - 1);
-            copy_async_wait<STAGE_DEPTH - 1>();
-#pragma unroll
-            for(int u = 0; u < U; ++u)
-#pragma unroll
-                for(int h = 0; h < 2; ++h)
-                    ring.read(raw[u][h], slot, 2 * u + h);
-            if(++slot == STAGE_DEPTH)
-                slot = 0;
-        }
+        __syncwarp(); // the slot that is filled now was the last row's way out
+        fetch(slot == 0 ? STAGE_DEPTH - 1 : slot - 1);
+        copy_async_wait<STAGE_DEPTH - 1>();
+        __syncwarp();
+        const int off = static_cast<int>(reinterpret_cast<uintptr_t>(now) & 15);
         uint64_t d[U][2][4];
         uint64_t sv = 0;
 #pragma unroll
         for(int u = 0; u < U; ++u)
+        {
+            uint32_t w[4 * sizeof(T)];
+            ring.read(w, slot, u * 512 + lane * 16, off);
 #pragma unroll
             for(int h = 0; h < 2; ++h)
             {
-                to_pairs(raw[u][h], d[u][h]);
+                Vec8<T> r;
+#pragma unroll
+                for(int i = 0; i < Vec8<T>::WORDS; ++i)
+                    r.w[i] = w[h * Vec8<T>::WORDS + i];
+                to_pairs(r, d[u][h]);
+                if(have - u * 512 - h * 8 < 8)
+                    keep_first(d[u][h], have - u * 512 - h * 8); // (what lies behind the row's end was never copied)
                 sv = add_f32x2(sv, add_f32x2(add_f32x2(d[u][h][0], d[u][h][1]), add_f32x2(d[u][h][2], d[u][h][3])));
             }
-        if constexpr(!RING)
-            fetch(0);
+        }
         float mean   = row_sum<KIND>(sum_f32x2(sv), buf + flip, group, tpr) * inv_n;
         uint64_t s1v = 0, s2v = 0;
 #pragma unroll
@@ -834,7 +973,7 @@ __global__ void __launch_bounds__(KIND == ROW_WARP ? 256 : KIND == ROW_GROUP ? 7
 #pragma unroll
             for(int h = 0; h < 2; ++h)
             {
-                distances(d[u][h], mean, have - offset(u, h));
+                distances(d[u][h], mean, have - u * 512 - h * 8);
 #pragma unroll
                 for(int i = 0; i < 4; ++i)
                 {
@@ -854,11 +993,13 @@ __global__ void __launch_bounds__(KIND == ROW_WARP ? 256 : KIND == ROW_GROUP ? 7
             if(P.rstd)
                 P.rstd[row] = rstd;
         }
+        if(warp_have > 0)
+        {
+            const uint32_t stage = ring.base + slot * Ring::SLOT; // (the row is in registers)
 #pragma unroll
-        for(int u = 0; u < U; ++u)
-            if(!__all_sync(0xffffffffu, have - offset(u, 0) <= 0))
-                layernorm_out16<T, E5M2>(P, y_row ? y_row + offset(u, 0) : nullptr, q_row ? q_row + offset(u, 0) : nullptr, s_row + u * 4 * P.ss_n,
-                                         have - offset(u, 0), d[u], shift, rstd, [&](int h, uint64_t (&g)[4], uint64_t (&b)[4]) {
+            for(int u = 0; u < U; ++u)
+            {
+                layernorm_y16(d[u], have - u * 512, shift, rstd, [&](int h, uint64_t (&g)[4], uint64_t (&b)[4]) {
                     if constexpr(KIND == ROW_GROUP)
                     {
 #pragma unroll
@@ -871,20 +1012,60 @@ __global__ void __launch_bounds__(KIND == ROW_WARP ? 256 : KIND == ROW_GROUP ? 7
                     }
                     else
                     {
-                        const int c = col0 + offset(u, h);
+                        const int c = warp_col + u * 512 + lane * 16 + h * 8;
                         load_weights8<T>(g, P.gamma, P.w_f32 != 0, c, P.N, P.w_vec != 0, 1.f);
                         load_weights8<T>(b, P.beta, P.w_f32 != 0, c, P.N, P.w_vec != 0, 0.f);
                     }
                 });
-        if(y_row)
-            y_row += step * P.ldy;
-        if(q_row)
-            q_row += step * P.ldq;
+            }
+            __syncwarp(); // every lane has read its part of the row
+            if(P.y)
+            {
+#pragma unroll
+                for(int u = 0; u < U; ++u)
+#pragma unroll
+                    for(int h = 0; h < 2; ++h)
+                    {
+                        float y[8];
+#pragma unroll
+                        for(int i = 0; i < 4; ++i)
+                            unpack_f32x2(d[u][h][i], y[2 * i], y[2 * i + 1]);
+                        stage8<T>(stage + (u * 512 + lane * 16 + h * 8) * static_cast<int>(sizeof(T)), y);
+                    }
+                store_span<Ring::BYTES, sizeof(T)>(stage, reinterpret_cast<uint8_t*>(y_row), warp_have < U * 512 ? warp_have * static_cast<int>(sizeof(T)) : Ring::BYTES);
+            }
+            if(P.q)
+            {
+#pragma unroll
+                for(int u = 0; u < U; ++u)
+                {
+                    uint4 q;
+                    const float s = layernorm_q16<E5M2>(d[u], P.qmax, P.qmax_recip, q);
+                    if((lane & 7) == 0 && have - u * 512 > 0)
+                        s_row[u * 4 * P.ss_n] = s;
+                    if(P.q_vec && have - u * 512 >= 16) // (16 bytes a lane, in order already)
+                        *reinterpret_cast<uint4*>(q_row + u * 512 + lane * 16) = q;
+                    else if(!P.q_vec)
+                        sts_words(stage + u * 512 + lane * 16, q.x, q.y, q.z, q.w);
+                    else if(have - u * 512 > 0)
+                    {
+                        store_q8(make_uint2(q.x, q.y), q_row + u * 512 + lane * 16, have - u * 512, false);
+                        store_q8(make_uint2(q.z, q.w), q_row + u * 512 + lane * 16 + 8, have - u * 512 - 8, false);
+                    }
+                }
+                if(!P.q_vec)
+                    store_span<U * 512, 1>(stage, q_row, warp_have < U * 512 ? warp_have : U * 512);
+            }
+        }
+        now += row_step;
+        y_row += step * P.ldy;
+        q_row += step * P.ldq;
         s_row += step * P.ss_m;
+        if(++slot == STAGE_DEPTH)
+            slot = 0;
         flip ^= 96;
     }
-    if constexpr(RING)
-        copy_async_wait_all();
+    copy_async_wait_all();
 }
 
 // Rows that do not fit the registers of a CTA: the row is read three times (the second and third time from L2).
@@ -950,12 +1131,29 @@ __global__ void __launch_bounds__(1024) layernorm_fwd_long_kernel(const __grid_c
                 to_pairs(r, d[h]);
                 distances(d[h], mean, m);
             }
-            layernorm_out16<T, E5M2>(P, P.y ? static_cast<T*>(P.y) + row * P.ldy + cc : nullptr, P.q ? P.q + row * P.ldq + cc : nullptr,
-                                     P.q ? P.q_scale + row * P.ss_m + (cc >> 7) * P.ss_n : nullptr, P.N - cc, d, shift, rstd,
-                                     [&](int h, uint64_t (&g)[4], uint64_t (&b)[4]) {
+            layernorm_y16(d, P.N - cc, shift, rstd, [&](int h, uint64_t (&g)[4], uint64_t (&b)[4]) {
                 load_weights8<T>(g, P.gamma, P.w_f32 != 0, cc + h * 8, P.N, P.w_vec != 0, 1.f);
                 load_weights8<T>(b, P.beta, P.w_f32 != 0, cc + h * 8, P.N, P.w_vec != 0, 0.f);
             });
+            if(P.y)
+#pragma unroll
+                for(int h = 0; h < 2; ++h)
+                {
+                    float y[8];
+#pragma unroll
+                    for(int i = 0; i < 4; ++i)
+                        unpack_f32x2(d[h][i], y[2 * i], y[2 * i + 1]);
+                    store8(y, static_cast<T*>(P.y) + row * P.ldy + cc + h * 8, P.N - cc - h * 8, P.y_vec != 0);
+                }
+            if(P.q)
+            {
+                uint4 q;
+                const float s = layernorm_q16<E5M2>(d, P.qmax, P.qmax_recip, q);
+                if((t & 7) == 0 && cc < P.N)
+                    P.q_scale[row * P.ss_m + (cc >> 7) * P.ss_n] = s;
+                store_q8(make_uint2(q.x, q.y), P.q + row * P.ldq + cc, P.N - cc, P.q_vec != 0);
+                store_q8(make_uint2(q.z, q.w), P.q + row * P.ldq + cc + 8, P.N - cc - 8, P.q_vec != 0);
+            }
         }
         __syncthreads(); // buf is used again
     }
@@ -971,7 +1169,8 @@ struct LayernormBwdParams
     int64_t lddy, ldx, lddx;
     int64_t M;
     int32_t N, parts;
-    int32_t w_f32, vec, w_vec;
+    int32_t w_f32, w_vec;
+    int32_t vec; // rows of dy, x and dx start on 16-byte boundaries
 };
 
 // Where element i of vector v of a thread lies.  STRIDED: neighbouring lanes hold neighbouring columns, for rows that
@@ -1167,6 +1366,153 @@ __global__ void __launch_bounds__(V == 1 ? 128 : 512, V == 1 ? 4 : 1) layernorm_
             for(int i = 0; i < 8; ++i)
             {
                 const int c = column_of<V, STRIDED>(v, i, t, tpr);
+                float a[2], b[2];
+                unpack_f32x2(dg[v][i / 2], a[0], a[1]);
+                unpack_f32x2(db[v][i / 2], b[0], b[1]);
+                if(c < P.N)
+                {
+                    pg[c] = a[i & 1];
+                    pb[c] = b[i & 1];
+                }
+            }
+    }
+}
+
+// The same with rows that come and go through shared memory in whole 16-byte pieces, as in the forward pass, for 16-bit
+// rows that start anywhere (8192 x 4097 in bf16: 122 us, STRIDED 249; with rows on 16-byte boundaries the kernel above takes
+// 50 us for 4096 columns and this one 65) and for 32-bit rows on 16-byte boundaries (8192 x 4096: 94 us, 118 the other way;
+// rows that start anywhere: 167, STRIDED 143).  Vector v of a lane of warp w: columns 256 (w V + v) + 8 lane .. + 7.
+template <typename T, int V>
+__global__ void __launch_bounds__(V == 1 ? 128 : 512, V == 1 ? 4 : 1) layernorm_bwd_shifted_kernel(const __grid_constant__ LayernormBwdParams P)
+{
+    grid_dependency_wait();
+    grid_launch_dependents();
+    extern __shared__ __align__(16) uint8_t ring_smem[];
+    __shared__ float buf[2 * 64];
+    const int tpr = blockDim.x, t = threadIdx.x, lane = t & 31;
+    const float inv_n = 1.f / static_cast<float>(P.N);
+    const int warp_col = (t >> 5) * (V * 256), warp_have = P.N - warp_col, have = warp_have - lane * 8;
+    uint64_t g[V][4], dg[V][4], db[V][4];
+#pragma unroll
+    for(int v = 0; v < V; ++v)
+    {
+        const int c = warp_col + v * 256 + lane * 8;
+        load_weights8<T>(g[v], P.gamma, P.w_f32 != 0, c < P.N ? c : 0, c < P.N ? P.N : 0, P.w_vec != 0, 1.f);
+        if(have - v * 256 < 8)
+            keep_first(g[v], have - v * 256);
+#pragma unroll
+        for(int i = 0; i < 4; ++i)
+            dg[v][i] = db[v][i] = 0;
+    }
+    using Ring = WarpRing<T, V * 256>;
+    const Ring x_ring(ring_smem, 0, 2), dy_ring(ring_smem, 1, 2);
+    const T* x_ahead  = static_cast<const T*>(P.x) + blockIdx.x * P.ldx + (warp_have > 0 ? warp_col : 0); // of the row that is fetched next
+    const T* dy_ahead = static_cast<const T*>(P.dy) + blockIdx.x * P.lddy + (warp_have > 0 ? warp_col : 0);
+    const T *x_now = x_ahead, *dy_now = dy_ahead;
+    const int64_t x_step = gridDim.x * P.ldx, dy_step = gridDim.x * P.lddy;
+    int64_t ahead_row = blockIdx.x;
+    auto fetch = [&](int slot) {
+        if(ahead_row < P.M)
+        {
+            x_ring.copy(slot, x_ahead, warp_have);
+            dy_ring.copy(slot, dy_ahead, warp_have);
+        }
+        copy_async_commit();
+        x_ahead += x_step;
+        dy_ahead += dy_step;
+        ahead_row += gridDim.x;
+    };
+    const float *mean_at = P.mean + blockIdx.x, *rstd_at = P.rstd + blockIdx.x;
+    T* out                = static_cast<T*>(P.dx) + (P.dx ? blockIdx.x * P.lddx + warp_col : 0);
+    const int64_t dx_step = gridDim.x * P.lddx;
+    float mean = 0.f, rstd = 0.f;
+    auto statistics = [&](bool on) {
+        mean = on ? __ldg(mean_at) : 0.f;
+        rstd = on ? __ldg(rstd_at) : 0.f;
+        mean_at += gridDim.x;
+        rstd_at += gridDim.x;
+    };
+    int64_t row = blockIdx.x;
+    int slot    = 0;
+#pragma unroll
+    for(int i = 0; i < STAGE_DEPTH - 1; ++i)
+        fetch(i);
+    statistics(row < P.M);
+    int flip = 0;
+    for(; row < P.M; row += gridDim.x)
+    {
+        __syncwarp(); // the slot that is filled now was the last row's way out
+        fetch(slot == 0 ? STAGE_DEPTH - 1 : slot - 1);
+        copy_async_wait<STAGE_DEPTH - 1>();
+        __syncwarp();
+        const int x_off = static_cast<int>(reinterpret_cast<uintptr_t>(x_now) & 15), dy_off = static_cast<int>(reinterpret_cast<uintptr_t>(dy_now) & 15);
+        const uint64_t m2 = pack_f32x2(-mean, -mean), r2 = pack_f32x2(rstd, rstd);
+        const float rs = rstd;
+        uint64_t h[V][4], w[V][4];
+        uint64_t s1v = 0, s2v = 0;
+#pragma unroll
+        for(int v = 0; v < V; ++v)
+        {
+            Vec8<T> rx, ry;
+            x_ring.read(rx.w, slot, v * 256 + lane * 8, x_off);
+            dy_ring.read(ry.w, slot, v * 256 + lane * 8, dy_off);
+            uint64_t gy[4];
+            to_pairs(rx, h[v]);
+            to_pairs(ry, gy);
+            if(have - v * 256 < 8)
+            {
+                keep_first(h[v], have - v * 256); // (what lies behind the row's end was never copied)
+                keep_first(gy, have - v * 256);
+            }
+            // (behind the row's end dy and gamma are zero, and so is all that xhat is multiplied with)
+#pragma unroll
+            for(int i = 0; i < 4; ++i)
+            {
+                h[v][i]  = mul_f32x2(add_f32x2(h[v][i], m2), r2);
+                w[v][i]  = mul_f32x2(gy[i], g[v][i]);
+                dg[v][i] = fma_f32x2(gy[i], h[v][i], dg[v][i]);
+                db[v][i] = add_f32x2(db[v][i], gy[i]);
+                s1v      = add_f32x2(s1v, w[v][i]);
+                s2v      = fma_f32x2(w[v][i], h[v][i], s2v);
+            }
+        }
+        float s1 = sum_f32x2(s1v), s2 = sum_f32x2(s2v);
+        statistics(row + gridDim.x < P.M);
+        row_sum2<ROW_CTA>(s1, s2, buf + flip, 0, tpr);
+        flip ^= 64;
+        if(P.dx && warp_have > 0)
+        {
+            const float c1 = s1 * inv_n, c2 = s2 * inv_n;
+            const uint64_t c1v = pack_f32x2(-c1, -c1), c2v = pack_f32x2(-c2, -c2), rsv = pack_f32x2(rs, rs);
+            const uint32_t stage = x_ring.base + slot * Ring::SLOT; // (the row is in registers, and all lanes have met since)
+#pragma unroll
+            for(int v = 0; v < V; ++v)
+            {
+                float o[8];
+#pragma unroll
+                for(int i = 0; i < 4; ++i)
+                    unpack_f32x2(mul_f32x2(rsv, fma_f32x2(h[v][i], c2v, add_f32x2(w[v][i], c1v))), o[2 * i], o[2 * i + 1]);
+                stage8<T>(stage + (v * 256 + lane * 8) * static_cast<int>(sizeof(T)), o);
+            }
+            store_span<Ring::BYTES, sizeof(T)>(stage, reinterpret_cast<uint8_t*>(out), warp_have < V * 256 ? warp_have * static_cast<int>(sizeof(T)) : Ring::BYTES);
+        }
+        out += dx_step;
+        x_now += x_step;
+        dy_now += dy_step;
+        if(++slot == STAGE_DEPTH)
+            slot = 0;
+    }
+    copy_async_wait_all();
+    if(P.partial)
+    {
+        float* pg = P.partial + static_cast<int64_t>(blockIdx.x) * P.N;
+        float* pb = pg + static_cast<int64_t>(P.parts) * P.N;
+#pragma unroll
+        for(int v = 0; v < V; ++v)
+#pragma unroll
+            for(int i = 0; i < 8; ++i)
+            {
+                const int c = warp_col + v * 256 + lane * 8 + i;
                 float a[2], b[2];
                 unpack_f32x2(dg[v][i / 2], a[0], a[1]);
                 unpack_f32x2(db[v][i / 2], b[0], b[1]);

@@ -192,7 +192,7 @@ int bwd_parts(const ckb_layernorm_bwd_desc* d)
 template <typename T>
 cudaError_t launch_bwd(LayernormBwdParams p, cudaStream_t stream)
 {
-    cudaError_t e;
+    cudaError_t e   = cudaSuccess;
     const bool sums = p.dgamma || p.dbeta;
     if(p.N > kBwdRegisterCols)
     {
@@ -213,12 +213,21 @@ cudaError_t launch_bwd(LayernormBwdParams p, cudaStream_t stream)
         const int threads = static_cast<int>(div_up(div_up(vecs, V), 32) * 32);
         if(!sums)
             p.partial = nullptr;
-        if(V == 1)
-            e = p.vec ? launch_big<&layernorm_bwd_kernel<T, 1, false>>(p.parts, threads, stream, p, RowRing<T, 2>::bytes(threads))
-                      : launch(layernorm_bwd_kernel<T, 1, true>, p.parts, 1, threads, stream, p);
-        else
-            e = p.vec ? launch_big<&layernorm_bwd_kernel<T, 2, false>>(p.parts, threads, stream, p, RowRing<T, 4>::bytes(threads))
-                      : launch(layernorm_bwd_kernel<T, 2, true>, p.parts, 1, threads, stream, p);
+        // 16-bit rows on 16-byte boundaries as they lie, others shifted out of whole pieces; 32-bit rows the latter way if
+        // they start on such boundaries (vectors of 32 bytes are not in order: 94 against 118 us at 8192 x 4096), others
+        // column by column
+        if constexpr(sizeof(T) == 2)
+        {
+            if(p.vec)
+                e = V == 1 ? launch_big<&layernorm_bwd_kernel<T, 1, false>>(p.parts, threads, stream, p, RowRing<T, 2>::bytes(threads))
+                           : launch_big<&layernorm_bwd_kernel<T, 2, false>>(p.parts, threads, stream, p, RowRing<T, 4>::bytes(threads));
+        }
+        else if(!p.vec)
+            e = V == 1 ? launch(layernorm_bwd_kernel<T, 1, true>, p.parts, 1, threads, stream, p)
+                       : launch(layernorm_bwd_kernel<T, 2, true>, p.parts, 1, threads, stream, p);
+        if((sizeof(T) == 2) != (p.vec != 0))
+            e = V == 1 ? launch_big<&layernorm_bwd_shifted_kernel<T, 1>>(p.parts, threads, stream, p, 2 * WarpRing<T, 256>::bytes(threads))
+                       : launch_big<&layernorm_bwd_shifted_kernel<T, 2>>(p.parts, threads, stream, p, 2 * WarpRing<T, 512>::bytes(threads));
     }
     if(e != cudaSuccess || !sums)
         return e;
@@ -321,7 +330,7 @@ int ckb_layernorm_fwd_run(const ckb_layernorm_fwd_desc* d, void* stream_, int n_
     const int U     = few || (warp && units <= 32) ? 1 : 2;
     p.tpr           = warp ? 32 : lng ? 1024 : static_cast<int>(div_up(div_up(units, U), 32) * 32);
     // parts of a CTA: 768 threads at most, rows and weights within shared memory, and no more than there are rows for
-    const int ring = p.x_vec ? STAGE_DEPTH * U * 2 * 8 * xb * p.tpr : 0, weights = 2 * U * 16 * 4 * p.tpr;
+    const int ring = STAGE_DEPTH * (U * 512 * xb + 16) * (p.tpr / 32), weights = 2 * U * 16 * 4 * p.tpr;
     int parts      = warp ? 8 : 1;
     if(!warp && !wide && !few)
     {
@@ -330,10 +339,10 @@ int ckb_layernorm_fwd_run(const ckb_layernorm_fwd_desc* d, void* stream_, int n_
             ++parts;
     }
     const int threads  = parts * p.tpr;
-    const int smem     = warp || lng || few ? 0 : parts * ring + (wide ? 0 : weights);
+    const int smem     = lng ? 0 : parts * ring + (warp || wide || few ? 0 : weights);
     p.w_offset         = parts * ring;
     const int64_t want = div_up(d->M, parts);
-    const int64_t most = static_cast<int64_t>(dev.sm_count) * (lng ? 2 : warp ? 8 : 1);
+    const int64_t most = static_cast<int64_t>(dev.sm_count) * (lng ? 2 : warp ? 4 : 1);
     const int64_t grid = want < most ? want : most;
     host_note_plan("layernorm_fwd %s threads=%d vectors=%d grid=%lld vec=%d", warp ? "warp" : lng ? "long" : "cta", threads, 2 * U,
                    static_cast<long long>(grid), p.x_vec);
@@ -346,15 +355,12 @@ int ckb_layernorm_fwd_run(const ckb_layernorm_fwd_desc* d, void* stream_, int n_
                 if(lng)
                     return launch(layernorm_fwd_long_kernel<T, E5>, grid, 1, threads, stream, p);
                 if(warp)
-                    return U == 1 ? launch(layernorm_fwd_kernel<T, E5, 1, ROW_WARP, false>, grid, 1, threads, stream, p)
-                                  : launch(layernorm_fwd_kernel<T, E5, 2, ROW_WARP, false>, grid, 1, threads, stream, p);
+                    return U == 1 ? launch_big<&layernorm_fwd_kernel<T, E5, 1, ROW_WARP>>(grid, threads, stream, p, smem)
+                                  : launch_big<&layernorm_fwd_kernel<T, E5, 2, ROW_WARP>>(grid, threads, stream, p, smem);
                 if(few)
-                    return launch(layernorm_fwd_kernel<T, E5, 1, ROW_CTA, false>, grid, 1, threads, stream, p);
-                if(wide)
-                    return p.x_vec ? launch_big<&layernorm_fwd_kernel<T, E5, 2, ROW_CTA, true>>(grid, threads, stream, p, smem)
-                                   : launch(layernorm_fwd_kernel<T, E5, 2, ROW_CTA, false>, grid, 1, threads, stream, p);
-                return p.x_vec ? launch_big<&layernorm_fwd_kernel<T, E5, 2, ROW_GROUP, true>>(grid, threads, stream, p, smem)
-                               : launch_big<&layernorm_fwd_kernel<T, E5, 2, ROW_GROUP, false>>(grid, threads, stream, p, smem);
+                    return launch_big<&layernorm_fwd_kernel<T, E5, 1, ROW_CTA>>(grid, threads, stream, p, smem);
+                return wide ? launch_big<&layernorm_fwd_kernel<T, E5, 2, ROW_CTA>>(grid, threads, stream, p, smem)
+                            : launch_big<&layernorm_fwd_kernel<T, E5, 2, ROW_GROUP>>(grid, threads, stream, p, smem);
             };
             return d->p_q && d->q_dtype == CKB_F8_E5M2 ? both(Flag<true>{}) : both(Flag<false>{});
         });
@@ -400,6 +406,7 @@ int ckb_layernorm_bwd_run(const ckb_layernorm_bwd_desc* d, void* workspace, size
     p.M = d->M, p.N = static_cast<int32_t>(d->N);
     p.parts = bwd_parts(d);
     p.w_f32 = d->w_dtype == CKB_F32;
+    p.w_vec = starts_on(d->p_gamma, 16);
     p.vec   = starts_on(d->p_dy, 16) && starts_on(d->p_x, 16) && starts_on(d->p_dx, 16) && d->lddy * xb % 16 == 0 && d->ldx * xb % 16 == 0 &&
             (!d->p_dx || d->lddx * xb % 16 == 0);
     const bool lng  = d->N > kBwdRegisterCols, sums = d->p_dgamma || d->p_dbeta;
