@@ -203,7 +203,6 @@ int scaled_run(const ScaledProblem& q, void* stream_, int n_rep, float* avg_ms)
     p.sv_row   = swapped ? a_row : b_row;
     p.sv_kb    = swapped ? a_kb : b_kb;
     p.sv_group = swapped ? 0 : b_grp;
-    p.v_shift  = swapped ? a_shift : b_shift;
     p.u_mn      = swapped ? b_mn : a_mn;
     p.v_mn      = swapped ? a_mn : b_mn;
     p.u_batched = rows && swapped;

@@ -46,7 +46,7 @@ struct ScaledParams
     const float *su, *sv;
     int64_t su_row, su_kb, su_group; // elements from one scale to the next: row block, K block, group
     int64_t sv_row, sv_kb, sv_group;
-    int32_t u_shift, v_shift;        // log2 of the rows per scale: 0 or 7
+    int32_t u_shift;                 // log2 of the rows per scale of U: 0 or 7 (V: an instance each)
     void* e;
     int64_t lde, e_group;
     int32_t e_dtype;                 // CKB_F16 / CKB_BF16 / CKB_F32

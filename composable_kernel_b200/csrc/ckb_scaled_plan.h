@@ -144,20 +144,23 @@ struct ScaledPlan
     double cycles;
 };
 
-// Cycles per K block of one CTA (pair): the tensor pipe, the operand bytes through the SM's share of L2, the thread
-// that issues the copies and MMAs, and the epilogue warps (per K block a wait, then chunks of 32 columns).
-inline double scaled_kb_cycles(int cg, int width, int vmode, bool v_mn)
+// Cycles, fitted to timings of pinned tiles (N = K = 4096, 4 to 384 rows; 1.92 GHz): a K block costs its instructions and
+// waits, not its bytes or products, and grows with the width.
+//   per K block   256 x 128 / 192 / 256: 295 / 395 / 444 ns, with a scale per column 440 / - / 643 ns
+//                 128 x 16 / 32 / 64 / 128 (single CTA, a scale per column): 282 / 305 / 406 / 506 ns
+//   per tile      its way out of the registers
+//   K split       handing the parts over: 1.5 us at 16 columns to 5.1 us at 128 between 2 CTAs, a third more between 4;
+//                 clusters beyond the first wave start only when a whole cluster has ended
+inline double scaled_kb_cycles(int cg, int width, int vmode)
 {
-    const double mma   = 2.0 * width;
-    const double bytes = 16384.0 + (v_mn ? 16384.0 : width / cg * 128.0);
-    const int chunks   = (width / 2 + 31) / 32;
-    const double epi   = (vmode == 0 ? 110.0 : 180.0) + chunks * (vmode == 0 ? 75.0 : 115.0);
-    double c           = mma;
-    if(bytes / 68.0 > c)
-        c = bytes / 68.0;
-    if(epi > c)
-        c = epi;
-    return c > 400.0 ? c : 400.0;
+    if(cg == 2)
+        return vmode == 0 ? 280.0 + 2.25 * width : 455.0 + 3.05 * width;
+    return vmode == 0 ? 450.0 + 2.9 * width : 490.0 + 3.9 * width;
+}
+inline double scaled_tile_cycles(int cg, int width) { return cg == 2 ? 600.0 + 10.0 * width : 8.0 * width; }
+inline double scaled_split_cycles(int ksplit, int width)
+{
+    return ksplit == 1 ? 0.0 : (2300.0 + 64.0 * width) * (ksplit == 2 ? 1.0 : 1.3);
 }
 
 constexpr int kScaledWidths[2][4] = {{16, 32, 64, 128}, {128, 192, 224, 256}}; // columns of V per tile, by CTAs per tile
@@ -173,66 +176,66 @@ inline bool plan_scaled(const ScaledPlanInput& in, ScaledPlan* out)
     for(int cg = 1; cg <= 2; ++cg)
     {
         const int swap = cg == 1 ? 1 : 0;
-            for(const int width : kScaledWidths[cg - 1])
-                for(int ks = 1; ks <= (cg == 1 ? 8 : 1); ks *= 2)
+        for(const int width : kScaledWidths[cg - 1])
+            for(int ks = 1; ks <= (cg == 1 ? 8 : 1); ks *= 2)
+            {
+                if((in.cg && in.cg != cg) || (in.cols && in.cols != width) || (in.ksplit ? in.ksplit != ks : in.cols && ks != 1))
+                    continue;
+                const bool v_mn = swap ? in.a_mn : in.b_mn;
+                if(cg == 1 && v_mn && width != 128) // an MN-major tile is 128 columns wide
+                    continue;
+                if(ks > 1 && (in.mode != SCALED_PLAIN || in.num_kb < 2 * ks))
+                    continue;
+                ScaledPlan p;
+                p.cg          = cg;
+                p.t.mode      = in.mode;
+                p.t.swapped   = swap;
+                p.t.u_rows    = 128 * cg;
+                p.t.width     = width;
+                const int64_t eu = swap ? in.N : in.M, ev = swap ? in.M : in.N;
+                p.t.ext_u     = static_cast<int32_t>(eu);
+                p.t.ext_v     = static_cast<int32_t>(ev);
+                const int64_t tu = (eu + p.t.u_rows - 1) / p.t.u_rows, tv = (ev + width - 1) / width;
+                p.t.tiles_u   = static_cast<int32_t>(tu);
+                p.t.tiles_v   = static_cast<int32_t>(tv);
+                p.t.num_kb    = in.num_kb;
+                p.t.groups    = in.groups;
+                p.t.ksplit    = ks;
+                p.t.band      = 8;
+                const int64_t most = in.mode == SCALED_PLAIN ? tu * tv : static_cast<int64_t>(in.groups) * tu * tv;
+                if(most * ks > 0x7fffff00ll || tv * 8 > 0x7fffff00ll)
+                    continue;
+                // tiles there will be: with rows per group unknown, every group with rows has half a tile of waste
+                double tiles = static_cast<double>(most), kb = in.num_kb;
+                int64_t cap  = most;
+                if(rows)
                 {
-                    if((in.cg && in.cg != cg) || (in.cols && in.cols != width) || (in.ksplit ? in.ksplit != ks : in.cols && ks != 1))
-                        continue;
-                    const bool v_mn = swap ? in.a_mn : in.b_mn;
-                    if(cg == 1 && v_mn && width != 128) // an MN-major tile is 128 columns wide
-                        continue;
-                    if(ks > 1 && (in.mode != SCALED_PLAIN || in.num_kb < 2 * ks))
-                        continue;
-                    ScaledPlan p;
-                    p.cg          = cg;
-                    p.t.mode      = in.mode;
-                    p.t.swapped   = swap;
-                    p.t.u_rows    = 128 * cg;
-                    p.t.width     = width;
-                    const int64_t eu = swap ? in.N : in.M, ev = swap ? in.M : in.N;
-                    p.t.ext_u     = static_cast<int32_t>(eu);
-                    p.t.ext_v     = static_cast<int32_t>(ev);
-                    const int64_t tu = (eu + p.t.u_rows - 1) / p.t.u_rows, tv = (ev + width - 1) / width;
-                    p.t.tiles_u   = static_cast<int32_t>(tu);
-                    p.t.tiles_v   = static_cast<int32_t>(tv);
-                    p.t.num_kb    = in.num_kb;
-                    p.t.groups    = in.groups;
-                    p.t.ksplit    = ks;
-                    p.t.band      = 8;
-                    const int64_t most = in.mode == SCALED_PLAIN ? tu * tv : static_cast<int64_t>(in.groups) * tu * tv;
-                    if(most * ks > 0x7fffff00ll || tv * 8 > 0x7fffff00ll)
-                        continue;
-                    // tiles there will be: with rows per group unknown, every group with rows has half a tile of waste
-                    double tiles = static_cast<double>(most), kb = in.num_kb;
-                    int64_t cap  = most;
-                    if(rows)
-                    {
-                        const int64_t own = swap ? width : p.t.u_rows, other = swap ? tu : tv;
-                        const double busy = in.M < in.groups ? static_cast<double>(in.M) : in.groups;
-                        const double mean = in.M / busy;
-                        const double per  = mean <= own / 2 ? 1.0 : mean / own + 0.5;
-                        tiles             = busy * per * other;
-                        cap               = (in.M / own + in.groups) * other; // offsets that do not decrease
-                    }
-                    else if(in.mode == SCALED_GROUP_K)
-                        kb = static_cast<double>(in.num_kb) / in.groups;
-                    p.num_tiles     = static_cast<int>(most);
-                    const int units = cg == 2 ? in.sm_count / 2 : ks == 1 ? in.sm_count : in.cluster_cap[ks == 2 ? 0 : ks == 4 ? 1 : 2];
-                    if(units < 1)
-                        continue;
-                    const int vmode   = scaled_vmode(swap ? in.a_block : in.b_block);
-                    const double per  = scaled_kb_cycles(cg, width, vmode, v_mn);
-                    const double waves = static_cast<double>((static_cast<int64_t>(tiles) + units - 1) / units);
-                    const int n_kb    = static_cast<int>((kb + ks - 1) / ks);
-                    p.cycles          = waves * (n_kb * per + 700.0) + 4000.0 + (ks > 1 ? 900.0 + 12.0 * width : 0.0) + (cg == 2 ? 600.0 : 0.0);
-                    const int64_t want = ks > 1 ? most : (cap < units ? cap : units);
-                    p.grid            = static_cast<int>(want) * (cg == 2 ? 2 : ks);
-                    if(!found || p.cycles < out->cycles)
-                    {
-                        *out  = p;
-                        found = true;
-                    }
+                    const int64_t own = swap ? width : p.t.u_rows, other = swap ? tu : tv;
+                    const double busy = in.M < in.groups ? static_cast<double>(in.M) : in.groups;
+                    const double mean = in.M / busy;
+                    const double per  = mean <= own / 2 ? 1.0 : mean / own + 0.5;
+                    tiles             = busy * per * other;
+                    cap               = (in.M / own + in.groups) * other; // offsets that do not decrease
                 }
+                else if(in.mode == SCALED_GROUP_K)
+                    kb = static_cast<double>(in.num_kb) / in.groups;
+                p.num_tiles = static_cast<int>(most);
+                const int units = cg == 2 ? in.sm_count / 2 : ks == 1 ? in.sm_count : in.cluster_cap[ks == 2 ? 0 : ks == 4 ? 1 : 2];
+                if(units < 1)
+                    continue;
+                const int vmode     = scaled_vmode(swap ? in.a_block : in.b_block);
+                const double per    = scaled_kb_cycles(cg, width, vmode);
+                const int64_t waves = (static_cast<int64_t>(tiles) + units - 1) / units;
+                const int n_kb      = static_cast<int>((kb + ks - 1) / ks);
+                p.cycles            = waves * (n_kb * per + scaled_tile_cycles(cg, width) + scaled_split_cycles(ks, width));
+                const int64_t want  = ks > 1 ? most : (cap < units ? cap : units);
+                p.grid              = static_cast<int>(want) * (cg == 2 ? 2 : ks);
+                if(!found || p.cycles < out->cycles)
+                {
+                    *out  = p;
+                    found = true;
+                }
+            }
     }
     return found;
 }
