@@ -15,6 +15,8 @@
 //   ck_profiler gemm_splitk           <dtype 1> <layout 0..3> <verify> <init> <log> <time> M N K StrideA StrideB StrideC KBatch
 //   ck_profiler conv_fwd              <dtype 1 fp16|2 bf16|3 int8> <layout 1 NHWC> <verify> <init> <log> <time> <nd 1|2|3> N K C
 //                                     <filter> <input> <strides> <dilations> <left pads> <right pads>   (nd values each)
+//   ck_profiler gemm_ab_scale | grouped_gemm_ab_scale | block_quantize | layernorm_fwd | layernorm_bwd
+//                                     (arguments in ck_profiler_block_scale.hpp)
 // gemm takes the reference's four matrix layouts (0: mk_kn, 1: mk_nk, 2: km_kn, 3: km_nk); the fused and grouped
 // sub-commands take layout 1.
 #include <cstring>
@@ -759,10 +761,22 @@ int profile_convnd_fwd(int argc, char* argv[])
     return ok ? 0 : 1;
 }
 
+#include "ck_profiler_block_scale.hpp"
+
 int main(int argc, char* argv[])
 {
     if(argc >= 2)
     {
+        if(std::strcmp(argv[1], "gemm_ab_scale") == 0)
+            return block_scale::profile_product(argc, argv, false);
+        if(std::strcmp(argv[1], "grouped_gemm_ab_scale") == 0)
+            return block_scale::profile_product(argc, argv, true);
+        if(std::strcmp(argv[1], "block_quantize") == 0)
+            return block_scale::profile_block_quantize(argc, argv);
+        if(std::strcmp(argv[1], "layernorm_fwd") == 0)
+            return block_scale::profile_layernorm(argc, argv, false);
+        if(std::strcmp(argv[1], "layernorm_bwd") == 0)
+            return block_scale::profile_layernorm(argc, argv, true);
         if(std::strcmp(argv[1], "gemm") == 0)
             return profile_gemm(argc, argv);
         if(std::strcmp(argv[1], "gemm_add_add_fastgelu") == 0)
@@ -790,6 +804,11 @@ int main(int argc, char* argv[])
                 "                        conv_fwd: ForwardConvolution 1-D / 2-D / 3-D\n"
                 "                        batched_gemm: Batched GEMM\n"
                 "                        gemm_bilinear: GEMM+Bilinear\n"
-                "                        gemm_splitk: Split-K GEMM)\n");
+                "                        gemm_splitk: Split-K GEMM\n"
+                "                        gemm_ab_scale: 8-bit GEMM with block scales\n"
+                "                        grouped_gemm_ab_scale: the same over groups of rows or of K blocks\n"
+                "                        block_quantize: 8-bit blocks with scales\n"
+                "                        layernorm_fwd: Layer norm, to 16 / 32 bits or 8-bit blocks\n"
+                "                        layernorm_bwd: Gradients of layer norm)\n");
     return 0;
 }
