@@ -1165,7 +1165,6 @@ struct LayernormBwdParams
     const float *mean, *rstd;
     void *dx, *dgamma, *dbeta;
     float* partial; // [2][parts][N]: partial sums of dgamma, then of dbeta
-    float* row_sums; // long rows: [2][M] means of w and of w xhat
     int64_t lddy, ldx, lddx;
     int64_t M;
     int32_t N, parts;
@@ -1525,7 +1524,8 @@ __global__ void __launch_bounds__(V == 1 ? 128 : 512, V == 1 ? 4 : 1) layernorm_
     }
 }
 
-// Long rows, first half: means of w and w xhat of a row, then dx (the row is read twice, the second time from L2).
+// Long rows (the column sums of a thread no longer fit its registers), first half: means of w and w xhat of a row, then dx
+// (the row is read twice, the second time from L2).
 template <typename T>
 __global__ void __launch_bounds__(1024) layernorm_bwd_long_kernel(const __grid_constant__ LayernormBwdParams P)
 {
@@ -1535,45 +1535,113 @@ __global__ void __launch_bounds__(1024) layernorm_bwd_long_kernel(const __grid_c
     const float n = static_cast<float>(P.N);
     for(int64_t row = blockIdx.x; row < P.M; row += gridDim.x)
     {
-        const T* x  = static_cast<const T*>(P.x) + row * P.ldx;
-        const T* dy = static_cast<const T*>(P.dy) + row * P.lddy;
-        const float mean = P.mean[row], rstd = P.rstd[row];
-        auto weight = [&](int64_t c) {
-            return !P.gamma ? 1.f : P.w_f32 ? static_cast<const float*>(P.gamma)[c] : to_f32(static_cast<const T*>(P.gamma)[c]);
+        const T* x      = static_cast<const T*>(P.x) + row * P.ldx;
+        const T* dy     = static_cast<const T*>(P.dy) + row * P.lddy;
+        const float rstd = P.rstd[row];
+        const uint64_t rs = pack_f32x2(rstd, rstd), minus_mean = pack_f32x2(-P.mean[row], -P.mean[row]);
+        // w and xhat of eight columns (w = 0 behind the row's end)
+        auto eight = [&](int64_t c, uint64_t (&w)[4], uint64_t (&h)[4]) {
+            const int have = static_cast<int>(P.N - c);
+            Vec8<T> a, b;
+            uint64_t g[4];
+            load8(a, dy + c, have, P.vec != 0);
+            load8(b, x + c, have, P.vec != 0);
+            load_weights8<T>(g, P.gamma, P.w_f32 != 0, static_cast<int>(c), P.N, P.w_vec != 0, 1.f);
+            to_pairs(a, w);
+            to_pairs(b, h);
+#pragma unroll
+            for(int i = 0; i < 4; ++i)
+            {
+                w[i] = mul_f32x2(w[i], g[i]);
+                h[i] = mul_f32x2(add_f32x2(h[i], minus_mean), rs);
+            }
         };
-        float s1 = 0.f, s2 = 0.f;
-        for(int64_t c = threadIdx.x; c < P.N; c += 1024)
+        uint64_t p1 = 0, p2 = 0, w[4], h[4];
+        for(int64_t c = threadIdx.x * 8; c < P.N; c += 8192)
         {
-            const float w = to_f32(dy[c]) * weight(c);
-            s1 += w;
-            s2 = __fmaf_rn(w, (to_f32(x[c]) - mean) * rstd, s2);
+            eight(c, w, h);
+#pragma unroll
+            for(int i = 0; i < 4; ++i)
+            {
+                p1 = add_f32x2(p1, w[i]);
+                p2 = fma_f32x2(w[i], h[i], p2);
+            }
         }
+        float s1 = sum_f32x2(p1), s2 = sum_f32x2(p2);
         row_sum2<ROW_CTA, true>(s1, s2, buf, 0, 1024);
-        const float c1 = s1 / n, c2 = s2 / n;
+        const float c1 = -s1 / n, c2 = -s2 / n;
+        const uint64_t c1v = pack_f32x2(c1, c1), c2v = pack_f32x2(c2, c2);
         T* out = static_cast<T*>(P.dx) + row * P.lddx;
-        for(int64_t c = threadIdx.x; c < P.N; c += 1024)
-            out[c] = from_f32<T>(rstd * (to_f32(dy[c]) * weight(c) - c1 - (to_f32(x[c]) - mean) * rstd * c2));
+        for(int64_t c = threadIdx.x * 8; c < P.N; c += 8192)
+        {
+            eight(c, w, h);
+            float o[8];
+#pragma unroll
+            for(int i = 0; i < 4; ++i)
+                unpack_f32x2(mul_f32x2(rs, fma_f32x2(h[i], c2v, add_f32x2(w[i], c1v))), o[2 * i], o[2 * i + 1]);
+            store8(o, out + c, static_cast<int>(P.N - c), P.vec != 0);
+        }
         __syncthreads();
     }
 }
-// Second half: column sums.  blockIdx.x = 1024 columns, blockIdx.y = one of P.parts sets of rows.
+// Second half: column sums.  blockIdx.x = LONG_SLAB columns, eight a thread, blockIdx.y = one of P.parts sets of rows, two
+// rows in flight.
+constexpr int LONG_SLAB = 2048;
 template <typename T>
-__global__ void __launch_bounds__(1024) layernorm_bwd_long_sums_kernel(const __grid_constant__ LayernormBwdParams P)
+__global__ void __launch_bounds__(LONG_SLAB / 8) layernorm_bwd_long_sums_kernel(const __grid_constant__ LayernormBwdParams P)
 {
     grid_dependency_wait();
     grid_launch_dependents();
-    const int64_t c = static_cast<int64_t>(blockIdx.x) * 1024 + threadIdx.x;
+    const int64_t c = static_cast<int64_t>(blockIdx.x) * LONG_SLAB + threadIdx.x * 8;
     if(c >= P.N)
         return;
-    float dg = 0.f, db = 0.f;
-    for(int64_t row = blockIdx.y; row < P.M; row += P.parts)
+    const int have = static_cast<int>(P.N - c);
+    const T* x     = static_cast<const T*>(P.x) + c;
+    const T* dy    = static_cast<const T*>(P.dy) + c;
+    uint64_t dg[4] = {}, db[4] = {};
+    for(int64_t row = blockIdx.y; row < P.M; row += 2 * P.parts)
     {
-        const float gy = to_f32(static_cast<const T*>(P.dy)[row * P.lddy + c]);
-        dg = __fmaf_rn(gy, (to_f32(static_cast<const T*>(P.x)[row * P.ldx + c]) - __ldg(P.mean + row)) * __ldg(P.rstd + row), dg);
-        db += gy;
+        Vec8<T> a[2], b[2];
+        float mean[2], rstd[2];
+#pragma unroll
+        for(int k = 0; k < 2; ++k)
+        {
+            const int64_t r = row + k * P.parts;
+            const bool on   = r < P.M;
+            mean[k]         = on ? __ldg(P.mean + r) : 0.f;
+            rstd[k]         = on ? __ldg(P.rstd + r) : 0.f;
+            load8(a[k], dy + (on ? r : row) * P.lddy, on ? have : 0, P.vec != 0);
+            load8(b[k], x + (on ? r : row) * P.ldx, on ? have : 0, P.vec != 0);
+        }
+#pragma unroll
+        for(int k = 0; k < 2; ++k)
+        {
+            uint64_t g[4], h[4];
+            to_pairs(a[k], g);
+            to_pairs(b[k], h);
+            const uint64_t rs = pack_f32x2(rstd[k], rstd[k]), minus_mean = pack_f32x2(-mean[k], -mean[k]);
+#pragma unroll
+            for(int i = 0; i < 4; ++i)
+            {
+                dg[i] = fma_f32x2(g[i], mul_f32x2(add_f32x2(h[i], minus_mean), rs), dg[i]);
+                db[i] = add_f32x2(db[i], g[i]);
+            }
+        }
     }
-    P.partial[blockIdx.y * static_cast<int64_t>(P.N) + c]             = dg;
-    P.partial[(P.parts + blockIdx.y) * static_cast<int64_t>(P.N) + c] = db;
+    float* pg = P.partial + blockIdx.y * static_cast<int64_t>(P.N) + c;
+    float* pb = pg + static_cast<int64_t>(P.parts) * P.N;
+#pragma unroll
+    for(int i = 0; i < 8; ++i)
+    {
+        float a[2], b[2];
+        unpack_f32x2(dg[i / 2], a[0], a[1]);
+        unpack_f32x2(db[i / 2], b[0], b[1]);
+        if(i < have)
+        {
+            pg[i] = a[i & 1];
+            pb[i] = b[i & 1];
+        }
+    }
 }
 
 // Sums the partial column sums, always in the same order: 32 columns a CTA, 32 threads a column (thread s takes parts

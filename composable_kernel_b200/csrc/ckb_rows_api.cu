@@ -1,4 +1,5 @@
 // Host side of the block quantizer and of layer norm (ckb_block_quantize_*, ckb_layernorm_*).
+#include <atomic>
 #include <cstring>
 
 #include "ckb_host.h"
@@ -38,7 +39,7 @@ constexpr int kMaxSmem = 220 * 1024; // (the kernels have up to 6 KB besides)
 template <auto KERN, typename P>
 cudaError_t launch_big(int64_t grid_x, int threads, cudaStream_t stream, const P& p, int smem)
 {
-    static bool done[64] = {};
+    static std::atomic<bool> done[64] = {};
     int dev         = 0;
     cudaError_t err = cudaGetDevice(&dev);
     if(err != cudaSuccess)
@@ -181,7 +182,7 @@ int bwd_parts(const ckb_layernorm_bwd_desc* d)
 {
     if(d->N > kBwdRegisterCols)
     {
-        const int64_t slabs = div_up(d->N, 1024);
+        const int64_t slabs = div_up(d->N, LONG_SLAB);
         const int64_t want  = div_up(592, slabs); // 4 CTAs per SM in all
         return static_cast<int>(want < d->M ? (want < 1 ? 1 : want) : d->M);
     }
@@ -204,7 +205,7 @@ cudaError_t launch_bwd(LayernormBwdParams p, cudaStream_t stream)
         }
         if(!sums)
             return cudaSuccess;
-        e = launch(layernorm_bwd_long_sums_kernel<T>, div_up(p.N, 1024), p.parts, 1024, stream, p);
+        e = launch(layernorm_bwd_long_sums_kernel<T>, div_up(p.N, LONG_SLAB), p.parts, LONG_SLAB / 8, stream, p);
     }
     else
     {

@@ -1,5 +1,7 @@
 // Launch of scaled_kernel instances; instantiated in ckb_scaled_inst_*.cu, one file per VMODE and CG.
 #pragma once
+#include <atomic>
+
 #include "ckb_host.h"
 #include "ckb_scaled_kernel.cuh"
 
@@ -11,7 +13,7 @@ cudaError_t launch_scaled_one(const ScaledParams& p, int grid, cudaStream_t stre
     constexpr int SMEM = ScaledSmem<BN, CG>::DYN_BYTES;
     static_assert(SMEM <= 227 * 1024, "pipeline does not fit in shared memory");
     auto kern = scaled_kernel<BN, CG, VMODE>;
-    static bool attr_done[64] = {};
+    static std::atomic<bool> attr_done[64] = {};
     int dev         = 0;
     cudaError_t err = cudaGetDevice(&dev);
     if(err != cudaSuccess)

@@ -314,7 +314,8 @@ int ckb_conv3d_fwd_run(const ckb_conv3d_fwd_desc* desc, void* stream, int n_rep,
  * Layouts as for the plain GEMM, so a layer's three products are all here: forward (A row-major, B column-major, blocks
  * 1 x 128 and 128 x 128), the input's gradient (B row-major) and the weights' gradient (A column-major, B row-major,
  * both with a scale per column and 128 tokens).  M, N and K are arbitrary; base and pitch of A and B are multiples of
- * 16 bytes.  A scale stride may be 0 (one scale for a whole row of blocks or a whole tensor). */
+ * 16 bytes.  A scale stride may be 0 (one scale for a whole row of blocks or a whole tensor).  As everywhere in this
+ * header, outputs overlap neither inputs nor one another. */
 typedef struct ckb_scaled_gemm_desc {
     int32_t a_dtype, b_dtype;    /* CKB_F8_E4M3 / CKB_F8_E5M2                            */
     int32_t e_dtype;             /* CKB_BF16 / CKB_F16 / CKB_F32                          */
