@@ -69,6 +69,81 @@ __device__ __forceinline__ void load8(Vec8<T>& r, const T* p, int n, bool vec)
         r = load8_slow(p, n);
 }
 
+// Eight values that start anywhere, in two steps, so that a thread has the loads of several vectors in flight before it
+// shifts the first one: the 16-byte pieces that hold them (VEC: p is 16-byte aligned, and they are the vector), then the
+// values.  A piece may reach up to 15 bytes beyond the tensor, never beyond the 16-byte granule of its first or last
+// value, so it stays inside the allocation.
+template <typename T, bool VEC>
+struct Raw8
+{
+    static constexpr int WORDS = Vec8<T>::WORDS + (VEC ? 0 : 4);
+    uint32_t w[WORDS];
+};
+template <typename T, bool VEC>
+__device__ __forceinline__ void fetch8(Raw8<T, VEC>& r, const T* p, int n)
+{
+    if constexpr(VEC)
+    {
+        Vec8<T> v;
+        load8(v, p, n, true);
+#pragma unroll
+        for(int i = 0; i < Vec8<T>::WORDS; ++i)
+            r.w[i] = v.w[i];
+    }
+    else
+    {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+        const int off      = static_cast<int>(at & 15);
+        const uint4* s     = reinterpret_cast<const uint4*>(at - off);
+        const int end      = n <= 0 ? 0 : off + (n < 8 ? n : 8) * static_cast<int>(sizeof(T));
+#pragma unroll
+        for(int i = 0; i < Raw8<T, VEC>::WORDS / 4; ++i)
+        {
+            uint4 q = make_uint4(0u, 0u, 0u, 0u);
+            if(i * 16 < end)
+                q = __ldg(s + i);
+            r.w[4 * i] = q.x, r.w[4 * i + 1] = q.y, r.w[4 * i + 2] = q.z, r.w[4 * i + 3] = q.w;
+        }
+    }
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void settle8(Vec8<T>& v, const Raw8<T, VEC>& r, const T* p, int n)
+{
+    constexpr int W = Vec8<T>::WORDS;
+    if constexpr(VEC)
+    {
+#pragma unroll
+        for(int i = 0; i < W; ++i)
+            v.w[i] = r.w[i];
+    }
+    else
+    {
+        const int off = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15);
+        uint32_t a[W + 2], b[W + 1];
+#pragma unroll
+        for(int i = 0; i < W + 2; ++i)
+            a[i] = off & 8 ? r.w[i + 2] : r.w[i];
+#pragma unroll
+        for(int i = 0; i < W + 1; ++i)
+            b[i] = off & 4 ? a[i + 1] : a[i];
+#pragma unroll
+        for(int i = 0; i < W; ++i)
+            v.w[i] = sizeof(T) == 4 ? b[i] : __funnelshift_r(b[i], b[i + 1], (off & 3) * 8);
+        if(n < 8) // values behind the row's end are zeros
+        {
+#pragma unroll
+            for(int i = 0; i < W; ++i)
+            {
+                const int first = sizeof(T) == 4 ? i : 2 * i; // value in the low half of the word
+                if(first >= n)
+                    v.w[i] = 0u;
+                else if(sizeof(T) == 2 && first + 1 >= n)
+                    v.w[i] &= 0xffffu;
+            }
+        }
+    }
+}
+
 // Two values, rounded, in one word (f32: as they are).
 __device__ __forceinline__ uint32_t round_pair(const __half*, float lo, float hi)
 {
@@ -272,6 +347,34 @@ __device__ __forceinline__ void store_q8(uint2 w, uint8_t* p, int n, bool vec)
         store_q8_slow(w, p, n);
 }
 
+// 128 bytes of a block's row, eight from each of 16 lanes, to any address: each lane writes the aligned 8 bytes in which its
+// own ones begin, with the end of its neighbour's; the pieces of less than 8 bytes at both ends are 4, 2 and 1 bytes.
+__device__ __forceinline__ void store_q128(uint2 w, uint8_t* p, int sub)
+{
+    const uint32_t group = 0xffffu << (threadIdx.x & 16);
+    const int off        = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 7);
+    const uint2 before   = make_uint2(__shfl_up_sync(group, w.x, 1, 16), __shfl_up_sync(group, w.y, 1, 16));
+    uint8_t* word        = p - off;
+    const uint64_t own = static_cast<uint64_t>(w.y) << 32 | w.x, prev = static_cast<uint64_t>(before.y) << 32 | before.x;
+    if(sub != 0 || off == 0) // bytes 8 - off .. 15 - off of (prev, own)
+        *reinterpret_cast<uint64_t*>(word) = off == 0 ? own : own << (8 * off) | prev >> (64 - 8 * off);
+    if(off != 0 && (sub == 0 || sub == 15))
+    {
+        // sub 0: bytes off .. 7 of its word; sub 15: bytes 0 .. off - 1 of the one behind its own
+        const int count    = sub == 0 ? 8 - off : off;
+        uint8_t* dst       = sub == 0 ? p : word + 8;
+        const uint64_t src = sub == 0 ? own : own >> (64 - 8 * off);
+        // pieces that end on a boundary come small ones first, pieces that start on one large ones first
+        const int at4 = sub == 0 ? count & 3 : 0, at2 = sub == 0 ? count & 1 : count & 4, at1 = sub == 0 ? 0 : count & 6;
+        if(count & 4)
+            *reinterpret_cast<uint32_t*>(dst + at4) = static_cast<uint32_t>(src >> (8 * at4));
+        if(count & 2)
+            *reinterpret_cast<uint16_t*>(dst + at2) = static_cast<uint16_t>(src >> (8 * at2));
+        if(count & 1)
+            dst[at1] = static_cast<uint8_t>(src >> (8 * at1));
+    }
+}
+
 struct QuantizeParams
 {
     const void* x;
@@ -283,7 +386,6 @@ struct QuantizeParams
     uint32_t div_mul, div_shr; // quotient by blocks_n (see FastDiv); mul = 0: blocks_n = 1
     int32_t total;    // blocks (1 x 128), or tiles of 128 x 128
     int32_t pow2;
-    int32_t x_vec, q_vec;
     float qmax, qmax_recip;
 };
 __device__ __forceinline__ int32_t block_row(const QuantizeParams& p, int32_t b)
@@ -291,9 +393,14 @@ __device__ __forceinline__ int32_t block_row(const QuantizeParams& p, int32_t b)
     return p.div_mul == 0 ? b : static_cast<int32_t>(__umulhi(static_cast<uint32_t>(b), p.div_mul) >> p.div_shr);
 }
 
-// Blocks of 1 x 128: 16 lanes per block, QB blocks per thread in flight.
+// Block quantizer: one read of x, one write of q.  VEC: rows of x start on 16-byte and rows of q on 8-byte boundaries;
+// other rows come in whole pieces (fetch8).
+//
+// Blocks of 1 x 128: 16 lanes per block, QB blocks per thread in flight.  8192 x 4096 bf16: 26.4 us (3.8 TB/s; on the GPU
+// its instructions take as long as its bytes), f32 33.5 us (5.0 TB/s); 8192 x 4097 bf16: 41.7 us, 47.3 with a load per
+// value, 54 with the bytes of q shifted between lanes (store_q128), which costs more here than stores byte by byte.
 constexpr int QB = 4;
-template <typename T, bool E5M2>
+template <typename T, bool E5M2, bool VEC>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const __grid_constant__ QuantizeParams P)
 {
     grid_dependency_wait();
@@ -303,7 +410,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const __grid_constan
     const int unit = threadIdx.x >> 4; // 16 per CTA
     for(int64_t base = static_cast<int64_t>(blockIdx.x) * (16 * QB); base < P.total; base += static_cast<int64_t>(gridDim.x) * (16 * QB))
     {
-        Vec8<T> raw[QB];
+        Raw8<T, VEC> fetched[QB];
         int row[QB], c0[QB], n[QB];
 #pragma unroll
         for(int j = 0; j < QB; ++j)
@@ -313,18 +420,20 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const __grid_constan
             row[j]          = on ? block_row(P, static_cast<int32_t>(b)) : 0;
             c0[j]           = on ? (static_cast<int32_t>(b) - row[j] * P.blocks_n) * 128 + sub * 8 : 0;
             n[j]            = on ? P.N - c0[j] : -1000;
-            load8(raw[j], x + row[j] * P.ldx + c0[j], n[j], P.x_vec != 0);
+            fetch8(fetched[j], x + row[j] * P.ldx + c0[j], n[j]);
         }
 #pragma unroll
         for(int j = 0; j < QB; ++j)
         {
-            const float s = block_scale(max16(max_abs8(raw[j])), P.qmax, P.qmax_recip, P.pow2 != 0);
+            Vec8<T> raw;
+            settle8(raw, fetched[j], x + row[j] * P.ldx + c0[j], n[j]);
+            const float s = block_scale(max16(max_abs8(raw)), P.qmax, P.qmax_recip, P.pow2 != 0);
             if(n[j] <= -1000)
                 continue; // (all 16 lanes of the block)
             uint64_t f[4];
-            to_pairs(raw[j], f);
+            to_pairs(raw, f);
             const uint2 w = quantize8<E5M2>(f, BlockDivisor(s));
-            store_q8(w, P.q + row[j] * P.ldq + c0[j], n[j], P.q_vec != 0);
+            store_q8(w, P.q + row[j] * P.ldq + c0[j], n[j], VEC);
             if(sub == 0)
                 P.scale[row[j] * P.ss_m + (c0[j] >> 7) * P.ss_n] = s;
         }
@@ -332,8 +441,10 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const __grid_constan
 }
 
 // Blocks of 128 x 128 (SQUARE) or 128 x 1: a CTA holds 128 rows x 128 columns in registers, 8 rows x 8 columns a
-// thread.  Row r of the tile belongs to threads 16 (r mod 16) .. + 15.
-template <typename T, bool E5M2, bool SQUARE>
+// thread.  8192 x 4096 bf16: 20.4 us (128 x 128, 4.9 TB/s) and 31.3 (128 x 1: a scale per value to divide by), f32 31.9 and
+// 36.2; 8192 x 4097 bf16: 50 and 57 us, 77 and 98 with a load per value and byte stores, 55 and 73 with byte stores alone.
+// Row r of the tile belongs to threads 16 (r mod 16) .. + 15.
+template <typename T, bool E5M2, bool SQUARE, bool VEC>
 __global__ void __launch_bounds__(256) quantize_tile_kernel(const __grid_constant__ QuantizeParams P)
 {
     grid_dependency_wait();
@@ -347,12 +458,19 @@ __global__ void __launch_bounds__(256) quantize_tile_kernel(const __grid_constan
         const int br = block_row(P, b);
         const int bc = b - br * P.blocks_n;
         const int c0 = bc * 128 + sub * 8, n = P.N - c0;
+        Raw8<T, VEC> fetched[8];
         Vec8<T> raw[8];
 #pragma unroll
         for(int i = 0; i < 8; ++i)
         {
             const int r = br * 128 + i * 16 + unit;
-            load8(raw[i], x + r * P.ldx + c0, r < P.M ? n : 0, P.x_vec != 0);
+            fetch8(fetched[i], x + r * P.ldx + c0, r < P.M ? n : 0);
+        }
+#pragma unroll
+        for(int i = 0; i < 8; ++i)
+        {
+            const int r = br * 128 + i * 16 + unit;
+            settle8(raw[i], fetched[i], x + r * P.ldx + c0, r < P.M ? n : 0);
         }
         uint64_t nscale[4], recip[4]; // of this thread's columns (SQUARE: all the same)
         bool fast = true;
@@ -439,7 +557,10 @@ __global__ void __launch_bounds__(256) quantize_tile_kernel(const __grid_constan
                 }
                 w = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
             }
-            store_q8(w, P.q + r * P.ldq + c0, n, P.q_vec != 0);
+            if(VEC || (c0 | 127) >= P.N)
+                store_q8(w, P.q + r * P.ldq + c0, n, VEC);
+            else
+                store_q128(w, P.q + r * P.ldq + c0, sub);
         }
         __syncthreads(); // s_max is used again
     }
@@ -1526,7 +1647,7 @@ __global__ void __launch_bounds__(V == 1 ? 128 : 512, V == 1 ? 4 : 1) layernorm_
 
 // Long rows (the column sums of a thread no longer fit its registers), first half: means of w and w xhat of a row, then dx
 // (the row is read twice, the second time from L2).
-template <typename T>
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(1024) layernorm_bwd_long_kernel(const __grid_constant__ LayernormBwdParams P)
 {
     grid_dependency_wait();
@@ -1542,10 +1663,13 @@ __global__ void __launch_bounds__(1024) layernorm_bwd_long_kernel(const __grid_c
         // w and xhat of eight columns (w = 0 behind the row's end)
         auto eight = [&](int64_t c, uint64_t (&w)[4], uint64_t (&h)[4]) {
             const int have = static_cast<int>(P.N - c);
+            Raw8<T, VEC> ra, rb;
             Vec8<T> a, b;
             uint64_t g[4];
-            load8(a, dy + c, have, P.vec != 0);
-            load8(b, x + c, have, P.vec != 0);
+            fetch8(ra, dy + c, have);
+            fetch8(rb, x + c, have);
+            settle8(a, ra, dy + c, have);
+            settle8(b, rb, x + c, have);
             load_weights8<T>(g, P.gamma, P.w_f32 != 0, static_cast<int>(c), P.N, P.w_vec != 0, 1.f);
             to_pairs(a, w);
             to_pairs(b, h);
@@ -1587,7 +1711,7 @@ __global__ void __launch_bounds__(1024) layernorm_bwd_long_kernel(const __grid_c
 // Second half: column sums.  blockIdx.x = LONG_SLAB columns, eight a thread, blockIdx.y = one of P.parts sets of rows, two
 // rows in flight.
 constexpr int LONG_SLAB = 2048;
-template <typename T>
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(LONG_SLAB / 8) layernorm_bwd_long_sums_kernel(const __grid_constant__ LayernormBwdParams P)
 {
     grid_dependency_wait();
@@ -1601,7 +1725,7 @@ __global__ void __launch_bounds__(LONG_SLAB / 8) layernorm_bwd_long_sums_kernel(
     uint64_t dg[4] = {}, db[4] = {};
     for(int64_t row = blockIdx.y; row < P.M; row += 2 * P.parts)
     {
-        Vec8<T> a[2], b[2];
+        Raw8<T, VEC> a[2], b[2];
         float mean[2], rstd[2];
 #pragma unroll
         for(int k = 0; k < 2; ++k)
@@ -1610,15 +1734,19 @@ __global__ void __launch_bounds__(LONG_SLAB / 8) layernorm_bwd_long_sums_kernel(
             const bool on   = r < P.M;
             mean[k]         = on ? __ldg(P.mean + r) : 0.f;
             rstd[k]         = on ? __ldg(P.rstd + r) : 0.f;
-            load8(a[k], dy + (on ? r : row) * P.lddy, on ? have : 0, P.vec != 0);
-            load8(b[k], x + (on ? r : row) * P.ldx, on ? have : 0, P.vec != 0);
+            fetch8(a[k], dy + r * P.lddy, on ? have : 0);
+            fetch8(b[k], x + r * P.ldx, on ? have : 0);
         }
 #pragma unroll
         for(int k = 0; k < 2; ++k)
         {
+            const int64_t r = row + k * P.parts;
+            Vec8<T> v;
             uint64_t g[4], h[4];
-            to_pairs(a[k], g);
-            to_pairs(b[k], h);
+            settle8(v, a[k], dy + r * P.lddy, r < P.M ? have : 0);
+            to_pairs(v, g);
+            settle8(v, b[k], x + r * P.ldx, r < P.M ? have : 0);
+            to_pairs(v, h);
             const uint64_t rs = pack_f32x2(rstd[k], rstd[k]), minus_mean = pack_f32x2(-mean[k], -mean[k]);
 #pragma unroll
             for(int i = 0; i < 4; ++i)

@@ -199,13 +199,15 @@ cudaError_t launch_bwd(LayernormBwdParams p, cudaStream_t stream)
     {
         if(p.dx)
         {
-            e = launch(layernorm_bwd_long_kernel<T>, p.M < 296 ? p.M : 296, 1, 1024, stream, p);
+            e = p.vec ? launch(layernorm_bwd_long_kernel<T, true>, p.M < 296 ? p.M : 296, 1, 1024, stream, p)
+                      : launch(layernorm_bwd_long_kernel<T, false>, p.M < 296 ? p.M : 296, 1, 1024, stream, p);
             if(e != cudaSuccess)
                 return e;
         }
         if(!sums)
             return cudaSuccess;
-        e = launch(layernorm_bwd_long_sums_kernel<T>, div_up(p.N, LONG_SLAB), p.parts, LONG_SLAB / 8, stream, p);
+        e = p.vec ? launch(layernorm_bwd_long_sums_kernel<T, true>, div_up(p.N, LONG_SLAB), p.parts, LONG_SLAB / 8, stream, p)
+                  : launch(layernorm_bwd_long_sums_kernel<T, false>, div_up(p.N, LONG_SLAB), p.parts, LONG_SLAB / 8, stream, p);
     }
     else
     {
@@ -268,8 +270,7 @@ int ckb_block_quantize_run(const ckb_block_quantize_desc* d, void* stream_, int 
     }
     p.total = static_cast<int32_t>(div_up(d->M, d->block_m == 1 ? 1 : 128) * p.blocks_n);
     p.pow2  = d->pow2_scale;
-    p.x_vec = starts_on(d->p_x, 16) && d->ldx * xb % 16 == 0;
-    p.q_vec = starts_on(d->p_q, 8) && d->ldq % 8 == 0;
+    const bool vec = starts_on(d->p_x, 16) && d->ldx * xb % 16 == 0 && starts_on(d->p_q, 8) && d->ldq % 8 == 0;
     p.qmax  = qmax_of(d->q_dtype);
     p.qmax_recip = 1.f / p.qmax;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
@@ -277,16 +278,20 @@ int ckb_block_quantize_run(const ckb_block_quantize_desc* d, void* stream_, int 
     const int64_t want = rows ? div_up(p.total, 16 * QB) : p.total;
     const int64_t most = static_cast<int64_t>(dev.sm_count) * (rows ? 8 * 16 : 64);
     const int64_t grid = want < most ? want : most;
-    host_note_plan("block_quantize %dx%d grid=%lld vec=%d/%d", d->block_m, d->block_n, static_cast<long long>(grid), p.x_vec, p.q_vec);
+    host_note_plan("block_quantize %dx%d grid=%lld vec=%d", d->block_m, d->block_n, static_cast<long long>(grid), vec);
     auto once = [&]() {
         return with_type(d->x_dtype, [&](auto t) {
             using T   = decltype(t);
             auto both = [&](auto e5) {
                 constexpr bool E5 = decltype(e5)::value;
-                if(rows)
-                    return launch(quantize_rows_kernel<T, E5>, grid, 1, 256, stream, p);
-                return square ? launch(quantize_tile_kernel<T, E5, true>, grid, 1, 256, stream, p)
-                              : launch(quantize_tile_kernel<T, E5, false>, grid, 1, 256, stream, p);
+                auto aligned      = [&](auto v) {
+                    constexpr bool VEC = decltype(v)::value;
+                    if(rows)
+                        return launch(quantize_rows_kernel<T, E5, VEC>, grid, 1, 256, stream, p);
+                    return square ? launch(quantize_tile_kernel<T, E5, true, VEC>, grid, 1, 256, stream, p)
+                                  : launch(quantize_tile_kernel<T, E5, false, VEC>, grid, 1, 256, stream, p);
+                };
+                return vec ? aligned(Flag<true>{}) : aligned(Flag<false>{});
             };
             return d->q_dtype == CKB_F8_E5M2 ? both(Flag<true>{}) : both(Flag<false>{});
         });

@@ -122,3 +122,19 @@ def test_many_blocks(cuda_device):
     x = torch.randn((5000, 3000), generator=L.gen(5), device="cuda").to(torch.bfloat16)
     for block in BLOCKS:
         check(x, block, ck.CKB_F8_E4M3)
+
+
+@pytest.mark.parametrize("block", BLOCKS)
+@pytest.mark.parametrize("xt", X)
+@pytest.mark.parametrize("N", [1, 7, 127, 128, 129, 264, 389])
+def test_every_alignment_of_rows(cuda_device, block, xt, N):
+    """Rows of x and q that start on every byte their elements allow, full and partial blocks, NaN between the rows."""
+    g = L.gen(N)
+    for pad in (0, 1, 3):
+        ld = N + pad + (N + pad + 1) % 2  # odd: the rows walk through all alignments
+        x = torch.full((150 * ld + 8,), float("nan"), dtype=L.WIDE[xt], device="cuda")
+        for start in (0, 1, 5):
+            v = x[start:start + 150 * ld].view(150, ld)[:, :N]
+            v.copy_(torch.randn((150, N), generator=g, device="cuda"))
+            check(v, block, ck.CKB_F8_E4M3, ldq=ld, q_offset=start)
+            x.fill_(float("nan"))
