@@ -759,36 +759,32 @@ __device__ __forceinline__ void store_span(uint32_t stage, uint8_t* dst, int n)
     }
     else
     {
-        if(n > BYTES)
-            n = BYTES;
-        for(int j = lane; 16 * j - off < n; j += 32)
+        n              = n > BYTES ? BYTES : n < 0 ? 0 : n;
+        const int head = off == 0 ? 0 : n < 16 - off ? n : 16 - off; // bytes before dst's first boundary
+        const int tail = head + ((n - head) & ~15);                  // where the last whole piece ends
+        for(int from = head + lane * 16; from < tail; from += 512)
         {
-            const int from = 16 * j - off; // piece j of dst takes bytes from .. from + 15 of the stage
-            if(from >= 0 && from + 16 <= n)
-            {
-                uint32_t w[4];
-                lds_words(w, stage + (from & ~15), from & 15);
-                *reinterpret_cast<uint4*>(dst + from) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
+            uint32_t w[4];
+            lds_words(w, stage + (from & ~15), from & 15);
+            *reinterpret_cast<uint4*>(dst + from) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        // both ends at once, an element per lane (one lane after the other they took longer than the rest)
+        const int b = (lane & 15) * ELEM + (lane & 16 ? tail : 0);
+        if(b < (lane & 16 ? n : head))
+        {
+            uint32_t v;
+            if constexpr(ELEM == 4)
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(stage + b) : "memory");
+            else if constexpr(ELEM == 2)
+                asm volatile("{.reg .b16 t; ld.shared.b16 t, [%1]; cvt.u32.u16 %0, t;}" : "=r"(v) : "r"(stage + b) : "memory");
             else
-            {
-                for(int b = from < 0 ? 0 : from; b < from + 16 && b < n; b += ELEM)
-                {
-                    uint32_t v;
-                    if constexpr(ELEM == 4)
-                        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(stage + b) : "memory");
-                    else if constexpr(ELEM == 2)
-                        asm volatile("{.reg .b16 t; ld.shared.b16 t, [%1]; cvt.u32.u16 %0, t;}" : "=r"(v) : "r"(stage + b) : "memory");
-                    else
-                        asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(stage + b) : "memory");
-                    if constexpr(ELEM == 4)
-                        *reinterpret_cast<uint32_t*>(dst + b) = v;
-                    else if constexpr(ELEM == 2)
-                        *reinterpret_cast<uint16_t*>(dst + b) = static_cast<uint16_t>(v);
-                    else
-                        dst[b] = static_cast<uint8_t>(v);
-                }
-            }
+                asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(stage + b) : "memory");
+            if constexpr(ELEM == 4)
+                *reinterpret_cast<uint32_t*>(dst + b) = v;
+            else if constexpr(ELEM == 2)
+                *reinterpret_cast<uint16_t*>(dst + b) = static_cast<uint16_t>(v);
+            else
+                dst[b] = static_cast<uint8_t>(v);
         }
     }
     __syncwarp();
@@ -992,6 +988,8 @@ __device__ __forceinline__ float layernorm_q16(const uint64_t (&d)[2][4], float 
 //              (read for every row from L2 they were 2.6 times the bytes of the rows, and their latency most of the time)
 //   ROW_CTA    longer rows, or a row per CTA: the weights from L2
 // Rows come and go through shared memory in 16-byte pieces, in order (WarpRing, store_span).
+// 8192 x 4096 bf16: 43 us (3.1 TB/s), x 4097 60; f32 83 us (3.2 TB/s), x 4097 129; 8192 x 5120 bf16 to 8 bits: 54 us, where
+// the arithmetic of norm and quantizer (about 45 instruction slots per value) takes longer than 126 MB.
 // Mean and variance in two passes over the registers; the second pass also sums the distances themselves, which takes
 // the rounding of the first mean out of both.
 template <typename T, bool E5M2, int U, int KIND>
@@ -1318,8 +1316,10 @@ __device__ __forceinline__ void load_columns(Vec8<T>& r, const T* row, int v, in
 // dx and the partial sums of dgamma and dbeta in one pass.  A CTA walks rows blockIdx.x, + gridDim.x, ...; a thread keeps
 // the same V x 8 columns throughout, so the column sums stay in its registers until the CTA writes them once.  Rows that
 // start on 16-byte boundaries come through shared memory (RowRing), STRIDED ones one ahead in registers.
+// bf16: 8192 x 4096 50 us (4.0 TB/s, 61 % of a copy's rate), x 5120 66 us; f32, STRIDED: 8192 x 4096 96 us (4.2 TB/s),
+// 65536 x 511 103 us.  Few warps, each with a row's chain of loads, sums, a barrier and stores: latency, not bytes.
 template <typename T, int V, bool STRIDED>
-__global__ void __launch_bounds__(V == 1 ? 128 : 512, V == 1 ? 4 : 1) layernorm_bwd_kernel(const __grid_constant__ LayernormBwdParams P)
+__global__ void __launch_bounds__(V == 1 ? 768 : 512, 1) layernorm_bwd_kernel(const __grid_constant__ LayernormBwdParams P)
 {
     grid_dependency_wait();
     grid_launch_dependents();
@@ -1440,7 +1440,7 @@ __global__ void __launch_bounds__(V == 1 ? 128 : 512, V == 1 ? 4 : 1) layernorm_
         if constexpr(STRIDED)
             fetch(0);
         statistics(row + gridDim.x < P.M);
-        row_sum2<ROW_CTA>(s1, s2, buf + flip, 0, tpr);
+        row_sum2<ROW_CTA, V == 1>(s1, s2, buf + flip, 0, tpr); // (one vector a thread: more than 16 warps)
         flip ^= 64;
         if(P.dx)
         {
@@ -1498,10 +1498,10 @@ __global__ void __launch_bounds__(V == 1 ? 128 : 512, V == 1 ? 4 : 1) layernorm_
     }
 }
 
-// The same with rows that come and go through shared memory in whole 16-byte pieces, as in the forward pass, for 16-bit
-// rows that start anywhere (8192 x 4097 in bf16: 122 us, STRIDED 249; with rows on 16-byte boundaries the kernel above takes
-// 50 us for 4096 columns and this one 65) and for 32-bit rows on 16-byte boundaries (8192 x 4096: 94 us, 118 the other way;
-// rows that start anywhere: 167, STRIDED 143).  Vector v of a lane of warp w: columns 256 (w V + v) + 8 lane .. + 7.
+// The same for 16-bit rows that start anywhere: they come and go through shared memory in whole 16-byte pieces, as in the
+// forward pass (8192 x 4097 bf16: 111 us, STRIDED 249; with rows on 16-byte boundaries the kernel above takes 50 us for 4096
+// columns and this one 65).  Bound by its instructions: shifting and the row's ends next to 16 values a lane.
+// Vector v of a lane of warp w: columns 256 (w V + v) + 8 lane .. + 7.
 template <typename T, int V>
 __global__ void __launch_bounds__(V == 1 ? 128 : 512, V == 1 ? 4 : 1) layernorm_bwd_shifted_kernel(const __grid_constant__ LayernormBwdParams P)
 {
@@ -1646,7 +1646,8 @@ __global__ void __launch_bounds__(V == 1 ? 128 : 512, V == 1 ? 4 : 1) layernorm_
 }
 
 // Long rows (the column sums of a thread no longer fit its registers), first half: means of w and w xhat of a row, then dx
-// (the row is read twice, the second time from L2).
+// (the row is read twice, the second time from L2; both halves at 2048 x 16384 bf16: 105 us, 219 with a value per thread and
+// load; x 16383: 192).
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(1024) layernorm_bwd_long_kernel(const __grid_constant__ LayernormBwdParams P)
 {

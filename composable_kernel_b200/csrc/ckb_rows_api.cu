@@ -176,17 +176,34 @@ int check_bwd(const ckb_layernorm_bwd_desc* d, bool need_pointers)
 
 constexpr int kBwdRegisterCols = 8192; // longest row whose column sums fit the registers of a CTA
 
+// Threads of a CTA for one row, each with V vectors of eight columns; `lean`: the kernel gets along with 80 registers at
+// V = 1, so that 768 threads hold a row that would leave less than 16 warps of V = 2 on an SM.
+struct BwdShape
+{
+    int V, threads;
+};
+BwdShape bwd_shape(int64_t N, bool lean)
+{
+    const int vecs = static_cast<int>(div_up(N, 8));
+    const int V    = vecs <= 128 || (lean && vecs > 512 && vecs <= 768) ? 1 : 2;
+    return {V, static_cast<int>(div_up(div_up(vecs, V), 32) * 32)};
+}
+
 // How many sets of rows sum columns on their own; depends on the sizes only, so that the workspace can be asked for
 // before the device is known.
 int bwd_parts(const ckb_layernorm_bwd_desc* d)
 {
+    int64_t want;
     if(d->N > kBwdRegisterCols)
+        want = div_up(592, div_up(d->N, LONG_SLAB)); // 4 CTAs per SM in all
+    else
     {
-        const int64_t slabs = div_up(d->N, LONG_SLAB);
-        const int64_t want  = div_up(592, slabs); // 4 CTAs per SM in all
-        return static_cast<int>(want < d->M ? (want < 1 ? 1 : want) : d->M);
+        // 16 warps per SM; more than 592 CTAs only where each has eight rows (what they sum is read once more)
+        const int warps = bwd_shape(d->N, false).threads / 32; // (one CTA per SM where `lean` matters)
+        want            = 148 * (warps < 16 ? 16 / warps : 1);
+        if(want > 592)
+            want = want < d->M / 8 ? want : d->M / 8 > 592 ? d->M / 8 : 592;
     }
-    const int64_t want = d->N <= 2048 ? 592 : d->N <= 4096 ? 296 : 148;
     return static_cast<int>(want < d->M ? want : d->M);
 }
 
@@ -211,26 +228,22 @@ cudaError_t launch_bwd(LayernormBwdParams p, cudaStream_t stream)
     }
     else
     {
-        const int vecs = static_cast<int>(div_up(p.N, 8));
-        const int V    = vecs <= 128 ? 1 : 2; // 128 threads or more of 16 columns
-        const int threads = static_cast<int>(div_up(div_up(vecs, V), 32) * 32);
         if(!sums)
             p.partial = nullptr;
-        // 16-bit rows on 16-byte boundaries as they lie, others shifted out of whole pieces; 32-bit rows the latter way if
-        // they start on such boundaries (vectors of 32 bytes are not in order: 94 against 118 us at 8192 x 4096), others
-        // column by column
-        if constexpr(sizeof(T) == 2)
-        {
-            if(p.vec)
-                e = V == 1 ? launch_big<&layernorm_bwd_kernel<T, 1, false>>(p.parts, threads, stream, p, RowRing<T, 2>::bytes(threads))
-                           : launch_big<&layernorm_bwd_kernel<T, 2, false>>(p.parts, threads, stream, p, RowRing<T, 4>::bytes(threads));
-        }
-        else if(!p.vec)
-            e = V == 1 ? launch(layernorm_bwd_kernel<T, 1, true>, p.parts, 1, threads, stream, p)
-                       : launch(layernorm_bwd_kernel<T, 2, true>, p.parts, 1, threads, stream, p);
-        if((sizeof(T) == 2) != (p.vec != 0))
-            e = V == 1 ? launch_big<&layernorm_bwd_shifted_kernel<T, 1>>(p.parts, threads, stream, p, 2 * WarpRing<T, 256>::bytes(threads))
-                       : launch_big<&layernorm_bwd_shifted_kernel<T, 2>>(p.parts, threads, stream, p, 2 * WarpRing<T, 512>::bytes(threads));
+        // 16-bit rows on 16-byte boundaries as they lie, others shifted out of whole pieces; 32-bit rows column by column
+        // (8192 x 4096: 96 us, shifted out of pieces 94; x 5120: 119 and 145; x 511: 103, x 512 in vectors 109)
+        const bool lean    = sizeof(T) == 4 || p.vec;
+        const BwdShape s   = bwd_shape(p.N, lean);
+        const int threads  = s.threads;
+        if constexpr(sizeof(T) == 4)
+            e = s.V == 1 ? launch(layernorm_bwd_kernel<T, 1, true>, p.parts, 1, threads, stream, p)
+                         : launch(layernorm_bwd_kernel<T, 2, true>, p.parts, 1, threads, stream, p);
+        else if(p.vec)
+            e = s.V == 1 ? launch_big<&layernorm_bwd_kernel<T, 1, false>>(p.parts, threads, stream, p, RowRing<T, 2>::bytes(threads))
+                         : launch_big<&layernorm_bwd_kernel<T, 2, false>>(p.parts, threads, stream, p, RowRing<T, 4>::bytes(threads));
+        else
+            e = s.V == 1 ? launch_big<&layernorm_bwd_shifted_kernel<T, 1>>(p.parts, threads, stream, p, 2 * WarpRing<T, 256>::bytes(threads))
+                         : launch_big<&layernorm_bwd_shifted_kernel<T, 2>>(p.parts, threads, stream, p, 2 * WarpRing<T, 512>::bytes(threads));
     }
     if(e != cudaSuccess || !sums)
         return e;
