@@ -147,17 +147,18 @@ struct ScaledPlan
 // Cycles, fitted to timings of pinned tiles (N = K = 4096, 4 to 384 rows; 1.92 GHz): a K block costs its instructions and
 // waits, not its bytes or products, and grows with the width.
 //   per K block   256 x 128 / 192 / 256: 295 / 395 / 444 ns, with a scale per column 440 / - / 643 ns
-//                 128 x 16 / 32 / 64 / 128 (single CTA, a scale per column): 282 / 305 / 406 / 506 ns
+//                 128 x 16 / 32 / 64 / 128 (single CTA, a scale per column): 282 / 305 / 406 / 506 ns, a tenth more with
+//                 all SMs at work
 //   per tile      its way out of the registers
 //   K split       handing the parts over: 1.5 us at 16 columns to 5.1 us at 128 between 2 CTAs, a third more between 4;
 //                 clusters beyond the first wave start only when a whole cluster has ended
 inline double scaled_kb_cycles(int cg, int width, int vmode)
 {
     if(cg == 2)
-        return vmode == 0 ? 280.0 + 2.25 * width : 455.0 + 3.05 * width;
-    return vmode == 0 ? 450.0 + 2.9 * width : 490.0 + 3.9 * width;
+        return vmode == 0 ? 280.0 + 2.25 * width : 500.0 + 3.05 * width;
+    return vmode == 0 ? 490.0 + 3.1 * width : 540.0 + 4.1 * width;
 }
-inline double scaled_tile_cycles(int cg, int width) { return cg == 2 ? 600.0 + 10.0 * width : 8.0 * width; }
+inline double scaled_tile_cycles(int cg, int width) { return (cg == 2 ? 10.0 : 8.0) * width; }
 inline double scaled_split_cycles(int ksplit, int width)
 {
     return ksplit == 1 ? 0.0 : (2300.0 + 64.0 * width) * (ksplit == 2 ? 1.0 : 1.3);
