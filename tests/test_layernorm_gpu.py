@@ -284,3 +284,27 @@ def test_gradients_against_differences(cuda_device):
             down = f()
             t[at] = keep
             assert abs((up - down) / (2 * h) - d[at].item()) <= 2e-3
+
+
+# More rows than CTAs, so that a CTA works on several rows side by side and one after the other, at every alignment of rows.
+@pytest.mark.parametrize("xt,wt", TYPES)
+@pytest.mark.parametrize("M,N", [(300, 1025), (1000, 1037), (700, 2050), (450, 4097), (333, 5120), (310, 8191), (300, 8192), (1300, 200), (310, 9001)])
+def test_many_rows_forward(cuda_device, xt, wt, M, N):
+    x, gamma, beta = inputs(M, N, xt, wt, M + N)
+    y, q, sc, mean, rstd = forward(x, gamma, beta, xt, wt, ck.CKB_F8_E4M3, ldy=N + 1 - N % 2, ldq=N + 1)
+    want, m, r, hat = norm64(x, gamma, beta)
+    mean_off, rstd_off = stat_bounds(x, r, N)
+    assert ((mean[:, None].double() - m).abs() <= mean_off + 1e-30).all() and ((rstd[:, None].double() - r).abs() <= rstd_off).all()
+    assert ((y.double() - want).abs() <= y_bound(x, want, gamma, beta, r, hat, mean_off, rstd_off, x.dtype)).all()
+    off = y_bound(x, want, gamma, beta, r, hat, mean_off, rstd_off, torch.float32)
+    s = sc.double()[:, torch.arange(N, device="cuda") // 128]
+    half = torch.finfo(torch.float8_e4m3fn).eps / 2
+    assert ((q.double() * s - want).abs() <= off + half * (want.abs() + off) + s * torch.finfo(torch.float8_e4m3fn).smallest_normal * half).all()
+
+
+@pytest.mark.parametrize("xt,wt", TYPES)
+@pytest.mark.parametrize("M,N", [(700, 5121), (500, 4104), (320, 6144), (400, 6145), (5000, 100), (6000, 257), (900, 513), (400, 12289), (1000, 16400)])
+def test_many_rows_backward(cuda_device, xt, wt, M, N):
+    x, gamma, _ = inputs(M, N, xt, wt, M + N)
+    dy = torch.randn((M, N), generator=L.gen(N), device="cuda").to(x.dtype)
+    check_backward(dy, x, gamma, xt, wt, lddx=N + 1 - N % 2)
