@@ -225,6 +225,8 @@ __device__ __forceinline__ float block_scale(float amax, float qmax, float qmax_
 // q = q0 + (x - q0 scale) r is the rounded quotient (P. Markstein, IBM J. Res. Dev. 34, 1990) as long as neither
 // quotient nor remainder leaves the normal range.  Where a quotient matters to the 8-bit value (>= 2^-18) that holds for
 // scales from 2^-80 to 2^120; other blocks divide.
+// The last step would add the remainder +0 of a zero to it, and -0 would come out as +0.  So the quotient by -scale is
+// formed, whose last step adds (+0)(-r) = -0 and leaves a zero as it is; the sign bits are turned in the 8-bit values.
 struct BlockDivisor
 {
     float scale, recip;
@@ -236,10 +238,12 @@ struct BlockDivisor
             recip = __frcp_rn(s);
     }
 };
-__device__ __forceinline__ uint64_t div_pair(uint64_t x, uint64_t nscale, uint64_t recip)
+constexpr uint32_t F8_SIGNS = 0x80808080u;
+// -(x / scale); minus_recip: -1 / scale
+__device__ __forceinline__ uint64_t minus_quotient(uint64_t x, uint64_t scale, uint64_t minus_recip)
 {
-    const uint64_t q0 = mul_f32x2(x, recip);
-    return fma_f32x2(fma_f32x2(q0, nscale, x), recip, q0);
+    const uint64_t q0 = mul_f32x2(x, minus_recip);
+    return fma_f32x2(fma_f32x2(q0, scale, x), minus_recip, q0);
 }
 
 template <bool E5M2>
@@ -269,15 +273,15 @@ __device__ __forceinline__ uint2 quantize8(const uint64_t (&f)[4], const BlockDi
     if(!d.fast)
         return quantize8_slow<E5M2>(make_ulonglong2(f[0], f[1]), make_ulonglong2(f[2], f[3]), d.scale);
     uint32_t w[4];
-    const uint64_t ns = pack_f32x2(-d.scale, -d.scale), r = pack_f32x2(d.recip, d.recip);
+    const uint64_t s2 = pack_f32x2(d.scale, d.scale), mr = pack_f32x2(-d.recip, -d.recip);
 #pragma unroll
     for(int i = 0; i < 4; ++i)
     {
         float lo, hi;
-        unpack_f32x2(div_pair(f[i], ns, r), lo, hi);
+        unpack_f32x2(minus_quotient(f[i], s2, mr), lo, hi);
         w[i] = to_f8x2<E5M2>(lo, hi);
     }
-    return make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+    return make_uint2((w[0] | w[1] << 16) ^ F8_SIGNS, (w[2] | w[3] << 16) ^ F8_SIGNS);
 }
 
 // The eight values of a vector as pairs, and their largest magnitude.
@@ -472,7 +476,7 @@ __global__ void __launch_bounds__(256) quantize_tile_kernel(const __grid_constan
             const int r = br * 128 + i * 16 + unit;
             settle8(raw[i], fetched[i], x + r * P.ldx + c0, r < P.M ? n : 0);
         }
-        uint64_t nscale[4], recip[4]; // of this thread's columns (SQUARE: all the same)
+        uint64_t scales[4], minus_recip[4]; // of this thread's columns (SQUARE: all the same)
         bool fast = true;
         float scale[8];
         if constexpr(SQUARE)
@@ -522,9 +526,9 @@ __global__ void __launch_bounds__(256) quantize_tile_kernel(const __grid_constan
             for(int k = 0; k < 4; ++k)
             {
                 const BlockDivisor lo(scale[2 * k]), hi(scale[2 * k + 1]);
-                nscale[k] = pack_f32x2(-lo.scale, -hi.scale);
-                recip[k]  = pack_f32x2(lo.recip, hi.recip);
-                fast      = fast && lo.fast && hi.fast;
+                scales[k]      = pack_f32x2(lo.scale, hi.scale);
+                minus_recip[k] = pack_f32x2(-lo.recip, -hi.recip);
+                fast           = fast && lo.fast && hi.fast;
             }
         }
 #pragma unroll
@@ -546,7 +550,7 @@ __global__ void __launch_bounds__(256) quantize_tile_kernel(const __grid_constan
                 {
                     float lo, hi;
                     if(fast)
-                        unpack_f32x2(div_pair(f[k], nscale[k], recip[k]), lo, hi);
+                        unpack_f32x2(minus_quotient(f[k], scales[k], minus_recip[k]), lo, hi);
                     else
                     {
                         unpack_f32x2(f[k], lo, hi);
@@ -555,7 +559,8 @@ __global__ void __launch_bounds__(256) quantize_tile_kernel(const __grid_constan
                     }
                     h[k] = to_f8x2<E5M2>(lo, hi);
                 }
-                w = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+                const uint32_t turn = fast ? F8_SIGNS : 0u;
+                w = make_uint2((h[0] | h[1] << 16) ^ turn, (h[2] | h[3] << 16) ^ turn);
             }
             if(VEC || (c0 | 127) >= P.N)
                 store_q8(w, P.q + r * P.ldq + c0, n, VEC);

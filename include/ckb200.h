@@ -377,7 +377,8 @@ int ckb_scaled_grouped_gemm_run(const ckb_scaled_grouped_gemm_desc* desc, void* 
  * smaller).  With amax = the largest magnitude of a block and qmax = 448 (e4m3) or 57344 (e5m2):
  *   scale = amax / qmax rounded to 32 bits, at least 2^-126; 1 for a block of zeros; with pow2_scale the next power of
  *           two that is not below it
- *   q     = x / scale rounded to the nearest 8-bit value (ties to even), limited to +-qmax
+ *   q     = x / scale rounded to 32 bits, then to the nearest 8-bit value (ties to even), limited to +-qmax; zeros keep
+ *           their sign
  * An infinity makes the scale of its block infinite, a NaN makes it NaN: every value of such a block reads back as NaN.
  * The input is never altered.  q may start anywhere and have any pitch (16-byte ones are faster). */
 typedef struct ckb_block_quantize_desc {
