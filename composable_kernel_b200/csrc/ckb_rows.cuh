@@ -1303,7 +1303,8 @@ __device__ __forceinline__ int column_of(int v, int i, int t, int tpr)
 {
     return STRIDED ? (v * 8 + i) * tpr + t : ((t >> 5) * V + v) * 256 + (t & 31) * 8 + i;
 }
-template <typename T>
+// Columns behind the row's end hold zero, or (REPEAT) its first value.
+template <bool REPEAT, typename T>
 __device__ __forceinline__ void load_columns(Vec8<T>& r, const T* row, int v, int t, int tpr, int N, bool on)
 {
     uint32_t e[8];
@@ -1311,19 +1312,26 @@ __device__ __forceinline__ void load_columns(Vec8<T>& r, const T* row, int v, in
     for(int i = 0; i < 8; ++i)
     {
         const int c = column_of<1, true>(v, i, t, tpr);
-        e[i]        = on && c < N ? bits_of(row[c]) : 0u;
+        e[i]        = on && (REPEAT || c < N) ? bits_of(row[c < N ? c : 0]) : 0u;
     }
 #pragma unroll
     for(int i = 0; i < Vec8<T>::WORDS; ++i)
         r.w[i] = sizeof(T) == 4 ? e[i & 7] : e[(2 * i) & 7] | e[(2 * i + 1) & 7] << 16;
 }
 
+// Behind the row's end dy and gamma are zero, and so is w.  What xhat is there counts nothing as long as it is a number, and
+// -mean * rstd, the xhat of a zero, is none in a row of values next to 1e36 and little else.  So x is one of the row's own
+// values there, or xhat is cut off.
+//
 // dx and the partial sums of dgamma and dbeta in one pass.  A CTA walks rows blockIdx.x, + gridDim.x, ...; a thread keeps
 // the same V x 8 columns throughout, so the column sums stay in its registers until the CTA writes them once.  Rows that
 // start on 16-byte boundaries come through shared memory (RowRing), STRIDED ones one ahead in registers.
-// bf16: 8192 x 4096 50 us (4.0 TB/s, 61 % of a copy's rate), x 5120 66 us; f32, STRIDED: 8192 x 4096 96 us (4.2 TB/s),
-// 65536 x 511 103 us.  Few warps, each with a row's chain of loads, sums, a barrier and stores: latency, not bytes.
-template <typename T, int V, bool STRIDED>
+// bf16: 8192 x 4096 50 us (4.0 TB/s, 61 % of a copy's rate), x 5120 67 us; f32, STRIDED: 8192 x 4096 97 us (4.2 TB/s),
+// 65536 x 511 107 us.  Few warps, each with a row's chain of loads, sums, a barrier and stores: latency, not bytes.
+// TAIL (see above): STRIDED, the threads have more columns than the row, x repeats its first value behind its end (8192 x 4097
+// f32 107 us, 103 without); else, the row ends inside a vector, whose xhat is cut off (in every kernel 2 to 7 % of the time).
+// Without TAIL a thread's vector lies in the row, or is copied from its start.
+template <typename T, int V, bool STRIDED, bool TAIL>
 __global__ void __launch_bounds__(V == 1 ? 768 : 512, 1) layernorm_bwd_kernel(const __grid_constant__ LayernormBwdParams P)
 {
     grid_dependency_wait();
@@ -1359,7 +1367,7 @@ __global__ void __launch_bounds__(V == 1 ? 768 : 512, 1) layernorm_bwd_kernel(co
     float mean = 0.f, rstd = 0.f;
     const int col0 = STRIDED ? 0 : column_of<V, false>(0, 0, t, tpr);
     const int have = P.N - col0; // values of the row from this thread's first column on
-    const T* x_ahead  = x + blockIdx.x * P.ldx + (have > 0 ? col0 : 0); // of the row that is fetched next
+    const T* x_ahead  = x + blockIdx.x * P.ldx; // of the row that is fetched next
     const T* dy_ahead = dy + blockIdx.x * P.lddy + (have > 0 ? col0 : 0);
     const int64_t x_step = gridDim.x * P.ldx, dy_step = gridDim.x * P.lddy;
     int64_t ahead_row = blockIdx.x;
@@ -1370,12 +1378,15 @@ __global__ void __launch_bounds__(V == 1 ? 768 : 512, 1) layernorm_bwd_kernel(co
         {
             if constexpr(STRIDED)
             {
-                load_columns<T>(rx[v], x_ahead, v, t, tpr, P.N, on);
-                load_columns<T>(ry[v], dy_ahead, v, t, tpr, P.N, on);
+                load_columns<TAIL>(rx[v], x_ahead, v, t, tpr, P.N, on);
+                load_columns<false>(ry[v], dy_ahead, v, t, tpr, P.N, on);
             }
             else if(on)
             {
-                ring.copy(slot, v, x_ahead + v * 256, have - v * 256);
+                if constexpr(TAIL)
+                    ring.copy(slot, v, x_ahead + (have > 0 ? col0 : 0) + v * 256, have - v * 256);
+                else
+                    ring.copy(slot, v, x_ahead + (have > v * 256 ? col0 + v * 256 : 0), 8);
                 ring.copy(slot, V + v, dy_ahead + v * 256, have - v * 256);
             }
         }
@@ -1431,7 +1442,8 @@ __global__ void __launch_bounds__(V == 1 ? 768 : 512, 1) layernorm_bwd_kernel(co
                 h[v][i] = mul_f32x2(add_f32x2(h[v][i], m2), r2);
                 w[v][i] = mul_f32x2(gy[i], g[v][i]);
             }
-            // (behind the row's end dy and gamma are zero, and so is all that xhat is multiplied with)
+            if(!STRIDED && TAIL && have - v * 256 < 8)
+                keep_first(h[v], have - v * 256);
 #pragma unroll
             for(int i = 0; i < 4; ++i)
             {
@@ -1584,16 +1596,17 @@ __global__ void __launch_bounds__(V == 1 ? 128 : 512, V == 1 ? 4 : 1) layernorm_
             uint64_t gy[4];
             to_pairs(rx, h[v]);
             to_pairs(ry, gy);
+#pragma unroll
+            for(int i = 0; i < 4; ++i)
+                h[v][i] = mul_f32x2(add_f32x2(h[v][i], m2), r2);
             if(have - v * 256 < 8)
             {
                 keep_first(h[v], have - v * 256); // (what lies behind the row's end was never copied)
                 keep_first(gy, have - v * 256);
             }
-            // (behind the row's end dy and gamma are zero, and so is all that xhat is multiplied with)
 #pragma unroll
             for(int i = 0; i < 4; ++i)
             {
-                h[v][i]  = mul_f32x2(add_f32x2(h[v][i], m2), r2);
                 w[v][i]  = mul_f32x2(gy[i], g[v][i]);
                 dg[v][i] = fma_f32x2(gy[i], h[v][i], dg[v][i]);
                 db[v][i] = add_f32x2(db[v][i], gy[i]);
@@ -1685,6 +1698,8 @@ __global__ void __launch_bounds__(1024) layernorm_bwd_long_kernel(const __grid_c
                 w[i] = mul_f32x2(w[i], g[i]);
                 h[i] = mul_f32x2(add_f32x2(h[i], minus_mean), rs);
             }
+            if(have < 8)
+                keep_first(h, have);
         };
         uint64_t p1 = 0, p2 = 0, w[4], h[4];
         for(int64_t c = threadIdx.x * 8; c < P.N; c += 8192)

@@ -231,17 +231,25 @@ cudaError_t launch_bwd(LayernormBwdParams p, cudaStream_t stream)
         if(!sums)
             p.partial = nullptr;
         // 16-bit rows on 16-byte boundaries as they lie, others shifted out of whole pieces; 32-bit rows column by column
-        // (8192 x 4096: 96 us, shifted out of pieces 94; x 5120: 119 and 145; x 511: 103, x 512 in vectors 109)
+        // (8192 x 4096: 96 us, shifted out of pieces 94; x 5120: 119 and 145; x 511: 107, x 512 in vectors 109)
         const bool lean    = sizeof(T) == 4 || p.vec;
         const BwdShape s   = bwd_shape(p.N, lean);
         const int threads  = s.threads;
-        if constexpr(sizeof(T) == 4)
-            e = s.V == 1 ? launch(layernorm_bwd_kernel<T, 1, true>, p.parts, 1, threads, stream, p)
-                         : launch(layernorm_bwd_kernel<T, 2, true>, p.parts, 1, threads, stream, p);
-        else if(p.vec)
-            e = s.V == 1 ? launch_big<&layernorm_bwd_kernel<T, 1, false>>(p.parts, threads, stream, p, RowRing<T, 2>::bytes(threads))
-                         : launch_big<&layernorm_bwd_kernel<T, 2, false>>(p.parts, threads, stream, p, RowRing<T, 4>::bytes(threads));
-        else
+        auto aligned       = [&](auto v, auto tail) {
+            constexpr int V     = decltype(v)::value;
+            constexpr bool TAIL = decltype(tail)::value;
+            if constexpr(sizeof(T) == 4)
+                return launch(layernorm_bwd_kernel<T, V, true, TAIL>, p.parts, 1, threads, stream, p);
+            else
+                return launch_big<&layernorm_bwd_kernel<T, V, false, TAIL>>(p.parts, threads, stream, p, RowRing<T, 2 * V>::bytes(threads));
+        };
+        auto either = [&](auto v) {
+            const bool tail = sizeof(T) == 4 ? p.N < 8 * s.V * threads : p.N % 8 != 0;
+            return tail ? aligned(v, std::true_type{}) : aligned(v, std::false_type{});
+        };
+        if(lean)
+            e = s.V == 1 ? either(std::integral_constant<int, 1>{}) : either(std::integral_constant<int, 2>{});
+        else if constexpr(sizeof(T) == 2)
             e = s.V == 1 ? launch_big<&layernorm_bwd_shifted_kernel<T, 1>>(p.parts, threads, stream, p, 2 * WarpRing<T, 256>::bytes(threads))
                          : launch_big<&layernorm_bwd_shifted_kernel<T, 2>>(p.parts, threads, stream, p, 2 * WarpRing<T, 512>::bytes(threads));
     }
