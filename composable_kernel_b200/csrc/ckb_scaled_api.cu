@@ -1,4 +1,5 @@
 // Host side of the 8-bit products with block scales (ckb_scaled_gemm_*, ckb_scaled_grouped_gemm_*).
+#include <cstdlib>
 #include <cstring>
 #include <mutex>
 
@@ -75,6 +76,15 @@ int check_scaled(const ScaledProblem& q, bool need_pointers)
             return host_fail(CKB_ERR_INVALID, "scales, offsets or E not aligned to their elements");
     }
     return CKB_OK;
+}
+
+// Test hook: CKB_TEST_SCALED_WAIT_EXTRA makes barriers of the products wait for one arrival more than will ever come, so that
+// (with a short CKB_WAIT_LIMIT_MS) waits run out while copies and MMAs are on their way.  Bit 0: the scales' barriers, bit
+// 1: those that say that a K block was multiplied; bit 2 / 3: only in even / odd CTAs (the first / second one of a pair).
+uint32_t scaled_test_wait()
+{
+    const char* s = getenv("CKB_TEST_SCALED_WAIT_EXTRA");
+    return s ? static_cast<uint32_t>(atoi(s)) & 15u : 0u;
 }
 
 // Clusters of 2 / 4 / 8 CTAs that the device holds at once, asked once per device (only the cost estimate uses it).
@@ -220,6 +230,7 @@ int scaled_run(const ScaledProblem& q, void* stream_, int n_rep, float* avg_ms)
     p.offsets       = q.offsets;
     p.wait_limit_ns = dev.wait_limit_ns;
     p.status        = dev.status;
+    p.test_wait     = scaled_test_wait();
     const int vmode = scaled_vmode(swapped ? d.scale_block_m : d.scale_block_n);
     auto* fn        = plan.cg == 1 ? (vmode == 0 ? &launch_scaled<0, 1> : &launch_scaled<1, 1>)
                                    : (vmode == 0 ? &launch_scaled<0, 2> : &launch_scaled<1, 2>);

@@ -34,7 +34,8 @@
 // weights 131-137 us (6.8 TB/s).  Bound by the instructions of the epilogue warps per K block (tensor pipe 46 % active), the
 // decode forms by launch, fill and hand-over, the grouped ones of few rows by the bytes of the weights.
 //
-// Every wait is bounded as in ckb_kernel.cuh; after a wait gave up all roles drain and leave.
+// Every wait is bounded as in ckb_kernel.cuh; after a wait gave up all roles leave their loops, and what is still on its way is
+// waited for behind the barrier of the exit.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -61,6 +62,7 @@ struct ScaledParams
     int32_t u_mn, v_mn;              // operand is MN-major
     int32_t u_batched, v_batched;    // operand has a third dimension: the group
     int32_t v_box_rows;              // rows of a K-major V box
+    uint32_t test_wait;              // test hook, 0 in use (see scaled_test_wait)
     uint32_t idesc;
     const int32_t* offsets;
     uint64_t wait_limit_ns;
@@ -76,13 +78,29 @@ struct ScaledParams
 // instructions but not time (424; the loops no longer fit the instruction caches: 365 against 282 at BN = 16).
 constexpr int SCALED_EPI_WARP0 = 4;
 
+// Words of shared memory beside the barriers
+enum
+{
+    MISC_TMEM,       // base address of the tensor memory
+    MISC_ABORT,      // a wait of this CTA gave up
+    MISC_COPY_DRAIN, // the wait for copies at the exit gave up
+    MISC_TILES,      // number of tiles (GROUP_ROWS)
+    MISC_MMA_DRAIN,  // the wait for MMAs at the exit gave up
+    MISC_PEER_ABORT, // a wait of the pair's other CTA gave up
+    MISC_LOADS,      // [CTA of the pair] stages that its producer filled
+    MISC_RELEASES = MISC_LOADS + 2, // [CTA of the pair][epilogue warp] accumulators that it released (~0: for every stage)
+    MISC_WORDS    = MISC_RELEASES + 2 * 8
+};
+
 template <int BN, int CG>
 struct ScaledSmem
 {
     static constexpr int EPI_WARPS   = 8;
     static constexpr int THREADS     = 32 * (SCALED_EPI_WARP0 + EPI_WARPS);
     static constexpr bool SPLIT_REGS = BN >= 128;
-    static constexpr int REGS_LOW = BN == 128 ? 72 : 56, REGS_HIGH = BN == 128 ? 216 : 224;
+    // (224 columns with a scale each: 2048 x 2688 x 4096 takes 59 us with 224 registers, which spill, 52.5 with 232; 256 columns
+    // spill with 40 registers in the first warpgroup)
+    static constexpr int REGS_LOW = BN == 128 ? 72 : BN == 224 ? 40 : 56, REGS_HIGH = BN == 128 ? 216 : BN == 224 ? 232 : 224;
     static_assert(REGS_LOW + 2 * REGS_HIGH == 3 * 168, "the shares add up to what the block is launched with");
     static constexpr int U_BYTES     = 128 * BK_BYTES;
     // (a pair's CTA always has room for 128 rows: an MN-major box is that wide whatever the tile)
@@ -109,7 +127,7 @@ struct ScaledSmem
     // full[STAGES], done[STAGES], scale_full[SLOTS], scale_empty[SLOTS], drain
     static constexpr int NUM_BARS    = 2 * STAGES + 2 * SLOTS + 1;
     static constexpr int MISC_OFFSET = BAR_OFFSET + NUM_BARS * 8;
-    static constexpr int TOTAL       = MISC_OFFSET + 16;
+    static constexpr int TOTAL       = MISC_OFFSET + MISC_WORDS * 4;
     static constexpr int DYN_BYTES   = TOTAL + 1024; // slack to align the base to 1024 B
 };
 
@@ -320,7 +338,6 @@ __global__ void __launch_bounds__(ScaledSmem<BN, CG>::THREADS, 1) scaled_kernel(
     const uint32_t drain_bar = bar_base + 8u * (2 * STAGES + 2 * SLOTS);
     float* scale_ring        = reinterpret_cast<float*>(smem + L::SCALE_OFFSET);
     volatile uint32_t* misc  = reinterpret_cast<volatile uint32_t*>(smem + L::MISC_OFFSET);
-    // misc[0] = TMEM base address, misc[1] = abort flag, misc[2] = constant 0, misc[3] = number of tiles (GROUP_ROWS)
     int32_t* grp_start = reinterpret_cast<int32_t*>(smem + L::GRP_OFFSET);
     int32_t* grp_row0  = grp_start + CKB_SCALED_MAX_GROUPS + 4;
     int32_t* grp_row1  = grp_row0 + CKB_SCALED_MAX_GROUPS;
@@ -332,36 +349,63 @@ __global__ void __launch_bounds__(ScaledSmem<BN, CG>::THREADS, 1) scaled_kernel(
     const bool is_leader     = CG == 1 || cta_rank == 0;
     const int unit           = static_cast<int>(blockIdx.x) / (CG == 2 ? 2 : ksplit);
 
+    // What the exit has to know about both CTAs of a pair goes to the leader.
+    auto tell_leader = [&](int word, uint32_t v) {
+        if constexpr(CG == 2)
+            st_cluster_u32(mapa_shared(base_addr + L::MISC_OFFSET + 4u * word, 0), v);
+        else
+            misc[word] = v;
+    };
+    // Barrier of the whole CTA (pair: the leader's MMAs and both producers' copies reach into the other CTA until the end).
+    auto exit_barrier = [&]() {
+        __syncwarp();
+        if constexpr(CG == 2)
+            cluster_sync_all();
+        else
+            asm volatile("bar.sync 0;" ::: "memory"); // (warps come to it at two places)
+    };
+    // The barrier behind which no role is in its loop any more; true if a wait gave up (the same answer in both CTAs of a pair).
+    auto roles_left = [&]() -> bool {
+        tc_fence_before_sync();
+        exit_barrier();
+        return misc[MISC_ABORT] != 0 || (CG == 2 && misc[MISC_PEER_ABORT] != 0);
+    };
+    auto gave_up = [&]() { // by each role whose wait gave up; MISC_ABORT is set already
+        if constexpr(CG == 2)
+            if(lane == 0)
+                st_cluster_u32(mapa_shared(base_addr + L::MISC_OFFSET + 4u * MISC_PEER_ABORT, cluster_ctarank() ^ 1u), 1u);
+    };
+
     if(threadIdx.x == 0)
     {
+        const uint32_t only = P.test_wait >> 2, hook = only == 0 || (only >> (blockIdx.x & 1) & 1) ? P.test_wait & 3u : 0u;
         for(int s = 0; s < STAGES; ++s)
         {
             // the (leader's) producer arrival, all bytes of the stage, and the release of the accumulator that the K block
             // will use: one arrival per epilogue warp (of both CTAs)
             mbar_init(full_bar(s), 1 + EPI_WARPS * CG);
-            mbar_init(done_bar(s), 1); // one tcgen05.commit arrival
+            mbar_init(done_bar(s), 1 + (hook >> 1)); // one tcgen05.commit arrival
         }
         for(int s = 0; s < SLOTS; ++s)
         {
-            mbar_init(scale_full_bar(s), 64); // one arrival per lane of the two scale warps
+            mbar_init(scale_full_bar(s), 64 + (hook & 1u)); // one arrival per lane of the two scale warps
             mbar_init(scale_empty_bar(s), EPI_WARPS);
         }
         mbar_init(drain_bar, 1);
-        misc[1] = 0;
-        misc[2] = 0;
-        misc[3] = 0;
         fence_mbar_init();
     }
+    if(threadIdx.x != MISC_TMEM && threadIdx.x < MISC_WORDS)
+        misc[threadIdx.x] = threadIdx.x < MISC_RELEASES ? 0u : ~0u;
     if(warp == 1)
     {
         if constexpr(CG == 2)
         {
-            tmem_alloc_pair(smem_u32(const_cast<uint32_t*>(&misc[0])), ACC_COLS);
+            tmem_alloc_pair(smem_u32(const_cast<uint32_t*>(&misc[MISC_TMEM])), ACC_COLS);
             tmem_relinquish_pair();
         }
         else
         {
-            tmem_alloc(smem_u32(const_cast<uint32_t*>(&misc[0])), ACC_COLS);
+            tmem_alloc(smem_u32(const_cast<uint32_t*>(&misc[MISC_TMEM])), ACC_COLS);
             tmem_relinquish();
         }
     }
@@ -371,7 +415,7 @@ __global__ void __launch_bounds__(ScaledSmem<BN, CG>::THREADS, 1) scaled_kernel(
     else
         __syncthreads();
     tc_fence_after_sync();
-    const uint32_t tmem_base = misc[0];
+    const uint32_t tmem_base = misc[MISC_TMEM];
     grid_dependency_wait();
     grid_launch_dependents();
 
@@ -405,11 +449,11 @@ __global__ void __launch_bounds__(ScaledSmem<BN, CG>::THREADS, 1) scaled_kernel(
             if(lane == 0)
             {
                 grp_start[P.tiles.groups] = total;
-                misc[3]                   = static_cast<uint32_t>(total);
+                misc[MISC_TILES]          = static_cast<uint32_t>(total);
             }
         }
         __syncthreads();
-        num_tiles = static_cast<int>(misc[3]);
+        num_tiles = static_cast<int>(misc[MISC_TILES]);
     }
     auto item_of = [&](int t) -> ScaledItem {
         if(P.tiles.mode == SCALED_GROUP_ROWS)
@@ -426,7 +470,7 @@ __global__ void __launch_bounds__(ScaledSmem<BN, CG>::THREADS, 1) scaled_kernel(
         return it;
     };
 
-    WaitCtx wc{&misc[1], P.wait_limit_ns, P.status};
+    WaitCtx wc{&misc[MISC_ABORT], P.wait_limit_ns, P.status};
     constexpr int NUM_ACC = L::NUM_ACC;
 
     if(warp < SCALED_EPI_WARP0)
@@ -492,15 +536,46 @@ __global__ void __launch_bounds__(ScaledSmem<BN, CG>::THREADS, 1) scaled_kernel(
                 }
             }
         }
-        // Do not leave while a bulk copy may still write shared memory (see ckb_kernel.cuh).
-        if(is_leader && lane == 0)
-            for(int s = 0; s < STAGES && s < loads; ++s)
-            {
-                const int last_fill = ((loads - 1 - s) / STAGES) * STAGES + s;
-                WaitCtx drain{&misc[2], kDrainLimitNs, P.status};
-                bounded_wait(full_bar(s), static_cast<uint32_t>(last_fill / STAGES) & 1u, drain, WAIT_DRAIN);
-            }
+        if(lane == 0)
+            tell_leader(MISC_LOADS + pair_rank, static_cast<uint32_t>(loads));
+        if(!ok)
+            gave_up();
         __syncwarp();
+        if(CG == 1 && ksplit > 1)
+            cluster_sync_all(); // (the one before the slices are summed)
+        // Do not leave while a bulk copy may still write shared memory.  Where no wait gave up, every stage has been
+        // multiplied, so every byte has come.  Otherwise stages may be filled whose barriers lack more than bytes: releases of
+        // epilogue warps that are gone, or the part of the CTA whose producer stopped first.  All roles have left their
+        // loops, so what is missing is known: it is made up for here, and then the barriers depend on the copies alone.  A
+        // stage is filled again only after its last K block was multiplied, so only the last STAGES fills can be
+        // incomplete, each on a barrier of its own.
+        // (Here and not in the common exit, where its registers would count in every role: 2 to 15 % of the time.)
+        if(roles_left())
+        {
+            if(is_leader && lane == 0)
+            {
+                const uint32_t own = misc[MISC_LOADS], other = CG == 2 ? misc[MISC_LOADS + 1] : own;
+                const uint32_t most = own > other ? own : other, first = most > STAGES ? most - STAGES : 0u;
+#pragma unroll 1
+                for(uint32_t i = first; i < most; ++i)
+                {
+                    const uint32_t bar = full_bar(i % STAGES);
+                    if(i >= own)
+                        mbar_arrive_expect_tx(bar, stage_tx / CG); // only the other CTA's copies are on their way
+                    else if(i >= other)
+                        mbar_complete_tx(bar, stage_tx / CG); // only this CTA's are
+#pragma unroll 1
+                    for(int w = 0; w < CG * EPI_WARPS; ++w)
+                        if(misc[MISC_RELEASES + w] <= i)
+                            mbar_arrive(bar);
+                }
+                WaitCtx drain{&misc[MISC_COPY_DRAIN], kDrainLimitNs, P.status};
+#pragma unroll 1
+                for(uint32_t i = first; i < most; ++i)
+                    bounded_wait(full_bar(i % STAGES), (i / STAGES) & 1u, drain, WAIT_DRAIN);
+            }
+            exit_barrier();
+        }
     }
     else if(warp == 1)
     {
@@ -557,6 +632,8 @@ __global__ void __launch_bounds__(ScaledSmem<BN, CG>::THREADS, 1) scaled_kernel(
                     }
                 }
             }
+            if(!ok)
+                gave_up();
             // Every MMA issued must be finished before the tensor memory is freed.
             if(issued_any)
             {
@@ -568,7 +645,7 @@ __global__ void __launch_bounds__(ScaledSmem<BN, CG>::THREADS, 1) scaled_kernel(
                         mma_commit(drain_bar);
                 }
                 __syncwarp();
-                WaitCtx drain{&misc[2], kDrainLimitNs, P.status};
+                WaitCtx drain{&misc[MISC_MMA_DRAIN], kDrainLimitNs, P.status};
                 bounded_wait(drain_bar, 0, drain, WAIT_DRAIN);
             }
         }
@@ -640,6 +717,8 @@ __global__ void __launch_bounds__(ScaledSmem<BN, CG>::THREADS, 1) scaled_kernel(
                 }
             }
         }
+        if(!ok)
+            gave_up();
         copy_async_wait_all(); // nothing may land in shared memory after the exit
         __syncwarp();
     }
@@ -672,7 +751,7 @@ __global__ void __launch_bounds__(ScaledSmem<BN, CG>::THREADS, 1) scaled_kernel(
         uint8_t* out_tile     = smem + L::OUT_OFFSET + (warp - SCALED_EPI_WARP0) * 2048;
         uint64_t acc[COLS / 2];
         int stage = 0, slot = 0, buf = 0;
-        uint32_t phase = 0, slot_phase = 0;
+        uint32_t round = 0, slot_phase = 0; // round: of the ring of stages
         bool ok = true;
         for(int t = unit; ok && t < num_tiles; t += P.num_units)
         {
@@ -715,7 +794,7 @@ __global__ void __launch_bounds__(ScaledSmem<BN, CG>::THREADS, 1) scaled_kernel(
                         su2[k]         = pack_f32x2(su, su);
                     }
                 }
-                ok = ok && block_wait(done_bar(stage), phase, wc, WAIT_TMEM_FULL);
+                ok = ok && block_wait(done_bar(stage), round & 1u, wc, WAIT_TMEM_FULL);
                 ok = __all_sync(0xffffffffu, ok);
                 if(!ok)
                     break;
@@ -827,7 +906,7 @@ __global__ void __launch_bounds__(ScaledSmem<BN, CG>::THREADS, 1) scaled_kernel(
                 if(++stage == STAGES)
                 {
                     stage = 0;
-                    phase ^= 1u;
+                    ++round;
                 }
             }
             if(!ok)
@@ -867,12 +946,20 @@ __global__ void __launch_bounds__(ScaledSmem<BN, CG>::THREADS, 1) scaled_kernel(
             else
                 store(static_cast<float*>(P.e));
         }
+        if(!ok)
+        {
+            if(lane == 0)
+                tell_leader(MISC_RELEASES + (CG == 2 ? cluster_ctarank() * EPI_WARPS : 0) + warp - SCALED_EPI_WARP0, round * STAGES + stage + NUM_ACC);
+            gave_up();
+        }
+        __syncwarp();
     }
 
     if(CG == 1 && ksplit > 1)
     {
-        cluster_sync_all(); // every slice is at its owner (release / acquire at cluster scope)
-        if(warp >= SCALED_EPI_WARP0 && misc[1] == 0 && unit < num_tiles)
+        if(warp != 0) // (the producer has been there)
+            cluster_sync_all(); // every slice is at its owner (release / acquire at cluster scope)
+        if(warp >= SCALED_EPI_WARP0 && misc[MISC_ABORT] == 0 && unit < num_tiles)
         {
             const ScaledItem it = item_of(unit);
             const int t = static_cast<int>(threadIdx.x) - 32 * SCALED_EPI_WARP0, row = t & 127;
@@ -890,11 +977,8 @@ __global__ void __launch_bounds__(ScaledSmem<BN, CG>::THREADS, 1) scaled_kernel(
     }
 
     // ---------------------------------------------------------------------- common exit
-    tc_fence_before_sync();
-    if constexpr(CG == 2)
-        cluster_sync_all(); // the leader's MMAs read the peer's shared memory until the very end
-    else
-        __syncthreads();
+    if(warp != 0 && roles_left()) // (the producer has been there)
+        exit_barrier();
     tc_fence_after_sync();
     if(warp == 1)
     {
