@@ -103,6 +103,20 @@ struct DeviceInfo
 DeviceInfo g_dev[64];
 std::mutex g_dev_mutex;
 
+// A process that may use only part of the GPU (an MPS active-thread percentage, a green context) says so
+// with CKB_SM_LIMIT: the K-split plans let units wait for one another, so every unit of a launch has to be
+// resident at the same time, and the runtime reports the whole device whatever the partition is.
+int limited_sms(int sm_count)
+{
+    if(const char* lim = getenv("CKB_SM_LIMIT"))
+    {
+        const int n = atoi(lim) & ~1;
+        if(n >= 2 && n < sm_count)
+            return n;
+    }
+    return sm_count;
+}
+
 int current_device(DeviceInfo** out)
 {
     int dev = 0;
@@ -116,15 +130,7 @@ int current_device(DeviceInfo** out)
         cudaDeviceProp prop;
         CKB_CUDA(cudaGetDeviceProperties(&prop, dev));
         d.sm_count = prop.multiProcessorCount;
-        // A process that may use only part of the GPU (an MPS active-thread percentage, a green context) says so
-        // with CKB_SM_LIMIT: the K-split plans let units wait for one another, so every unit of a launch has to be
-        // resident at the same time, and the runtime reports the whole device whatever the partition is.
-        if(const char* lim = getenv("CKB_SM_LIMIT"))
-        {
-            const int n = atoi(lim) & ~1;
-            if(n >= 2 && n < d.sm_count)
-                d.sm_count = n;
-        }
+        d.sm_count = limited_sms(d.sm_count);
         d.cc_major = prop.major;
         d.cc_minor = prop.minor;
         if(prop.major != 10)
@@ -667,6 +673,8 @@ int host_device(HostDevice* out)
     out->wait_limit_ns = wait_limit_ns();
     return CKB_OK;
 }
+
+int host_limited_sms(int sm_count) { return limited_sms(sm_count); }
 
 int host_check_pointer(const void* p, const char* what)
 {

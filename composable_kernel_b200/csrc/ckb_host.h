@@ -20,6 +20,9 @@ struct HostDevice
 };
 int host_device(HostDevice* out);
 
+// The SMs that a process may use of a device with `sm_count` of them (CKB_SM_LIMIT).
+int host_limited_sms(int sm_count);
+
 // Refuses a pointer that kernels of the current device cannot read: host memory, or memory of another device.
 // nullptr passes (optional tensors).
 int host_check_pointer(const void* p, const char* what);

@@ -87,7 +87,8 @@ uint32_t scaled_test_wait()
     return s ? static_cast<uint32_t>(atoi(s)) & 15u : 0u;
 }
 
-// Clusters of 2 / 4 / 8 CTAs that the device holds at once, asked once per device (only the cost estimate uses it).
+// Clusters of 2 / 4 / 8 CTAs that the device (the part that CKB_SM_LIMIT leaves of it) holds at once, asked once per device:
+// what the planner reckons with, and a K split over a cluster that does not fit (0) is not made.
 int cluster_caps(const HostDevice& dev, int (&cap)[3])
 {
     static std::mutex mutex;
@@ -99,20 +100,22 @@ int cluster_caps(const HostDevice& dev, int (&cap)[3])
     std::lock_guard<std::mutex> lock(mutex);
     if(!asked[ordinal])
     {
+        bool all = true;
         for(int i = 0; i < 3; ++i)
         {
             ScaledParams p;
             memset(&p, 0, sizeof(p));
-            int n = 0;
+            const int limit = dev.sm_count / (2 << i);
+            int n           = 0;
             if(launch_scaled<0, 1>(128, p, (2 << i) * 64, nullptr, 2 << i, &n) != cudaSuccess)
             {
-                cudaGetLastError();
-                n = 0;
+                cudaGetLastError(); // not an answer: as many as there are SMs for, and the next call asks again
+                n   = limit;
+                all = false;
             }
-            const int limit   = dev.sm_count / (2 << i);
             known[ordinal][i] = n < limit ? n : limit;
         }
-        asked[ordinal] = true;
+        asked[ordinal] = all;
     }
     for(int i = 0; i < 3; ++i)
         cap[i] = known[ordinal][i];
@@ -150,9 +153,14 @@ int scaled_supported(const ScaledProblem& q)
 {
     if(int rc = check_scaled(q, false))
         return rc;
+    // a whole B200, or the part that CKB_SM_LIMIT leaves of it (the run asks the device, which this call does not need)
     ScaledPlan plan;
-    const int cap[3] = {64, 32, 16};
-    if(!plan_problem(q, 148, cap, &plan))
+    const int sms = host_limited_sms(148);
+    int cap[3]    = {64, 32, 16};
+    for(int i = 0; i < 3; ++i)
+        if(cap[i] > sms / (2 << i))
+            cap[i] = sms / (2 << i);
+    if(!plan_problem(q, sms, cap, &plan))
         return host_fail(CKB_ERR_UNSUPPORTED, "no tile fits: too many tiles, or a pinned tile that the problem cannot use");
     return CKB_OK;
 }
