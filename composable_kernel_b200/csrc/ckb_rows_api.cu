@@ -1,6 +1,7 @@
 // Host side of the block quantizer and of layer norm (ckb_block_quantize_*, ckb_layernorm_*).
 #include <atomic>
 #include <cstring>
+#include <numeric>
 
 #include "ckb_host.h"
 #include "ckb_rows.cuh"
@@ -81,6 +82,18 @@ int check_pointers(const Used (&used)[N])
     return CKB_OK;
 }
 
+// Whether two of the m x n blocks share a scale at strides sm and sn (none negative), which would be a race: the smallest step
+// that leads from one scale to the same one is sn / gcd blocks down and sm / gcd back.
+bool scales_collide(int64_t sm, int64_t sn, int64_t m, int64_t n)
+{
+    if(m <= 1 && n <= 1)
+        return false;
+    if(m <= 1 || n <= 1)
+        return (m <= 1 ? sn : sm) == 0;
+    const int64_t g = std::gcd(sm, sn);
+    return g == 0 || (sn / g < m && sm / g < n);
+}
+
 // ---- block quantizer ------------------------------------------------------------------------------
 int check_quantize(const ckb_block_quantize_desc* d, bool need_pointers)
 {
@@ -99,9 +112,7 @@ int check_quantize(const ckb_block_quantize_desc* d, bool need_pointers)
     const int64_t blocks = div_up(d->M, d->block_m == 1 ? 1 : 128) * div_up(d->N, 128);
     if(blocks > 0x7fffffffll)
         return host_fail(CKB_ERR_UNSUPPORTED, "more than 2^31 blocks");
-    // several blocks on one scale would be a race
-    const int64_t bm = div_up(d->M, d->block_m), bn = div_up(d->N, d->block_n);
-    if((bm > 1 && d->scale_stride_m == 0) || (bn > 1 && d->scale_stride_n == 0))
+    if(scales_collide(d->scale_stride_m, d->scale_stride_n, div_up(d->M, d->block_m), div_up(d->N, d->block_n)))
         return host_fail(CKB_ERR_INVALID, "every block needs a scale of its own");
     if(need_pointers)
     {
@@ -139,7 +150,7 @@ int check_fwd(const ckb_layernorm_fwd_desc* d, bool need_pointers)
             return host_fail(CKB_ERR_UNSUPPORTED, "8-bit output is CKB_F8_E4M3 or CKB_F8_E5M2");
         if(!d->p_q_scale)
             return host_fail(CKB_ERR_INVALID, "8-bit output needs a tensor of scales");
-        if(d->q_scale_stride_m < 0 || d->q_scale_stride_n < 0 || (d->M > 1 && d->q_scale_stride_m == 0) || (d->N > 128 && d->q_scale_stride_n == 0))
+        if(d->q_scale_stride_m < 0 || d->q_scale_stride_n < 0 || scales_collide(d->q_scale_stride_m, d->q_scale_stride_n, d->M, div_up(d->N, 128)))
             return host_fail(CKB_ERR_INVALID, "every block needs a scale of its own");
     }
     if(need_pointers)

@@ -380,6 +380,7 @@ int ckb_scaled_grouped_gemm_run(const ckb_scaled_grouped_gemm_desc* desc, void* 
  *   q     = x / scale rounded to 32 bits, then to the nearest 8-bit value (ties to even), limited to +-qmax; zeros keep
  *           their sign
  * An infinity makes the scale of its block infinite, a NaN makes it NaN: every value of such a block reads back as NaN.
+ * The scale strides give every block a scale of its own (no two blocks one place): others are refused.
  * The input is never altered.  q may start anywhere and have any pitch (16-byte ones are faster). */
 typedef struct ckb_block_quantize_desc {
     int32_t x_dtype;             /* CKB_BF16 / CKB_F16 / CKB_F32                          */
