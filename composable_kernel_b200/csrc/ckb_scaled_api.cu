@@ -58,7 +58,8 @@ int check_scaled(const ScaledProblem& q, bool need_pointers)
             if(q.b_group < 0 || q.b_group % 16 != 0 || q.b_group >= (1ll << 40) || q.b_scale_group < 0)
                 return host_fail(CKB_ERR_INVALID, "b_group_stride must be a multiple of 16, no group stride negative");
         }
-        else if(q.e_group < 0 || (q.groups > 1 && q.e_group < (d.M - 1) * d.lde + d.N))
+        // (a division, because the size of a matrix may pass 64 bits)
+        else if(q.e_group < 0 || (q.groups > 1 && (q.e_group < d.N || (q.e_group - d.N) / d.lde < d.M - 1)))
             return host_fail(CKB_ERR_INVALID, "e_group_stride is smaller than a matrix of E");
     }
     const int cols = d.tile_config & 0xFFF, cg = (d.tile_config >> 12) & 0xF, ks = (d.tile_config >> 20) & 0xF;
