@@ -460,13 +460,7 @@ __global__ void __launch_bounds__(ScaledSmem<BN, CG>::THREADS, 1) scaled_kernel(
             return scaled_group_item(P.tiles, t, grp_start, grp_row0, grp_row1);
         ScaledItem it = scaled_item(P.tiles, t, P.offsets);
         if(CG == 1 && ksplit > 1)
-        {
-            // slice `rank` of the K blocks, lengths differing by one at most
-            const int n = it.kb1 - it.kb0, r = static_cast<int>(cta_rank);
-            const int a = it.kb0 + static_cast<int>(static_cast<int64_t>(n) * r / ksplit);
-            it.kb1      = it.kb0 + static_cast<int>(static_cast<int64_t>(n) * (r + 1) / ksplit);
-            it.kb0      = a;
-        }
+            scaled_slice(&it, static_cast<int>(cta_rank), ksplit);
         return it;
     };
 

@@ -93,6 +93,15 @@ CKB_SP_HD ScaledItem scaled_item(const ScaledTiles& p, int32_t t, const int32_t*
     return it;
 }
 
+// Slice `rank` of a tile's K blocks (of `ksplit`): in order, lengths that differ by one at most.
+CKB_SP_HD void scaled_slice(ScaledItem* it, int rank, int ksplit)
+{
+    const int32_t first = it->kb0;
+    const int64_t n     = it->kb1 - first;
+    it->kb0             = first + static_cast<int32_t>(n * rank / ksplit);
+    it->kb1             = first + static_cast<int32_t>(n * (rank + 1) / ksplit);
+}
+
 // Item of tile t of a GROUP_ROWS problem.  starts[g] = tiles before group g (starts[groups] = all of them),
 // row0[g] / row1[g] = its rows.
 CKB_SP_HD ScaledItem scaled_group_item(const ScaledTiles& p, int32_t t, const int32_t* starts, const int32_t* row0,
