@@ -182,13 +182,11 @@ __device__ __forceinline__ uint32_t out_piece(int row, int c) { return row * 64 
 // Writes one pass (columns n0 .. n0 + 64 bytes of the warp's COLS columns) to E.  `dst` is this lane's first piece: row
 // lane / 4, columns n0 + (lane % 4) * PER; rows: how many of the warp's 32 rows exist, cols: columns from n0 on that do.
 // `whole`: all of them, in 16-byte pieces.
-template <typename T, int LEFT>
+template <typename T>
 __device__ __forceinline__ void store_pass(const uint8_t* tile, T* dst, int64_t lde8, int rows, int cols, bool vec, bool whole, int lane)
 {
     constexpr int PER = 16 / sizeof(T); // values of a piece
     const int c = lane & 3, n = c * PER;
-    if(LEFT < 4 * PER && n >= LEFT) // (the tile's columns end inside the pass)
-        return;
 #pragma unroll
     for(int i = 0; i < 4; ++i, dst += lde8)
     {
@@ -265,7 +263,7 @@ __device__ __forceinline__ void store_rows(const uint64_t (&acc)[COLS / 2], uint
                 }
         }
         __syncwarp();
-        store_pass<T, (COLS - PASS < 0 ? COLS : PASS)>(tile, dst + n0, lde8, rows, cols - n0 < COLS - n0 ? cols - n0 : COLS - n0, vec, whole && n0 + PASS <= COLS, lane);
+        store_pass<T>(tile, dst + n0, lde8, rows, cols - n0 < COLS - n0 ? cols - n0 : COLS - n0, vec, whole && n0 + PASS <= COLS, lane);
     }
 }
 
