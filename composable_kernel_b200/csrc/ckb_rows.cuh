@@ -400,9 +400,10 @@ __device__ __forceinline__ int32_t block_row(const QuantizeParams& p, int32_t b)
 // Block quantizer: one read of x, one write of q.  VEC: rows of x start on 16-byte and rows of q on 8-byte boundaries;
 // other rows come in whole pieces (fetch8).
 //
-// Blocks of 1 x 128: 16 lanes per block, QB blocks per thread in flight.  8192 x 4096 bf16: 26.4 us (3.8 TB/s; on the GPU
-// its instructions take as long as its bytes), f32 33.5 us (5.0 TB/s); 8192 x 4097 bf16: 41.7 us, 47.3 with a load per
-// value, 54 with the bytes of q shifted between lanes (store_q128), which costs more here than stores byte by byte.
+// Blocks of 1 x 128: 16 lanes per block, QB blocks per thread in flight.  8192 x 4096 bf16: 27.5 us (3.7 TB/s), bound by its
+// instructions: 20 per value, 71 % of the issue slots at 45 % of the warps; f32 33.9 us (5.0 TB/s); 8192 x 4097 bf16: 42.5 us,
+// 47.3 with a load per value, 54 with the bytes of q shifted between lanes (store_q128), which costs more here than stores byte
+// by byte.
 constexpr int QB = 4;
 template <typename T, bool E5M2, bool VEC>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const __grid_constant__ QuantizeParams P)
@@ -445,8 +446,9 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const __grid_constan
 }
 
 // Blocks of 128 x 128 (SQUARE) or 128 x 1: a CTA holds 128 rows x 128 columns in registers, 8 rows x 8 columns a
-// thread.  8192 x 4096 bf16: 20.4 us (128 x 128, 4.9 TB/s) and 31.3 (128 x 1: a scale per value to divide by), f32 31.9 and
-// 36.2; 8192 x 4097 bf16: 50 and 57 us, 77 and 98 with a load per value and byte stores, 55 and 73 with byte stores alone.
+// thread.  8192 x 4096 bf16: 22.0 us (128 x 128, 4.6 TB/s) and 33.0 (128 x 1: a scale per value to divide by, 117 registers
+// and with them 16 warps per SM, 42 % of the issue slots), f32 32.5 and 36.9; 8192 x 4097 bf16: 52 and 59 us, 77 and 98 with a
+// load per value and byte stores, 55 and 73 with byte stores alone.
 // Row r of the tile belongs to threads 16 (r mod 16) .. + 15.
 template <typename T, bool E5M2, bool SQUARE, bool VEC>
 __global__ void __launch_bounds__(256) quantize_tile_kernel(const __grid_constant__ QuantizeParams P)
@@ -993,8 +995,10 @@ __device__ __forceinline__ float layernorm_q16(const uint64_t (&d)[2][4], float 
 //              (read for every row from L2 they were 2.6 times the bytes of the rows, and their latency most of the time)
 //   ROW_CTA    longer rows, or a row per CTA: the weights from L2
 // Rows come and go through shared memory in 16-byte pieces, in order (WarpRing, store_span).
-// 8192 x 4096 bf16: 43 us (3.1 TB/s), x 4097 60; f32 83 us (3.2 TB/s), x 4097 129; 8192 x 5120 bf16 to 8 bits: 54 us, where
-// the arithmetic of norm and quantizer (about 45 instruction slots per value) takes longer than 126 MB.
+// 8192 x 4096 bf16: 43 us (3.1 TB/s), x 4097 61; f32 83 us (3.2 TB/s), x 4097 130; 8192 x 5120 bf16 to 8 bits: 53 us.  Neither
+// DRAM (21 to 31 %) nor the issue slots (25 to 60 %) are full: norm and quantizer take 26 instructions per value, 30 us at full
+// issue.  Each part of a CTA takes its row through one chain - two sums with a barrier each, the weights, the way out through
+// shared memory - and 12 to 24 warps are all that overlap.
 // Mean and variance in two passes over the registers; the second pass also sums the distances themselves, which takes
 // the rounding of the first mean out of both.
 template <typename T, bool E5M2, int U, int KIND>
@@ -1193,6 +1197,7 @@ __global__ void __launch_bounds__(KIND == ROW_WARP ? 256 : KIND == ROW_GROUP ? 7
 }
 
 // Rows that do not fit the registers of a CTA: the row is read three times (the second and third time from L2).
+// 1024 x 32768 bf16: 82 us.  Rows off 16-byte boundaries are loaded and stored value by value: x 32767 280 us.
 template <typename T, bool E5M2>
 __global__ void __launch_bounds__(1024) layernorm_fwd_long_kernel(const __grid_constant__ LayernormFwdParams P)
 {

@@ -29,10 +29,13 @@
 // pushes its sums to the CTA that owns the columns (st.shared::cluster), a cluster barrier, and the owners add the
 // slices in slice order (deterministic) and store.
 //
-// Measured: 3840 x 4096 x 4096 to bf16 72-83 us (1.8-1.55 PFLOP/s, the slower under the power cap), 11008 x 4096 x 8190 with
-// a scale per column on both sides to f32 460-540 us, 4 x 4096 x 4096 7.8 us, 64 groups with 4 rows each and 4096 x 4096
-// weights 131-137 us (6.8 TB/s).  Bound by the instructions of the epilogue warps per K block (tensor pipe 46 % active), the
-// decode forms by launch, fill and hand-over, the grouped ones of few rows by the bytes of the weights.
+// Measured: 3840 x 4096 x 4096 to bf16 69-76 us back to back (1.7-1.87 PFLOP/s, SM clock 1.8-1.965 GHz; the fp16 product of the
+// same size in the same run 74-79 us on small whole numbers, 90-93 on normal ones), 84 us among other passes; 11008 x 4096 x 8190 with a scale per column on
+// both sides to f32 480-555 us, the longer the hotter; 4 x 4096 x 4096 8.5 us; 64 groups of 4 rows each with 4096 x 4096
+// weights 170 us (6.3 TB/s), 247 rows spread over 64 groups at random 124-150 us (41 to 57 groups have rows, and the weights of
+// the others are not read).  The large products are bound by the chain that each epilogue warp goes through per K block (wait,
+// scales, tensor-memory load, wait, release): tensor pipe 46 % and issue slots 44 % active, neither full.  The decode forms are
+// bound by launch, fill and hand-over, the grouped ones of few rows by the bytes of the weights.
 //
 // Every wait is bounded as in ckb_kernel.cuh; after a wait gave up all roles leave their loops, and what is still on its way is
 // waited for behind the barrier of the exit.
@@ -72,10 +75,11 @@ struct ScaledParams
 // Warps 0-3 (producer, MMA issuer, two for the scales) form one warpgroup, the epilogue warps two more, so that registers
 // can be dealt out unevenly: 128 sums per lane (BN = 256) next to a chunk of 32 accumulator columns, addresses and scales
 // do not fit the 168 that twelve warps get at launch, and spills in the first warpgroup cost as much as in the others.
-// What the K loop of an epilogue warp costs is instructions, not arithmetic: about 190 per K block for 64 packed
-// multiply-adds, 5 cycles each.  Sixteen warps with a quarter of the columns each repeat the hand-overs of eight (511
-// against 436 ns per K block of a 256 x 256 tile), and groups of four K blocks unrolled with fixed stages save
-// instructions but not time (424; the loops no longer fit the instruction caches: 365 against 282 at BN = 16).
+// What the K loop of an epilogue warp costs is its chain of hand-overs, about 190 instructions per K block around 64 packed
+// multiply-adds, in which every warp goes through every K block.  Sixteen warps with a quarter of the columns each repeat the
+// hand-overs of eight (511 against 436 ns per K block of a 256 x 256 tile), and groups of four K blocks unrolled with fixed
+// stages save instructions but not time (424; the loops no longer fit the instruction caches: 365 against 282 at BN = 16).
+// Fewer hand-overs per warp (sets of warps that take K blocks in turn) were not tried.
 constexpr int SCALED_EPI_WARP0 = 4;
 
 // Words of shared memory beside the barriers

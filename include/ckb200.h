@@ -310,7 +310,8 @@ int ckb_conv3d_fwd_run(const ckb_conv3d_fwd_desc* desc, void* stream, int n_rep,
  *                                        sum over k in kb of A[m,k] * B[k,n]
  * A and B hold 8-bit floats (e4m3 or e5m2, each its own), SA and SB 32-bit scales, E is bf16, f16 or f32.  Products
  * and sums of a block are 32-bit on the tensor cores; the scaled blocks are added in 32 bits and E is rounded once.
- * (The pair of scales is multiplied first: scales whose product is subnormal lose bits.)
+ * (The pair of scales is multiplied first: scales whose product is subnormal lose bits, and where it passes the largest
+ * 32-bit number the result is no number or infinite, whatever the block's sum.)
  * Layouts as for the plain GEMM, so a layer's three products are all here: forward (A row-major, B column-major, blocks
  * 1 x 128 and 128 x 128), the input's gradient (B row-major) and the weights' gradient (A column-major, B row-major,
  * both with a scale per column and 128 tokens).  M, N and K are arbitrary; base and pitch of A and B are multiples of
@@ -404,7 +405,9 @@ int ckb_block_quantize_run(const ckb_block_quantize_desc* desc, void* stream, in
  *   mean = sum x / N,  rstd = 1 / sqrt(sum (x - mean)^2 / N + eps),  y = (x - mean) * rstd * gamma + beta
  * Y is written as x_dtype (p_y) and (or) as 8-bit blocks of 1 x 128 of the unrounded y (p_q, p_q_scale, as the block
  * quantizer makes them); at least one of the two.  gamma and beta (w_dtype: x_dtype or CKB_F32) may be null (1 and 0),
- * p_mean and p_rstd (M 32-bit values each) may be null. */
+ * p_mean and p_rstd (M 32-bit values each) may be null.
+ * The sums are 32-bit too: a row whose sum of x or of (x - mean)^2 passes the largest 32-bit number does not follow the
+ * formulas.  A row with an infinity or a NaN is NaN throughout; other rows are not touched by it. */
 typedef struct ckb_layernorm_fwd_desc {
     int32_t x_dtype;             /* CKB_BF16 / CKB_F16 / CKB_F32                          */
     int32_t w_dtype;             /* x_dtype or CKB_F32                                    */
